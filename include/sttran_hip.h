@@ -42,7 +42,8 @@ enum {
 };
 
 enum { STTRAN_MODE_PREDCLS = 0, STTRAN_MODE_SGCLS = 1, STTRAN_MODE_SGDET = 2 };
-enum { STTRAN_DTYPE_F32 = 0, STTRAN_DTYPE_I64 = 1, STTRAN_DTYPE_I32 = 2 };
+enum { STTRAN_DTYPE_F32 = 0, STTRAN_DTYPE_I64 = 1, STTRAN_DTYPE_I32 = 2,
+       STTRAN_DTYPE_BF16 = 3 /* the sequence operators only */ };
 /* STTRAN: lib/sttran.py::STTran.  DSG_DETR: lib/dsg_detr.py::STTran (same fusion front-end and heads;
  * stock encoder layers per frame and per object-class sequence; sgdet mode only). */
 enum { STTRAN_MODEL_STTRAN = 0, STTRAN_MODEL_DSG_DETR = 1 };
@@ -298,6 +299,108 @@ int sttran_objcls_select(const SttranObjclsSelect* args, int64_t* num_boxes_out,
  * out [P,C,pooled,pooled]; device pointers; enqueue only. */
 int sttran_roi_align(const float* fmaps, int32_t T, int32_t C, int32_t H, int32_t W, const float* rois, int64_t num_rois,
                      int32_t pooled, float spatial_scale, int32_t sampling_ratio, float* out, void* stream);
+
+/* Sequence operators: the pieces of a relation-transformer layer that sttran_forward does not offer by themselves -- training
+ * (gradients, dropout: the reference trains its layers with nn.MultiheadAttention + dropout 0.1, lib/transformer.py:20-30, 49-58), longer
+ * clips (rotary positions, order and prefix masks, distance bias) and clips that grow token by token.  No handle: device
+ * pointers on the current device, enqueue only, no allocation; every call may be captured into a HIP graph.
+ * Element type: STTRAN_DTYPE_F32 or STTRAN_DTYPE_BF16 for all of q, k, v, outputs and gradients of a call.  Strides are in
+ * elements and >= 0; the head dim's stride is 1.  A row stride is at most 2^24 bytes.
+ *
+ * sttran_attention_forward: attention over packed sequences.  q [q_rows, num_q_heads, head_dim], k / v [kv_rows, num_kv_heads,
+ * head_dim]; sequence s owns query rows seq_off[s] .. seq_off[s+1] and key rows key_off[s] .. key_off[s+1] (both ascending,
+ * int32, on the device); query head h reads key head h / (num_q_heads / num_kv_heads).  The place of query row i of a sequence
+ * with lq queries and lk keys is i + lk - lq (the newest query stands at the newest key).  A row sees its own sequence's keys;
+ * with `causal` those at j <= place, and always those at j < prefix_len[s].
+ *   z = score_cap * tanh(scale * q.k / score_cap) - distance_slope[h] * |place - j|     (no cap: scale * q.k)
+ *   out = softmax(z) v;  rows that see nothing, or belong to no sequence, become zeros.
+ * What a mask hides does not reach a result, infinities and NaN included.  Offsets are device data: they are clamped to the
+ * tensors, never checked.
+ * For a later backward: lse [num_q_heads, q_rows] fp32 (base-2 log-sums, private), and for bfloat16 out_residual like out (what
+ * the rounding of out took away).
+ * sttran_attention_backward: dq [q_rows, num_q_heads, head_dim], dk, dv [kv_rows, num_kv_heads, head_dim], contiguous, from dout
+ * and the forward's inputs, out, out_residual and lse.  Every row is written (zeros where nothing reaches it); the result does
+ * not depend on the order of workgroups.  Needs sttran_attention_workspace_bytes(args, 1) bytes of device memory. */
+typedef struct SttranAttention {
+  uint32_t struct_size;            /* = sizeof(SttranAttention) */
+  int32_t dtype;                   /* STTRAN_DTYPE_F32 / STTRAN_DTYPE_BF16 */
+  int32_t num_seq, num_q_heads, num_kv_heads, head_dim;     /* head_dim 1 .. 256 */
+  int64_t q_rows, kv_rows;         /* < 2^31 - 1024 */
+  const void *q, *k, *v;
+  int64_t q_row_stride, q_head_stride, k_row_stride, k_head_stride, v_row_stride, v_head_stride;
+  const int32_t *seq_off, *key_off;        /* [num_seq + 1] */
+  const int32_t* prefix_len;               /* [num_seq] or NULL: none */
+  const float* distance_slope;             /* [num_q_heads] or NULL: none */
+  int32_t causal;
+  float score_cap;                         /* 0: none */
+  float scale;
+  int32_t reserved;
+  void *out, *out_residual;                /* contiguous [q_rows, num_q_heads, head_dim]; out_residual may be NULL */
+  float* lse;                              /* [num_q_heads, q_rows]; forward: may be NULL */
+  const void* dout;                        /* backward only, from here on */
+  int64_t dout_row_stride, dout_head_stride;
+  void *dq, *dk, *dv;
+  void* workspace;
+  int64_t workspace_bytes;
+} SttranAttention;
+int64_t sttran_attention_workspace_bytes(const SttranAttention* args, int32_t backward);
+int sttran_attention_forward(const SttranAttention* args, void* stream);
+int sttran_attention_backward(const SttranAttention* args, void* stream);
+
+/* One new token a sequence: q [num_seq, num_q_heads, head_dim] over the first lengths[s] rows (clamped to capacity) of the caches
+ * k / v [num_seq, capacity, num_kv_heads, head_dim]; the token's place is lengths[s] - 1.  Same z as above; length 0 gives zeros.
+ * Rows from lengths[s] on are not read.  num_seq <= 65535.  Workspace: sttran_attention_step_workspace_bytes(args). */
+typedef struct SttranAttentionStep {
+  uint32_t struct_size;            /* = sizeof(SttranAttentionStep) */
+  int32_t dtype;
+  int32_t num_seq, num_q_heads, num_kv_heads, head_dim;
+  int64_t capacity;
+  const void *q, *k, *v;
+  int64_t q_seq_stride, q_head_stride, k_seq_stride, k_row_stride, k_head_stride, v_seq_stride, v_row_stride, v_head_stride;
+  const int32_t* lengths;          /* [num_seq] */
+  const float* distance_slope;     /* [num_q_heads] or NULL */
+  float score_cap, scale;
+  void* out;                       /* contiguous [num_seq, num_q_heads, head_dim] */
+  void* workspace;
+  int64_t workspace_bytes;
+} SttranAttentionStep;
+int64_t sttran_attention_step_workspace_bytes(const SttranAttentionStep* args);
+int sttran_attention_step(const SttranAttentionStep* args, void* stream);
+
+/* Per-head norm and rotary positions of queries and keys in one pass: y = R(positions[t]) x', x' = weight * x / sqrt(mean(x^2) + eps)
+ * where the weights are given (both or neither; fp32 [head_dim]), x' = x otherwise.  R turns pair i of the first rotary_dim (even)
+ * columns by positions[t] * freq[i]; pairs are (2i, 2i+1) with `interleaved`, else (i, i + rotary_dim / 2).  The backward writes
+ * dq, dk (and dq_weight, dk_weight, fp32) from dq_out, dk_out and the forward's inputs.  Outputs and gradients are contiguous. */
+typedef struct SttranRotary {
+  uint32_t struct_size;            /* = sizeof(SttranRotary) */
+  int32_t dtype;
+  int64_t tokens;
+  int32_t num_q_heads, num_kv_heads, head_dim, rotary_dim;
+  const void *q, *k;               /* [tokens, heads, head_dim] */
+  int64_t q_row_stride, q_head_stride, k_row_stride, k_head_stride;
+  const int64_t* positions;        /* [tokens] */
+  const float* freq;               /* [rotary_dim / 2] */
+  const float *q_weight, *k_weight;
+  float eps;
+  int32_t interleaved;
+  void *q_out, *k_out;             /* forward */
+  const void *dq_out, *dk_out;     /* backward, from here on */
+  int64_t dq_row_stride, dq_head_stride, dk_row_stride, dk_head_stride;
+  void *dq, *dk;
+  float *dq_weight, *dk_weight;
+  void* workspace;
+  int64_t workspace_bytes;
+} SttranRotary;
+int64_t sttran_rotary_workspace_bytes(const SttranRotary* args);
+int sttran_rotary_forward(const SttranRotary* args, void* stream);
+int sttran_rotary_backward(const SttranRotary* args, void* stream);
+
+/* Dropout with the residual sum, n contiguous elements: y = residual + (dropped ? 0 : x / (1 - p)).  Element i is dropped where word
+ * i of the generator's stream is below round(p * 2^32); word i is word i % 4 of Philox 4x32-10 at the 128-bit counter
+ * (i / 4, offset) under the 64-bit key.  (key, offset) come from rng_state (device int64[2]) or, with rng_state == NULL, from the
+ * arguments; `used` (device int64[2], optional) receives them, for a backward call: dx = the same call on dy without residual. */
+int sttran_dropout_add(const void* x, const void* residual, void* y, int64_t n, int32_t dtype, double p, const int64_t* rng_state,
+                       int64_t key, int64_t offset, int64_t* used, void* stream);
 
 /* profiling (no reference counterpart; SURVEY 5 "Tracing / profiling: none") */
 int sttran_profile_enable(SttranHandle* h, int32_t enable);

@@ -22,7 +22,7 @@ STTRAN_ERR_INVALID = 1
 ERR_NAMES = {1: "INVALID", 2: "HIP", 3: "EMPTY", 4: "WEIGHTS", 5: "ORDER", 6: "LIMIT", 7: "INDEX"}
 MODE = {"predcls": 0, "sgcls": 1, "sgdet": 2}
 MODEL_STTRAN, MODEL_DSG_DETR = 0, 1
-DTYPE_F32, DTYPE_I64, DTYPE_I32 = 0, 1, 2
+DTYPE_F32, DTYPE_I64, DTYPE_I32, DTYPE_BF16 = 0, 1, 2, 3
 PROF_CLASSES = 8
 PROF_NAMES = ["gemm", "union_conv", "mask_conv", "attention", "layernorm", "index", "other", "_"]
 
@@ -97,6 +97,39 @@ class SttranObjclsSelect(C.Structure):
                 ("out_human_idx", C.c_void_p), ("scratch", C.c_void_p), ("scratch_bytes", C.c_int64)]
 
 
+def _fields(ctype, names):
+    return [(n, ctype) for n in names.split()]
+
+
+class SttranAttention(C.Structure):
+    _fields_ = ([("struct_size", C.c_uint32)] + _fields(C.c_int32, "dtype num_seq num_q_heads num_kv_heads head_dim") +
+                _fields(C.c_int64, "q_rows kv_rows") + _fields(C.c_void_p, "q k v") +
+                _fields(C.c_int64, "q_row_stride q_head_stride k_row_stride k_head_stride v_row_stride v_head_stride") +
+                _fields(C.c_void_p, "seq_off key_off prefix_len distance_slope") +
+                [("causal", C.c_int32), ("score_cap", C.c_float), ("scale", C.c_float), ("reserved", C.c_int32)] +
+                _fields(C.c_void_p, "out out_residual lse dout") + _fields(C.c_int64, "dout_row_stride dout_head_stride") +
+                _fields(C.c_void_p, "dq dk dv workspace") + [("workspace_bytes", C.c_int64)])
+
+
+class SttranAttentionStep(C.Structure):
+    _fields_ = ([("struct_size", C.c_uint32)] + _fields(C.c_int32, "dtype num_seq num_q_heads num_kv_heads head_dim") +
+                [("capacity", C.c_int64)] + _fields(C.c_void_p, "q k v") +
+                _fields(C.c_int64, "q_seq_stride q_head_stride k_seq_stride k_row_stride k_head_stride v_seq_stride v_row_stride "
+                                   "v_head_stride") +
+                _fields(C.c_void_p, "lengths distance_slope") + _fields(C.c_float, "score_cap scale") +
+                _fields(C.c_void_p, "out workspace") + [("workspace_bytes", C.c_int64)])
+
+
+class SttranRotary(C.Structure):
+    _fields_ = ([("struct_size", C.c_uint32), ("dtype", C.c_int32), ("tokens", C.c_int64)] +
+                _fields(C.c_int32, "num_q_heads num_kv_heads head_dim rotary_dim") + _fields(C.c_void_p, "q k") +
+                _fields(C.c_int64, "q_row_stride q_head_stride k_row_stride k_head_stride") +
+                _fields(C.c_void_p, "positions freq q_weight k_weight") + [("eps", C.c_float), ("interleaved", C.c_int32)] +
+                _fields(C.c_void_p, "q_out k_out dq_out dk_out") +
+                _fields(C.c_int64, "dq_row_stride dq_head_stride dk_row_stride dk_head_stride") +
+                _fields(C.c_void_p, "dq dk dq_weight dk_weight workspace") + [("workspace_bytes", C.c_int64)])
+
+
 # every symbol include/sttran_hip.h (the drop-in boundary) and include/sttran_hip_debug.h (test hooks, experiment
 # switches: names `sttran_debug_*` and sttran_set_gemm_engine) declare: (name, restype, argtypes)
 SYMBOLS = [
@@ -129,6 +162,16 @@ SYMBOLS = [
     ("sttran_objcls_select", C.c_int, [C.POINTER(SttranObjclsSelect), C.POINTER(C.c_int64), C.POINTER(C.c_int64), C.c_void_p]),
     ("sttran_roi_align", C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_int64, C.c_int32,
                                    C.c_float, C.c_int32, C.c_void_p, C.c_void_p]),
+    ("sttran_attention_workspace_bytes", C.c_int64, [C.POINTER(SttranAttention), C.c_int32]),
+    ("sttran_attention_forward", C.c_int, [C.POINTER(SttranAttention), C.c_void_p]),
+    ("sttran_attention_backward", C.c_int, [C.POINTER(SttranAttention), C.c_void_p]),
+    ("sttran_attention_step_workspace_bytes", C.c_int64, [C.POINTER(SttranAttentionStep)]),
+    ("sttran_attention_step", C.c_int, [C.POINTER(SttranAttentionStep), C.c_void_p]),
+    ("sttran_rotary_workspace_bytes", C.c_int64, [C.POINTER(SttranRotary)]),
+    ("sttran_rotary_forward", C.c_int, [C.POINTER(SttranRotary), C.c_void_p]),
+    ("sttran_rotary_backward", C.c_int, [C.POINTER(SttranRotary), C.c_void_p]),
+    ("sttran_dropout_add", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_double, C.c_void_p,
+                                     C.c_int64, C.c_int64, C.c_void_p, C.c_void_p]),
     ("sttran_debug_gemm", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                     C.c_int64, C.c_int64, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_void_p]),
     ("sttran_debug_gemm_padded", C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p,

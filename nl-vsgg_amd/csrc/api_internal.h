@@ -6,6 +6,7 @@
 //   api_lanes.hip    lanes, stream ordering, sttran_forward / forward_lane / reserve / sync_check
 //   api_profile.hip  HIP-event profile of the launch sites (bench.py's roofline leg)
 //   api_ops.hip      the entry points without a handle (union boxes, evaluator, ObjectClassifier selection, ROIAlign)
+//   api_sequence.hip the sequence operators (packed attention, attention step, rotary positions, dropout): no handle either
 //   api_debug.hip    sttran_debug_* test hooks (include/sttran_hip_debug.h)
 #pragma once
 #include <hip/hip_runtime.h>

@@ -1,0 +1,283 @@
+// kernels_seq_attn.hip -- attention over packed sequences, forward.
+//   o_i = sum_j p_ij v_j,  p_i = softmax over the visible keys j of z_ij,
+//   z_ij = cap * tanh(scale * q_i.k_j / cap) - slope_h * |place_i - j|
+#include "kernels_seq.h"
+#include "seq_attn.h"
+
+namespace sttran {
+
+// the own rows in `rows`, key by key over what each of them sees in [beg, end)
+template <class C>
+__device__ __forceinline__ void seq_attn_fwd_again(const SeqAttnArgs& A, const SeqScore& sc, uint32_t rows, SeqRow me, int row0, int head,
+                                                             int beg, int end, int dh) {
+  using T = typename C::E;
+  const int lane = threadIdx.x & 63, kvh = head / (A.hq / A.hk);
+#pragma unroll 1
+  for (int n = 0; n < 32; ++n) {
+    const int row = row0 + n;
+    if (!(rows >> n & 1) || row >= A.tq || (C::DS == 2 && (n & 1) != dh)) continue;
+    const int lo = max(__shfl(me.lo, n), beg), hi = min(__shfl(me.hi, n), end), base = __shfl(me.base, n);
+    const SeqSpread q = seq_spread<T>(A.q + head * A.q_h + (int64_t)row * A.q_t, A.d);
+    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f}, unused;
+#pragma unroll 1
+    for (int key = lo; key < hi; ++key) {
+      const SeqSpread k = seq_spread<T>(A.k + kvh * A.k_h + (int64_t)key * A.k_t, A.d);
+      const SeqSpread v = seq_spread<T>(A.v + kvh * A.v_h + (int64_t)key * A.v_t, A.d);
+      const float z = seq_z<T>(A, sc, seq_spread_dot(q, k), base, key, unused);
+      const float mn = fmaxf(m, z), ms = mn == -INFINITY ? 0.f : mn, al = __builtin_amdgcn_exp2f(m - ms), p = __builtin_amdgcn_exp2f(z - ms);
+      l = fmaf(l, al, p);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) o[u] = fmaf(o[u], al, p * v.x[u]);
+      m = mn;
+    }
+    if (A.splits > 1) {
+      const int64_t at = ((int64_t)blockIdx.y * A.hq + head) * A.tq + row;
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (lane + 64 * u < A.d) A.part[at * A.d + lane + 64 * u] = o[u];
+      float* ps = A.part + (int64_t)A.splits * A.hq * A.tq * A.d + at * 2;
+      if (lane == 0) { ps[0] = m; ps[1] = l; }
+      continue;
+    }
+    const int64_t at = ((int64_t)row * A.hq + head) * A.d * C::ES;
+    seq_spread_store<T>(A.out + at, A.out_lo ? A.out_lo + at : nullptr, o, l == 0.f ? 0.f : 1.f / l, A.d);
+    if (A.lse && lane == 0) A.lse[(int64_t)head * A.tq + row] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+  }
+}
+
+// One pass over the keys with the running maximum m and sum l of the softmax (both fp32, base 2).  The accumulator is rescaled
+// only when the maximum grows by more than 8 (a factor of 256): p stays below 2^8 and the final division by l undoes any
+// common factor exactly as the textbook form does.
+template <class C>
+__global__ void __launch_bounds__(C::NT) __attribute__((amdgpu_waves_per_eu(2, 2)))
+seq_attn_fwd_kernel(SeqAttnArgs A) {
+  using T = typename C::E;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  char *kt_lds = smem, *vt_lds = smem + C::kTileBytes, *xch = smem + 2 * C::kTileBytes;
+  int* red = reinterpret_cast<int*>(xch + C::kXchBytes);
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  const int tiles = (A.tq + C::RB - 1) / C::RB;
+  const int id = seq_xcd_order(blockIdx.x, gridDim.x);
+  const int head = id / tiles, tile = tiles - 1 - id % tiles;      // rows that see most keys first where the order masks
+  const int kvh = head / (A.hq / A.hk), dh = C::DS == 2 ? (w & 1) : 0;
+  const int row0 = tile * C::RB + 32 * (w / C::DS), row = row0 + (lane & 31);
+  const int dbytes = A.d * C::ES;
+
+  const SeqRow me = seq_row(A, row);
+  int lo = me.hi > me.lo ? me.lo : INT_MAX, hi = me.hi;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    lo = min(lo, __shfl_xor(lo, o));
+    hi = max(hi, __shfl_xor(hi, o));
+  }
+  const int wlo = lo, whi = hi;                                     // what this wave's rows see
+  if (lane == 0) { red[2 * w] = lo; red[2 * w + 1] = hi; }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < C::NW; ++i) { lo = min(lo, red[2 * i]); hi = max(hi, red[2 * i + 1]); }
+  int beg = lo, end = max(hi, lo);
+  if (hi <= 0) beg = end = 0;
+  if (A.splits > 1) {                                               // this workgroup's share of the keys, whole tiles
+    const int per = ((end - beg + A.splits - 1) / A.splits + C::BR - 1) / C::BR * C::BR;
+    beg = min(beg + (int)blockIdx.y * per, end);
+    end = min(beg + per, end);
+  }
+
+  seq_u32x4 own[C::NF];
+  seq_own_load<C>(own, A.q + head * A.q_h, A.q_t, row0, A.tq, dh, dbytes);
+  const char *kp = A.k + kvh * A.k_h, *vp = A.v + kvh * A.v_h;
+  const SeqScore sc(A, head);
+  const bool capped = A.cap > 0.f;
+
+  seq_f32x16 acc[C::NB];
+  float m, l;
+#pragma unroll
+  for (int nb = 0; nb < C::NB; ++nb)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[nb][e] = 0.f;
+  m = -INFINITY; l = 0.f;
+  seq_u32x4 kr[C::NL], vr[C::NL];
+  if (beg < end) {
+    seq_tile_load<C>(kr, kp, A.k_t, beg, end, dbytes);
+    seq_tile_load<C>(vr, vp, A.v_t, beg, end, dbytes);
+  }
+  for (int kt = beg; kt < end; kt += C::BR) {
+    __syncthreads();
+    seq_tile_store<C>(kr, kt_lds, dbytes);
+    seq_tile_store<C>(vr, vt_lds, dbytes);
+    __syncthreads();
+    if (kt + C::BR < end) {
+      seq_tile_load<C>(kr, kp, A.k_t, kt + C::BR, end, dbytes);
+      seq_tile_load<C>(vr, vp, A.v_t, kt + C::BR, end, dbytes);
+    }
+    const bool active = wlo < min(kt + C::BR, end) && whi > kt;
+    seq_f32x16 s[C::NSUB];
+    if (active || C::DS == 2) {
+#pragma unroll
+      for (int u = 0; u < C::NSUB; ++u) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[u][e] = 0.f;
+        if (active) seq_scores<C>(s[u], kt_lds, u, dh, own);
+        if (C::DS == 2) {
+          if (u > 0) __syncthreads();
+          seq_exchange<C>(s[u], xch);
+        }
+      }
+    }
+    if (!active) continue;
+    const int rlo = max(me.lo, beg), rhi = min(me.hi, end);        // this lane's visible keys of this workgroup
+    const bool full = __all(rlo <= kt && rhi >= kt + C::BR);
+    float mt = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < C::NSUB; ++u) {
+      if (capped) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[u][e] = sc.capl * seq_tanh<T>(s[u][e] * sc.mul);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[u][e] *= sc.mul;
+      }
+      const int k0 = kt + 32 * u + 4 * h;
+      if (A.slope) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[u][e] = fmaf(-sc.slope, fabsf((float)(me.base - k0 - 8 * (e >> 2) - (e & 3))), s[u][e]);
+      }
+      if (!full) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int key = k0 + 8 * (e >> 2) + (e & 3);
+          s[u][e] = key >= rlo && key < rhi ? s[u][e] : -INFINITY;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[u][e]);
+    }
+    mt = fmaxf(mt, __shfl_xor(mt, 32));
+    if (__any(mt > m + 8.f || (m == -INFINITY && mt > -INFINITY))) {
+      const float mn = fmaxf(m, mt);
+      const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn; l *= al;
+#pragma unroll
+      for (int nb = 0; nb < C::NB; ++nb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[nb][e] *= al;
+    }
+    const float ms = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int u = 0; u < C::NSUB; ++u) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        s[u][e] = __builtin_amdgcn_exp2f(s[u][e] - ms);
+        l += s[u][e];
+      }
+      seq_reduce<C>(acc, vt_lds, u, dh, s[u]);
+    }
+  }
+  const uint32_t bad = seq_bad_rows<C>(acc, 0, red);
+  l += __shfl_xor(l, 32);
+  if (bad) seq_attn_fwd_again<C>(A, sc, bad, me, row0, head, beg, end, dh);
+  if (row >= A.tq || (bad >> (lane & 31) & 1)) return;
+  if (A.splits > 1) {
+    // unnormalised share of this split: [split][head][row][d], then [split][head][row][2]
+    const int64_t at = ((int64_t)blockIdx.y * A.hq + head) * A.tq + row;
+    float* po = A.part + at * A.d;
+#pragma unroll
+    for (int nb = 0; nb < C::NB; ++nb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int col = dh * C::DH + 32 * nb + 8 * (e >> 2) + 4 * h + (e & 3);
+        if (col < A.d) po[col] = acc[nb][e];
+      }
+    if (dh == 0 && h == 0) {
+      float* ps = A.part + (int64_t)A.splits * A.hq * A.tq * A.d + at * 2;
+      ps[0] = m; ps[1] = l;
+    }
+    return;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int64_t at = ((int64_t)row * A.hq + head) * dbytes;
+  seq_store_own<C>(acc, inv, A.out + at, A.out_lo ? A.out_lo + at : nullptr, dh, A.d, A.aln);
+  if (A.lse && dh == 0 && h == 0) A.lse[(int64_t)head * A.tq + row] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+}
+
+// joins the shares of a launch that was split over the keys, in the order of the splits: one wave a (row, head)
+template <class T>
+__global__ void __launch_bounds__(256) seq_attn_join_kernel(SeqAttnArgs A, const int* lens, int chunk, int capacity) {
+  const int lane = threadIdx.x & 63;
+  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);         // head * tq + row
+  if (i >= (int64_t)A.hq * A.tq) return;
+  const int head = (int)(i / A.tq), row = (int)(i % A.tq);
+  const int64_t step = (int64_t)A.hq * A.tq;
+  const int shares = lens ? min((min(max(lens[row], 1), capacity) + chunk - 1) / chunk, A.splits) : A.splits;
+  const float* ps = A.part + (int64_t)A.splits * step * A.d;
+  float m = -INFINITY;
+  for (int s = 0; s < shares; ++s) m = fmaxf(m, ps[(s * step + i) * 2]);
+  const float ms = m == -INFINITY ? 0.f : m;
+  float o[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
+  for (int s = 0; s < shares; ++s) {
+    const float mx = ps[(s * step + i) * 2], lx = ps[(s * step + i) * 2 + 1];
+    if (lx == 0.f) continue;                                               // nothing visible there
+    const float f = __builtin_amdgcn_exp2f(mx - ms);
+    l = fmaf(lx, f, l);
+    const float* po = A.part + (s * step + i) * A.d;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (lane + 64 * u < A.d) o[u] = fmaf(po[lane + 64 * u], f, o[u]);
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int64_t at = ((int64_t)row * A.hq + head) * A.d;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    if (lane + 64 * u >= A.d) continue;
+    const float x = o[u] * inv;
+    if constexpr (sizeof(T) == 4) {
+      reinterpret_cast<float*>(A.out)[at + lane + 64 * u] = x;
+    } else {
+      const float y = SeqElt<T>::round(x);
+      reinterpret_cast<uint16_t*>(A.out)[at + lane + 64 * u] = (uint16_t)SeqElt<T>::bits(y);
+      if (A.out_lo) reinterpret_cast<uint16_t*>(A.out_lo)[at + lane + 64 * u] = (uint16_t)SeqElt<T>::bits(x - y);
+    }
+  }
+  if (A.lse && lane == 0) A.lse[i] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+}
+
+hipError_t launch_seq_attn_join(hipStream_t s, int bf16, const SeqAttnArgs& A, const int* lens, int chunk, int capacity) {
+  const unsigned grid = (unsigned)(((int64_t)A.hq * A.tq + 3) / 4);
+  if (bf16) seq_attn_join_kernel<__bf16><<<grid, 256, 0, s>>>(A, lens, chunk, capacity);
+  else seq_attn_join_kernel<float><<<grid, 256, 0, s>>>(A, lens, chunk, capacity);
+  return hipGetLastError();
+}
+
+int seq_attn_splits(int bf16, const SeqAttnArgs& A) {
+  (void)bf16; (void)A;
+  return 1;
+}
+
+template <class C>
+static hipError_t fwd(hipStream_t s, const SeqAttnArgs& A) {
+  constexpr int lds = 2 * C::kTileBytes + C::kXchBytes + C::NW * 8;
+  static DeviceMarks marks;
+  auto fn = seq_attn_fwd_kernel<C>;
+  hipError_t e = marks.raise_lds(reinterpret_cast<const void*>(fn), lds);
+  if (e != hipSuccess) return e;
+  const int tiles = (A.tq + C::RB - 1) / C::RB;
+  fn<<<dim3((unsigned)(tiles * A.hq), (unsigned)A.splits), C::NT, lds, s>>>(A);
+  e = hipGetLastError();
+  return e != hipSuccess || A.splits == 1 ? e : launch_seq_attn_join(s, C::ES == 2, A, nullptr, 0, 0);
+}
+
+template <class T, bool VEC>
+static hipError_t pick(hipStream_t s, const SeqAttnArgs& A) {
+  if (A.d <= 64) return fwd<SeqTile<T, 64, 1, 4, 64, VEC>>(s, A);
+  if (A.d <= 128) return fwd<SeqTile<T, 128, 1, 4, sizeof(T) == 2 ? 64 : 32, VEC>>(s, A);
+  return fwd<SeqTile<T, 256, 2, 8, 32, VEC>>(s, A);
+}
+
+hipError_t launch_seq_attn_forward(hipStream_t s, int bf16, const SeqAttnArgs& A) {
+  if (A.tq == 0) return hipSuccess;
+  const bool vec = A.aln >= 4 && A.d * (bf16 ? 2 : 4) >= 16;
+  if (bf16) return vec ? pick<__bf16, true>(s, A) : pick<__bf16, false>(s, A);
+  return vec ? pick<float, true>(s, A) : pick<float, false>(s, A);
+}
+
+}  // namespace sttran

@@ -1,0 +1,411 @@
+// kernels_seq_attn_bwd.hip -- gradients of attention over packed sequences (kernels_seq_attn.hip).
+//   p_ij  = exp(z_ij - lse_i)            (recomputed from q, k and the saved log-sum)
+//   ds_ij = p_ij * (dout_i.v_j - delta_i) * dz/ds,   delta_i = dout_i.o_i,   dz/ds = 1 - tanh^2 under a cap
+//   dq_i  = scale * sum_j ds_ij k_j      dk_j = scale * sum_i ds_ij q_i      dv_j = sum_i p_ij dout_i
+// Two passes over the score blocks, each writing every output row once from one workgroup: nothing is added atomically, so
+// results do not depend on the order of workgroups (the price: 7 products where one pass with atomic adds takes 5).  Key heads
+// that several query heads share sum over them inside the workgroup.
+#include <type_traits>
+
+#include "kernels_seq.h"
+#include "seq_attn.h"
+
+namespace sttran {
+
+// delta and the rows' key ranges: LPR lanes a (row, head), 16 bytes a lane.  The sums take out in full width: out + what its
+// rounding took (out_lo), because delta's error is common to a whole row of ds
+template <class T, int LPR>
+__global__ void __launch_bounds__(256) seq_attn_delta_kernel(SeqAttnArgs A) {
+  const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPR;
+  const int c = threadIdx.x % LPR;
+  if (item >= (int64_t)A.tq * A.hq) return;
+  const int row = (int)(item / A.hq), head = (int)(item % A.hq), dbytes = A.d * (int)sizeof(T);
+  const int valid = dbytes - 16 * c;
+  const seq_u32x4 g = seq_load16(A.dout + row * A.do_t + head * A.do_h + 16 * c, valid, A.aln);
+  const seq_u32x4 o = seq_load16(A.out + item * dbytes + 16 * c, valid, A.aln);
+  seq_u32x4 r = {0, 0, 0, 0};
+  if (A.out_lo) r = seq_load16(A.out_lo + item * dbytes + 16 * c, valid, A.aln);
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < SeqElt<T>::kPer16; ++i)
+    s = fmaf(SeqElt<T>::get(g, i), SeqElt<T>::get(o, i) + (sizeof(T) == 2 ? SeqElt<T>::get(r, i) : 0.f), s);
+#pragma unroll
+  for (int x = 1; x < LPR; x <<= 1) s += __shfl_xor(s, x);
+  if (c) return;
+  A.delta[(int64_t)head * A.tq + row] = s;
+  if (head == 0) {
+    const SeqRow i = seq_row(A, row);
+    A.rows[row] = make_int4(i.lo, i.hi, i.base, 0);
+  }
+}
+
+// p and ds of one pair from its products (s = q.k, dp = dout.v); hidden pairs become exact zeros in both
+template <class T, bool CAP, bool SLOPE>
+__device__ __forceinline__ void seq_pair(const SeqScore& sc, float& s, float& dp, bool seen, float lse, float delta, int away) {
+  float z, bend = 1.f;
+  if constexpr (CAP) {
+    const float t = seq_tanh<T>(s * sc.mul);
+    bend = 1.f - t * t;
+    z = fmaf(sc.capl, t, -lse);
+  } else {
+    z = fmaf(s, sc.mul, -lse);
+  }
+  if constexpr (SLOPE) z = fmaf(-sc.slope, fabsf((float)away), z);
+  const float p = __builtin_amdgcn_exp2f(z);
+  dp = (dp - delta) * p;
+  if constexpr (CAP) dp *= bend;
+  s = seen ? p : 0.f;
+  dp = seen ? dp : 0.f;
+}
+template <class T>
+__device__ __forceinline__ void seq_pair_any(const SeqAttnArgs& A, const SeqScore& sc, float& s, float& dp, bool seen, float lse, float delta,
+                                             int away) {
+  if (A.cap > 0.f) {
+    if (A.slope) seq_pair<T, true, true>(sc, s, dp, seen, lse, delta, away);
+    else seq_pair<T, true, false>(sc, s, dp, seen, lse, delta, away);
+  } else {
+    if (A.slope) seq_pair<T, false, true>(sc, s, dp, seen, lse, delta, away);
+    else seq_pair<T, false, false>(sc, s, dp, seen, lse, delta, away);
+  }
+}
+// one of four bodies, chosen outside the loop over a block's elements
+template <class F>
+__device__ __forceinline__ void seq_by_score(const SeqAttnArgs& A, F f) {
+  if (A.cap > 0.f) {
+    if (A.slope) f(std::true_type{}, std::true_type{});
+    else f(std::true_type{}, std::false_type{});
+  } else {
+    if (A.slope) f(std::false_type{}, std::true_type{});
+    else f(std::false_type{}, std::false_type{});
+  }
+}
+
+// ---- dq: own rows = queries, keys and values stream ---------------------------------------------------------------------
+template <class C>
+__device__ __forceinline__ void seq_attn_dq_again(const SeqAttnArgs& A, const SeqScore& sc, uint32_t rows, SeqRow me, int row0, int head, int dh) {
+  using T = typename C::E;
+  const int kvh = head / (A.hq / A.hk);
+#pragma unroll 1
+  for (int n = 0; n < 32; ++n) {
+    const int row = row0 + n;
+    if (!(rows >> n & 1) || row >= A.tq || (C::DS == 2 && (n & 1) != dh)) continue;
+    const int lo = __shfl(me.lo, n), hi = __shfl(me.hi, n), base = __shfl(me.base, n);
+    const SeqSpread q = seq_spread<T>(A.q + head * A.q_h + (int64_t)row * A.q_t, A.d);
+    const SeqSpread g = seq_spread<T>(A.dout + head * A.do_h + (int64_t)row * A.do_t, A.d);
+    const float lse = A.lse[(int64_t)head * A.tq + row], delta = A.delta[(int64_t)head * A.tq + row];
+    float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int key = lo; key < hi; ++key) {
+      const SeqSpread k = seq_spread<T>(A.k + kvh * A.k_h + (int64_t)key * A.k_t, A.d);
+      const SeqSpread v = seq_spread<T>(A.v + kvh * A.v_h + (int64_t)key * A.v_t, A.d);
+      float s = seq_spread_dot(q, k), dp = seq_spread_dot(g, v);
+      seq_pair_any<T>(A, sc, s, dp, true, lse, delta, base - key);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) o[u] = fmaf(dp, k.x[u], o[u]);
+    }
+    seq_spread_store<T>(A.dq + ((int64_t)row * A.hq + head) * A.d * C::ES, nullptr, o, A.scale, A.d);
+  }
+}
+
+template <class C>
+__global__ void __launch_bounds__(C::NT) __attribute__((amdgpu_waves_per_eu(C::NT / 256, C::NT / 256)))
+seq_attn_dq_kernel(SeqAttnArgs A) {
+  using T = typename C::E;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  char *kt_lds = smem, *vt_lds = smem + C::kTileBytes, *xch = smem + 2 * C::kTileBytes;
+  int* red = reinterpret_cast<int*>(xch + 2 * C::kXchBytes);
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  const int tiles = (A.tq + C::RB - 1) / C::RB;
+  const int id = seq_xcd_order(blockIdx.x, gridDim.x);
+  const int head = id / tiles, tile = tiles - 1 - id % tiles;
+  const int kvh = head / (A.hq / A.hk), dh = C::DS == 2 ? (w & 1) : 0;
+  const int row0 = tile * C::RB + 32 * (w / C::DS), row = row0 + (lane & 31);
+  const int dbytes = A.d * C::ES;
+
+  SeqRow me{0, 0, 0};
+  float lse = INFINITY, delta = 0.f;
+  if (row < A.tq) {
+    const int4 r = A.rows[row];
+    me.lo = r.x; me.hi = r.y; me.base = r.z;
+    lse = A.lse[(int64_t)head * A.tq + row];
+    delta = A.delta[(int64_t)head * A.tq + row];
+  }
+  int lo = me.hi > me.lo ? me.lo : INT_MAX, hi = me.hi;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    lo = min(lo, __shfl_xor(lo, o));
+    hi = max(hi, __shfl_xor(hi, o));
+  }
+  const int wlo = lo, whi = hi;
+  if (lane == 0) { red[2 * w] = lo; red[2 * w + 1] = hi; }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < C::NW; ++i) { lo = min(lo, red[2 * i]); hi = max(hi, red[2 * i + 1]); }
+  int beg = lo, end = max(hi, lo);
+  if (hi <= 0) beg = end = 0;
+
+  seq_u32x4 oq[C::NF], og[C::NF];
+  seq_own_load<C>(oq, A.q + head * A.q_h, A.q_t, row0, A.tq, dh, dbytes);
+  seq_own_load<C>(og, A.dout + head * A.do_h, A.do_t, row0, A.tq, dh, dbytes);
+  const char *kp = A.k + kvh * A.k_h, *vp = A.v + kvh * A.v_h;
+  const SeqScore sc(A, head);
+  seq_f32x16 acc[C::NB];
+#pragma unroll
+  for (int nb = 0; nb < C::NB; ++nb)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[nb][e] = 0.f;
+  seq_u32x4 kr[C::NL], vr[C::NL];
+  if (beg < end) {
+    seq_tile_load<C>(kr, kp, A.k_t, beg, end, dbytes);
+    seq_tile_load<C>(vr, vp, A.v_t, beg, end, dbytes);
+  }
+  for (int kt = beg; kt < end; kt += C::BR) {
+    __syncthreads();
+    seq_tile_store<C>(kr, kt_lds, dbytes);
+    seq_tile_store<C>(vr, vt_lds, dbytes);
+    __syncthreads();
+    if (kt + C::BR < end) {
+      seq_tile_load<C>(kr, kp, A.k_t, kt + C::BR, end, dbytes);
+      seq_tile_load<C>(vr, vp, A.v_t, kt + C::BR, end, dbytes);
+    }
+#pragma unroll 1
+    for (int u = 0; u < C::NSUB; ++u) {
+      const int kb = kt + 32 * u;
+      const bool active = wlo < min(kb + 32, end) && whi > kb;
+      if (C::DS == 1 && !active) continue;
+      seq_f32x16 s, dp;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) { s[e] = 0.f; dp[e] = 0.f; }
+      if (active) {
+        seq_scores<C>(s, kt_lds, u, dh, oq);
+        seq_scores<C>(dp, vt_lds, u, dh, og);
+      }
+      if constexpr (C::DS == 2) {
+        if (u > 0) __syncthreads();
+        seq_exchange2<C>(s, dp, xch);
+        if (!active) continue;
+      }
+      seq_by_score(A, [&](auto cap, auto slope) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int key = kb + 4 * h + 8 * (e >> 2) + (e & 3);
+          float x = s[e], y = dp[e];
+          seq_pair<T, cap.value, slope.value>(sc, x, y, key >= me.lo && key < me.hi, lse, delta, me.base - key);
+          dp[e] = y;
+        }
+      });
+      seq_reduce<C>(acc, kt_lds, u, dh, dp);
+    }
+  }
+  const uint32_t bad = seq_bad_rows<C>(acc, 0, red);
+  if (bad) seq_attn_dq_again<C>(A, sc, bad, me, row0, head, dh);
+  if (row >= A.tq || (bad >> (lane & 31) & 1)) return;
+  seq_store_own<C>(acc, A.scale, A.dq + ((int64_t)row * A.hq + head) * dbytes, nullptr, dh, A.d, A.aln);
+}
+
+// ---- dk, dv: own rows = keys, queries and dout stream ---------------------------------------------------------------------
+template <class C>
+__device__ __forceinline__ void seq_attn_dkv_again(const SeqAttnArgs& A, uint32_t rows, int row0, int kvh, int qbeg, int qend, int dh) {
+  using T = typename C::E;
+  const int grp = A.hq / A.hk;
+#pragma unroll 1
+  for (int n = 0; n < 32; ++n) {
+    const int key = row0 + n;
+    if (!(rows >> n & 1) || key >= A.tk || (C::DS == 2 && (n & 1) != dh)) continue;
+    const SeqSpread k = seq_spread<T>(A.k + kvh * A.k_h + (int64_t)key * A.k_t, A.d);
+    const SeqSpread v = seq_spread<T>(A.v + kvh * A.v_h + (int64_t)key * A.v_t, A.d);
+    float dk[4] = {0.f, 0.f, 0.f, 0.f}, dv[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int g = 0; g < grp; ++g) {
+      const int head = kvh * grp + g;
+      const SeqScore sc(A, head);
+#pragma unroll 1
+      for (int row = qbeg; row < qend; ++row) {
+        const int4 r = A.rows[row];
+        if (key < r.x || key >= r.y) continue;
+        const SeqSpread q = seq_spread<T>(A.q + head * A.q_h + (int64_t)row * A.q_t, A.d);
+        const SeqSpread o = seq_spread<T>(A.dout + head * A.do_h + (int64_t)row * A.do_t, A.d);
+        float s = seq_spread_dot(q, k), dp = seq_spread_dot(o, v);
+        seq_pair_any<T>(A, sc, s, dp, true, A.lse[(int64_t)head * A.tq + row], A.delta[(int64_t)head * A.tq + row], r.z - key);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          dk[u] = fmaf(dp, q.x[u], dk[u]);
+          dv[u] = fmaf(s, o.x[u], dv[u]);
+        }
+      }
+    }
+    const int64_t at = ((int64_t)key * A.hk + kvh) * A.d * C::ES;
+    seq_spread_store<T>(A.dk + at, nullptr, dk, A.scale, A.d);
+    seq_spread_store<T>(A.dv + at, nullptr, dv, 1.f, A.d);
+  }
+}
+
+template <class C>
+__global__ void __launch_bounds__(C::NT) __attribute__((amdgpu_waves_per_eu(C::ES == 4 && C::DS == 2 ? 1 : 2, C::ES == 4 && C::DS == 2 ? 1 : 2)))
+seq_attn_dkv_kernel(SeqAttnArgs A) {
+  using T = typename C::E;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  char *qt_lds = smem, *gt_lds = smem + C::kTileBytes, *xch = smem + 2 * C::kTileBytes;
+  float* rowf = reinterpret_cast<float*>(xch + 2 * C::kXchBytes);       // [2][BR]: lse, delta
+  int* rowi = reinterpret_cast<int*>(rowf + 2 * C::BR);                 // [3][BR]: lo, hi, base
+  int* red = rowi + 3 * C::BR;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  const int tiles = (A.tk + C::RB - 1) / C::RB, grp = A.hq / A.hk;
+  const int id = seq_xcd_order(blockIdx.x, gridDim.x);
+  const int kvh = id / tiles, tile = id % tiles, dh = C::DS == 2 ? (w & 1) : 0;
+  const int first = tile * C::RB, row0 = first + 32 * (w / C::DS), key = row0 + (lane & 31);
+  const int dbytes = A.d * C::ES;
+
+  // query rows that may see a key of this tile: those of the sequences that the tile touches
+  int qbeg = 0, qend = 0;
+  {
+    const int s0 = seq_find(A.off_k, A.nseq, first), s1 = min(seq_find(A.off_k, A.nseq, min(first + C::RB, A.tk) - 1), A.nseq - 1);
+    if (s0 < A.nseq) {
+      qbeg = A.off_q[s0];
+      qend = min(max(A.off_q[s1 + 1], 0), A.tq);
+      const int at = max(first - A.off_k[s0], 0);
+      if (A.causal && !(A.prefix && A.prefix[s0] > at)) {
+        const int lq = A.off_q[s0 + 1] - qbeg, lk = A.off_k[s0 + 1] - A.off_k[s0];
+        qbeg += min(max(at - (lk - lq), 0), max(lq, 0));
+      }
+      qbeg = min(max(qbeg, 0), A.tq);
+    }
+  }
+
+  seq_u32x4 ok[C::NF], ov[C::NF];
+  seq_own_load<C>(ok, A.k + kvh * A.k_h, A.k_t, row0, A.tk, dh, dbytes);
+  seq_own_load<C>(ov, A.v + kvh * A.v_h, A.v_t, row0, A.tk, dh, dbytes);
+  seq_f32x16 dk[C::NB], dv[C::NB];
+#pragma unroll
+  for (int nb = 0; nb < C::NB; ++nb)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) { dk[nb][e] = 0.f; dv[nb][e] = 0.f; }
+
+  for (int g = 0; g < grp; ++g) {
+    const int head = kvh * grp + g;
+    const char *qp = A.q + head * A.q_h, *gp = A.dout + head * A.do_h;
+    const float *lse = A.lse + (int64_t)head * A.tq, *delta = A.delta + (int64_t)head * A.tq;
+    const SeqScore sc(A, head);
+    seq_u32x4 qr[C::NL], gr[C::NL];
+    float rf[2] = {INFINITY, 0.f};
+    int4 ri = make_int4(0, 0, 0, 0);
+    const auto load = [&](int qt) {
+      seq_tile_load<C>(qr, qp, A.q_t, qt, qend, dbytes);
+      seq_tile_load<C>(gr, gp, A.do_t, qt, qend, dbytes);
+      rf[0] = INFINITY; rf[1] = 0.f; ri = make_int4(0, 0, 0, 0);
+      if (tid < C::BR && qt + tid < qend) { rf[0] = lse[qt + tid]; rf[1] = delta[qt + tid]; ri = A.rows[qt + tid]; }
+    };
+    if (qbeg < qend) load(qbeg);
+    for (int qt = qbeg; qt < qend; qt += C::BR) {
+      __syncthreads();
+      seq_tile_store<C>(qr, qt_lds, dbytes);
+      seq_tile_store<C>(gr, gt_lds, dbytes);
+      if (tid < C::BR) {
+        rowf[tid] = rf[0]; rowf[C::BR + tid] = rf[1];
+        rowi[tid] = ri.x; rowi[C::BR + tid] = ri.y; rowi[2 * C::BR + tid] = ri.z;
+      }
+      __syncthreads();
+      if (qt + C::BR < qend) load(qt + C::BR);
+#pragma unroll 1
+      for (int u = 0; u < C::NSUB; ++u) {
+        const int rl = rowi[32 * u + (lane & 31)], rh = rowi[C::BR + 32 * u + (lane & 31)];
+        const bool active = __any(rl < row0 + 32 && rh > row0);
+        if (C::DS == 1 && !active) continue;
+        seq_f32x16 s, dp;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) { s[e] = 0.f; dp[e] = 0.f; }
+        if (active) {
+          seq_scores<C>(s, qt_lds, u, dh, ok);
+          seq_scores<C>(dp, gt_lds, u, dh, ov);
+        }
+        if constexpr (C::DS == 2) {
+          if (u > 0) __syncthreads();
+          seq_exchange2<C>(s, dp, xch);
+          if (!active) continue;
+        }
+        seq_by_score(A, [&](auto cap, auto slope) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int at = 32 * u + 8 * q + 4 * h;
+            const seq_f32x4 l4 = *reinterpret_cast<const seq_f32x4*>(rowf + at), d4 = *reinterpret_cast<const seq_f32x4*>(rowf + C::BR + at);
+            const int4 lo4 = *reinterpret_cast<const int4*>(rowi + at), hi4 = *reinterpret_cast<const int4*>(rowi + C::BR + at),
+                       b4 = *reinterpret_cast<const int4*>(rowi + 2 * C::BR + at);
+            const int lo[4] = {lo4.x, lo4.y, lo4.z, lo4.w}, hi[4] = {hi4.x, hi4.y, hi4.z, hi4.w}, ba[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float x = s[4 * q + i], y = dp[4 * q + i];
+              seq_pair<T, cap.value, slope.value>(sc, x, y, key >= lo[i] && key < hi[i], l4[i], d4[i], ba[i] - key);
+              s[4 * q + i] = x; dp[4 * q + i] = y;
+            }
+          }
+        });
+        seq_reduce<C>(dv, gt_lds, u, dh, s);
+        seq_reduce<C>(dk, qt_lds, u, dh, dp);
+      }
+    }
+  }
+  uint32_t bad = seq_bad_rows<C>(dk, 0, red);
+  bad = seq_bad_rows<C>(dv, bad, red);
+  if (bad) seq_attn_dkv_again<C>(A, bad, row0, kvh, qbeg, qend, dh);
+  if (key >= A.tk || (bad >> (lane & 31) & 1)) return;
+  const int64_t at = ((int64_t)key * A.hk + kvh) * dbytes;
+  seq_store_own<C>(dk, A.scale, A.dk + at, nullptr, dh, A.d, A.aln);
+  seq_store_own<C>(dv, 1.f, A.dv + at, nullptr, dh, A.d, A.aln);
+}
+
+template <class C>
+static hipError_t dq(hipStream_t s, const SeqAttnArgs& A) {
+  constexpr int lds = 2 * C::kTileBytes + 2 * C::kXchBytes + C::NW * 8;
+  static DeviceMarks marks;
+  auto fn = seq_attn_dq_kernel<C>;
+  hipError_t e = marks.raise_lds(reinterpret_cast<const void*>(fn), lds);
+  if (e != hipSuccess) return e;
+  fn<<<(unsigned)((A.tq + C::RB - 1) / C::RB * A.hq), C::NT, lds, s>>>(A);
+  return hipGetLastError();
+}
+template <class C>
+static hipError_t dkv(hipStream_t s, const SeqAttnArgs& A) {
+  constexpr int lds = 2 * C::kTileBytes + 2 * C::kXchBytes + 5 * C::BR * 4 + C::NW * 8;
+  static DeviceMarks marks;
+  auto fn = seq_attn_dkv_kernel<C>;
+  hipError_t e = marks.raise_lds(reinterpret_cast<const void*>(fn), lds);
+  if (e != hipSuccess) return e;
+  fn<<<(unsigned)((A.tk + C::RB - 1) / C::RB * A.hk), C::NT, lds, s>>>(A);
+  return hipGetLastError();
+}
+template <class T>
+static hipError_t delta(hipStream_t s, const SeqAttnArgs& A) {
+  const int chunks = (A.d * (int)sizeof(T) + 15) / 16;
+  const int64_t items = (int64_t)A.tq * A.hq;
+  const auto grid = [&](int lpr) { return (unsigned)((items * lpr + 255) / 256); };
+  if (chunks <= 8) seq_attn_delta_kernel<T, 8><<<grid(8), 256, 0, s>>>(A);
+  else if (chunks <= 16) seq_attn_delta_kernel<T, 16><<<grid(16), 256, 0, s>>>(A);
+  else if (chunks <= 32) seq_attn_delta_kernel<T, 32><<<grid(32), 256, 0, s>>>(A);
+  else seq_attn_delta_kernel<T, 64><<<grid(64), 256, 0, s>>>(A);
+  return hipGetLastError();
+}
+
+template <class T, bool VEC>
+static hipError_t pick(hipStream_t s, const SeqAttnArgs& A) {
+  hipError_t e = hipSuccess;
+  if (A.tq > 0) {
+    e = delta<T>(s, A);
+    if (e != hipSuccess) return e;
+    if (A.d <= 64) e = dq<SeqTile<T, 64, 1, 4, 64, VEC>>(s, A);
+    else if (A.d <= 128) e = dq<SeqTile<T, 128, 1, 4, sizeof(T) == 2 ? 64 : 32, VEC>>(s, A);
+    else e = dq<SeqTile<T, 256, 2, 4, 32, VEC>>(s, A);
+    if (e != hipSuccess) return e;
+  }
+  if (A.tk == 0) return e;
+  if (A.d <= 64) return dkv<SeqTile<T, 64, 1, 4, 64, VEC>>(s, A);
+  if (A.d <= 128) return dkv<SeqTile<T, 128, 1, 4, 32, VEC>>(s, A);
+  return dkv<SeqTile<T, 256, 2, 4, 32, VEC>>(s, A);
+}
+
+hipError_t launch_seq_attn_backward(hipStream_t s, int bf16, const SeqAttnArgs& A) {
+  const bool vec = A.aln >= 4 && A.d * (bf16 ? 2 : 4) >= 16;
+  if (bf16) return vec ? pick<__bf16, true>(s, A) : pick<__bf16, false>(s, A);
+  return vec ? pick<float, true>(s, A) : pick<float, false>(s, A);
+}
+
+}  // namespace sttran

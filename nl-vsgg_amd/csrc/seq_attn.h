@@ -1,0 +1,354 @@
+// seq_attn.h -- what the forward and backward kernels of attention over packed sequences share (kernels_seq_attn.hip,
+// kernels_seq_attn_bwd.hip).
+//
+// One scheme for every product.  A wave owns 32 STATIONARY rows (queries; keys in the dk/dv kernel), one per lane column of a
+// 32x32 matrix-instruction block, held in registers as the B operand.  The other side STREAMS through LDS in tiles of BR rows.
+//   scores      S[stream row][own row] = sum_d X[stream row][d] Y[own row][d]      A = tile rows as they lie (16-byte reads)
+//   reductions  Z[d][own row] += sum_r W[r][d] P[r][own row]                       A = tile columns (transposed reads), B = P
+// The accumulator layout of the score block (lane = own row, 16 registers = stream rows) IS the B layout of the second product
+// once the contraction index is permuted, so probabilities go from the exponential into the next matrix instruction without
+// leaving their lane; row statistics of an own row live in one lane (plus its partner 32 lanes further).
+// bfloat16: v_mfma_f32_32x32x16_bf16, transposed reads by ds_read_b64_tr_b16; fp32: v_mfma_f32_32x32x2_f32 (exact products).
+// Head dims are padded to DP = 64 / 128 / 256 with zeros.  At DP = 256 two waves share 32 own rows, each contracting (scores)
+// and accumulating (reductions) one half of d; the partial scores are exchanged through LDS (DS = 2).
+#pragma once
+#include "seq_common.h"
+
+namespace sttran {
+
+template <class T, int DP_, int DS_, int NW_, int BR_, bool VEC_>
+struct SeqTile {
+  using E = T;
+  static constexpr bool VEC = VEC_;
+  static constexpr int DP = DP_, DS = DS_, NW = NW_, BR = BR_;
+  static constexpr int ES = sizeof(T);
+  static constexpr int NT = NW * 64;                 // threads
+  static constexpr int DH = DP / DS;                 // columns of one wave
+  static constexpr int RS = DP * ES;                 // bytes of a tile row
+  static constexpr int NC = RS / 16;                 // 16-byte chunks of a tile row
+  static constexpr int NF = DH * ES / 32;            // fragments (16 bytes a lane) of one own row's half
+  static constexpr int NB = DH / 32;                 // 32-column blocks of one wave's accumulator
+  static constexpr int NSUB = BR / 32;
+  static constexpr int RB = 32 * NW / DS;            // own rows of a workgroup
+  static constexpr int NL = BR * NC / NT;            // chunks a thread moves per tile
+  static constexpr int kTileBytes = BR * RS;
+  static constexpr int kXchBytes = DS == 2 ? NW * 4096 : 0;      // one 32x32 block of partial scores a wave
+  static_assert(BR * NC % NT == 0 && NT % NC == 0, "whole chunks, one chunk column a thread");
+};
+
+// chunk position of (row, chunk): an XOR that spreads both access patterns over the banks -- eight consecutive rows at one
+// chunk (16-byte reads of the scores) and four consecutive rows at one or two neighbouring chunks (transposed reads)
+template <class C>
+__device__ __forceinline__ int seq_swz(int row) {
+  if constexpr (C::NC == 8) return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+  else if constexpr (C::ES == 2) return ((row & 3) << 2) | ((row >> 2) & 3);
+  else return (row & 7) | (((row >> 2) & 1) << 3);
+}
+
+// ---- loads.  VEC (addresses and row lengths divisible by 4, a row of 16 bytes or more): buffer loads, whose bounds check turns
+// rows from `hi` on and chunks behind the row's end into zeros (nothing there is read, so what lies behind the last sequence
+// cannot reach a sum).  The last chunk of a row that is no multiple of 16 bytes is read as the row's last 16 bytes and shifted.
+// Otherwise (odd head dims of 2-byte elements): element by element.
+constexpr uint32_t kSeqOob = 0x80000000u;
+__device__ __forceinline__ auto seq_rsrc(const char* base, int64_t stride, int rows, int dbytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, rows > 0 ? (int)((rows - 1) * stride + dbytes) : 0, 0x00027000);
+}
+// byte offset of chunk c within a row, as the load wants it
+__device__ __forceinline__ uint32_t seq_chunk_off(int c, int dbytes) {
+  const int at = 16 * c;
+  return at + 16 <= dbytes ? (uint32_t)at : at < dbytes ? (uint32_t)(dbytes - 16) : kSeqOob;
+}
+// (selects alone: the same as an if / else if chain over the tail's length has been compiled to a path that skips one of them)
+__device__ __forceinline__ seq_u32x4 seq_tail(seq_u32x4 r, int c, int dbytes) {
+  const int rem = dbytes & 15;                       // 4, 8 or 12 where a tail exists
+  const bool t = rem != 0 && c == dbytes >> 4, t4 = t && rem == 4, t8 = t && rem == 8, t12 = t && rem == 12;
+  seq_u32x4 x;
+  x[0] = t4 ? r[3] : t8 ? r[2] : t12 ? r[1] : r[0];
+  x[1] = t4 ? 0u : t8 ? r[3] : t12 ? r[2] : r[1];
+  x[2] = t4 || t8 ? 0u : t12 ? r[3] : r[2];
+  x[3] = t ? 0u : r[3];
+  return x;
+}
+
+// tile rows row0 .. row0 + BR - 1, global -> registers; rows from `hi` on are zeros.  A thread's chunk is the same in each of its rows
+template <class C>
+__device__ __forceinline__ void seq_tile_load(seq_u32x4 (&r)[C::NL], const char* base, int64_t stride, int row0, int hi, int dbytes) {
+  const int rows = min(hi - row0, C::BR), c = threadIdx.x % C::NC;
+  if constexpr (C::VEC) {
+    const auto rs = seq_rsrc(base + (int64_t)row0 * stride, stride, rows, dbytes);
+    const uint32_t co = seq_chunk_off(c, dbytes), off = co == kSeqOob ? kSeqOob : (threadIdx.x / C::NC) * (uint32_t)stride + co;
+#pragma unroll
+    for (int i = 0; i < C::NL; ++i)
+      r[i] = __builtin_bit_cast(seq_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, off, i * (C::NT / C::NC) * (uint32_t)stride, 0));
+  } else {
+#pragma unroll
+    for (int i = 0; i < C::NL; ++i) {
+      const int row = threadIdx.x / C::NC + i * (C::NT / C::NC);
+      r[i] = seq_load16(base + (int64_t)(row0 + row) * stride + 16 * c, row < rows ? dbytes - 16 * c : 0, 2);
+    }
+  }
+}
+template <class C>
+__device__ __forceinline__ void seq_tile_store(const seq_u32x4 (&r)[C::NL], char* tile, int dbytes) {
+  const int c = threadIdx.x % C::NC;
+#pragma unroll
+  for (int i = 0; i < C::NL; ++i) {
+    const int row = threadIdx.x / C::NC + i * (C::NT / C::NC);
+    *reinterpret_cast<seq_u32x4*>(tile + row * C::RS + ((c ^ seq_swz<C>(row)) << 4)) = C::VEC ? seq_tail(r[i], c, dbytes) : r[i];
+  }
+}
+
+// own rows row0 .. row0 + 31 of this wave as B fragments
+template <class C>
+__device__ __forceinline__ void seq_own_load(seq_u32x4 (&f)[C::NF], const char* base, int64_t stride, int row0, int rows, int dh, int dbytes) {
+  const int h = (threadIdx.x >> 5) & 1, n = threadIdx.x & 31, c0 = dh * (C::DH * C::ES / 16) + h;
+  const int left = min(rows - row0, 32);
+  const char* p = base + (int64_t)row0 * stride;
+  if constexpr (C::VEC) {
+    const auto rs = seq_rsrc(p, stride, left, dbytes);
+#pragma unroll
+    for (int i = 0; i < C::NF; ++i) {
+      const int c = c0 + 2 * i;
+      const uint32_t co = seq_chunk_off(c, dbytes);
+      f[i] = seq_tail(__builtin_bit_cast(seq_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, co == kSeqOob ? kSeqOob : n * (uint32_t)stride + co, 0, 0)),
+                      c, dbytes);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < C::NF; ++i) {
+      const int c = c0 + 2 * i;
+      f[i] = seq_load16(p + (int64_t)n * stride + 16 * c, n < left ? dbytes - 16 * c : 0, 2);
+    }
+  }
+}
+
+// acc[stream row][own row] += tile . own
+template <class C>
+__device__ __forceinline__ void seq_scores(seq_f32x16& acc, const char* tile, int sub, int dh, const seq_u32x4 (&own)[C::NF]) {
+  const int lane = threadIdx.x & 63, row = 32 * sub + (lane & 31), h = lane >> 5;
+  const char* p = tile + row * C::RS;
+  const int x = (h ^ seq_swz<C>(row)) << 4;
+#pragma unroll
+  for (int f = 0; f < C::NF; ++f) {
+    const seq_u32x4 a = *reinterpret_cast<const seq_u32x4*>(p + ((dh * C::DH * C::ES + 32 * f) ^ x));
+    if constexpr (C::ES == 2) {
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(seq_bf16x8, a), __builtin_bit_cast(seq_bf16x8, own[f]), acc, 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[u]), __uint_as_float(own[f][u]), acc, 0, 0, 0);
+    }
+  }
+}
+
+// acc[d][own row] += tile^T . w, w = a score block's registers.  bfloat16: w is rounded to 8 bits of mantissa here, the one
+// rounding of probabilities (or of their derivatives) on the way into the matrix instruction; sums stay in fp32
+template <class C>
+__device__ __forceinline__ void seq_reduce(seq_f32x16 (&acc)[C::NB], const char* tile, int sub, int dh, const seq_f32x16& w) {
+  const int lane = threadIdx.x & 63;
+  if constexpr (C::ES == 2) {
+    const int g = lane >> 4, i = lane & 15, h = g >> 1;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      seq_bf16x8 b;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) b[j] = (__bf16)w[8 * t + j];
+      const int row0 = 32 * sub + 16 * t + 4 * h + (i >> 2), row1 = row0 + 8;
+      const int col = 2 * (dh * C::DH + 16 * (g & 1)) + 8 * (i & 3);                // byte within the row, block 0
+      const int x0 = seq_swz<C>(row0) << 4, x1 = seq_swz<C>(row1) << 4;
+#pragma unroll
+      for (int nb = 0; nb < C::NB; ++nb) {
+        typedef __attribute__((address_space(3))) seq_s16x4 lds_s16x4;
+        const seq_s16x4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + row0 * C::RS + ((col + 64 * nb) ^ x0)));
+        const seq_s16x4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + row1 * C::RS + ((col + 64 * nb) ^ x1)));
+        typedef short s16x8 __attribute__((ext_vector_type(8)));
+        const s16x8 a = {a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]};
+        acc[nb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(seq_bf16x8, a), b, acc[nb], 0, 0, 0);
+      }
+    }
+  } else {
+    const int m = lane & 31, h = lane >> 5;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int row = 32 * sub + 8 * (i >> 2) + 4 * h + (i & 3);
+      const int col = 4 * (dh * C::DH + m), x = seq_swz<C>(row) << 4;
+#pragma unroll
+      for (int nb = 0; nb < C::NB; ++nb) {
+        const float a = *reinterpret_cast<const float*>(tile + row * C::RS + ((col + 128 * nb) ^ x));
+        acc[nb] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, w[i], acc[nb], 0, 0, 0);
+      }
+    }
+  }
+}
+
+// Own rows (bits of the answer) whose sums are not finite.  A matrix instruction multiplies what a mask hides by an exact 0,
+// which is right unless that row holds an infinity or NaN (0 * inf): such own rows are done again, pair by pair over the
+// visible rows alone, so that what a mask hides cannot spread.  With DS == 2 the two waves of a pair share the answer.
+// Every wave of the workgroup calls this (barriers inside).
+template <class C>
+__device__ __forceinline__ uint32_t seq_bad_rows(const seq_f32x16 (&acc)[C::NB], uint32_t more, int* red) {
+  bool bad = false;
+#pragma unroll
+  for (int nb = 0; nb < C::NB; ++nb)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) bad |= !(fabsf(acc[nb][e]) < INFINITY);
+  const uint64_t b = __ballot(bad);
+  uint32_t rows = (uint32_t)b | (uint32_t)(b >> 32) | more;
+  if constexpr (C::DS == 2) {
+    const int w = threadIdx.x >> 6;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[w] = (int)rows;
+    __syncthreads();
+    rows |= (uint32_t)red[w ^ 1];
+  }
+  return rows;
+}
+
+// one row spread over a wave: lane holds columns lane, lane + 64, ...
+struct SeqSpread { float x[4]; };
+template <class T>
+__device__ __forceinline__ SeqSpread seq_spread(const char* p, int d) {
+  SeqSpread r;
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) r.x[u] = lane + 64 * u < d ? SeqElt<T>::at(p + (int64_t)(lane + 64 * u) * sizeof(T)) : 0.f;
+  return r;
+}
+__device__ __forceinline__ float seq_spread_dot(const SeqSpread& a, const SeqSpread& b) {
+  float s = 0.f;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) s = fmaf(a.x[u], b.x[u], s);
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) s += __shfl_xor(s, o);
+  return s;
+}
+template <class T>
+__device__ __forceinline__ void seq_spread_store(char* out, char* out_lo, const float (&x)[4], float mul, int d) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    if (lane + 64 * u >= d) continue;
+    const float y = x[u] * mul;
+    if constexpr (sizeof(T) == 4) {
+      reinterpret_cast<float*>(out)[lane + 64 * u] = y;
+    } else {
+      const float z = SeqElt<T>::round(y);
+      reinterpret_cast<uint16_t*>(out)[lane + 64 * u] = (uint16_t)SeqElt<T>::bits(z);
+      if (out_lo) reinterpret_cast<uint16_t*>(out_lo)[lane + 64 * u] = (uint16_t)SeqElt<T>::bits(y - z);
+    }
+  }
+}
+
+// DS == 2: add the partner wave's partial block.  Every wave of the workgroup calls this (barrier inside)
+template <class C>
+__device__ __forceinline__ void seq_exchange(seq_f32x16& s, char* xch) {
+  if constexpr (C::DS == 2) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    seq_f32x4* mine = reinterpret_cast<seq_f32x4*>(xch + w * 4096);
+    const seq_f32x4* other = reinterpret_cast<const seq_f32x4*>(xch + (w ^ 1) * 4096);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mine[i * 64 + lane] = seq_f32x4{s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]};
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const seq_f32x4 o = other[i * 64 + lane];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) s[4 * i + u] += o[u];
+    }
+  }
+}
+
+template <class C>
+__device__ __forceinline__ void seq_exchange2(seq_f32x16& a, seq_f32x16& b, char* xch) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  seq_f32x4* mine = reinterpret_cast<seq_f32x4*>(xch + w * 8192);
+  const seq_f32x4* other = reinterpret_cast<const seq_f32x4*>(xch + (w ^ 1) * 8192);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    mine[i * 64 + lane] = seq_f32x4{a[4 * i], a[4 * i + 1], a[4 * i + 2], a[4 * i + 3]};
+    mine[256 + i * 64 + lane] = seq_f32x4{b[4 * i], b[4 * i + 1], b[4 * i + 2], b[4 * i + 3]};
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const seq_f32x4 x = other[i * 64 + lane], y = other[256 + i * 64 + lane];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) { a[4 * i + u] += x[u]; b[4 * i + u] += y[u]; }
+  }
+}
+
+// Z[d][own row] registers -> a contiguous output row
+template <class C>
+__device__ __forceinline__ void seq_store_own(const seq_f32x16 (&acc)[C::NB], float mul, char* out, char* out_lo, int dh, int d, int aln) {
+  using T = typename C::E;
+  const int h = (threadIdx.x >> 5) & 1;
+#pragma unroll
+  for (int nb = 0; nb < C::NB; ++nb)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int col = dh * C::DH + 32 * nb + 8 * q + 4 * h;
+      if (col >= d) continue;
+      if constexpr (C::ES == 4) {
+        seq_u32x4 r;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) r[u] = __float_as_uint(acc[nb][4 * q + u] * mul);
+        seq_store16(out + 4 * col, r, 4 * (d - col), aln);
+      } else {
+        uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const float x = acc[nb][4 * q + u] * mul, y = SeqElt<T>::round(x);
+          hi[u >> 1] |= SeqElt<T>::bits(y) << (16 * (u & 1));
+          if (out_lo) lo[u >> 1] |= SeqElt<T>::bits(x - y) << (16 * (u & 1));
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          char* o = k ? out_lo : out;
+          const uint32_t* v = k ? lo : hi;
+          if (!o) continue;
+          if (col + 4 <= d && aln >= 8) {
+            *reinterpret_cast<uint2*>(o + 2 * col) = make_uint2(v[0], v[1]);
+          } else {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              if (col + u < d) *reinterpret_cast<uint16_t*>(o + 2 * (col + u)) = (uint16_t)(v[u >> 1] >> (16 * (u & 1)));
+          }
+        }
+      }
+    }
+}
+
+// ---- score arithmetic: z in base-2 units (z * log2 e), so that exp is one v_exp_f32 --------------------------------------
+// z = cap * tanh(scale * s / cap) - slope * |base - key|; without a cap z = scale * s - slope * |base - key|
+struct SeqScore {
+  float mul, capl, slope;                 // scale*log2e (or scale / cap), cap*log2e, slope*log2e
+  __device__ __forceinline__ SeqScore(const SeqAttnArgs& A, int head)
+      : mul(A.cap > 0.f ? A.scale / A.cap : A.scale * kSeqLog2e), capl(A.cap * kSeqLog2e), slope(A.slope ? A.slope[head] * kSeqLog2e : 0.f) {}
+};
+template <class T>
+__device__ __forceinline__ float seq_tanh(float x) {
+  if constexpr (sizeof(T) == 4) return tanhf(x);
+  // 1 - 2 / (1 + e^2x): absolute error about 1e-7, times a cap of some tens far below the rounding of the scores' inputs
+  else return 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * (2.f * kSeqLog2e)));
+}
+// one pair's z from its scaled-less product; slope_z = dz / d(scale * product) where a cap bends it
+template <class T>
+__device__ __forceinline__ float seq_z(const SeqAttnArgs& A, const SeqScore& sc, float s, int base, int key, float& slope_z) {
+  slope_z = 1.f;
+  if (A.cap > 0.f) {
+    const float t = seq_tanh<T>(s * sc.mul);
+    slope_z = 1.f - t * t;
+    s = sc.capl * t;
+  } else {
+    s *= sc.mul;
+  }
+  return A.slope ? fmaf(-sc.slope, fabsf((float)(base - key)), s) : s;
+}
+
+// workgroups of one head's neighbouring tiles on one XCD (they share its L2): blocks are dealt to the 8 XCDs in turn
+__device__ __forceinline__ int seq_xcd_order(int b, int n) {
+  const int q = n >> 3, r = n & 7, x = b & 7, i = b >> 3;
+  return x < r ? x * (q + 1) + i : r * (q + 1) + (x - r) * q + i;
+}
+
+}  // namespace sttran
