@@ -62,7 +62,11 @@ bool attention_args(const SttranAttention* a, SeqAttnArgs& A, Alignment& al) {
 }
 
 int64_t attention_workspace(const SeqAttnArgs& A, int bf16, bool backward) {
-  if (backward) return (int64_t)A.hq * A.tq * 4 + (int64_t)A.tq * 16 + 16;
+  if (backward) {
+    const int64_t rows = ((int64_t)A.hq * A.tq * 4 + (int64_t)A.tq * 16 + 16 + 255) / 256 * 256;      // ranges, delta
+    const int parts = seq_attn_dkv_splits(bf16, A);
+    return rows + (parts > 1 ? (int64_t)parts * 2 * A.tk * A.hk * A.d * 4 : 0);
+  }
   const int splits = seq_attn_splits(bf16, A);
   return splits > 1 ? (int64_t)splits * A.hq * A.tq * (A.d + 2) * 4 : 0;
 }
@@ -177,6 +181,8 @@ int sttran_attention_backward(const SttranAttention* args, void* stream) {
   if (!A.aln) return STTRAN_ERR_INVALID;
   A.rows = (int4*)args->workspace;
   A.delta = (float*)((char*)args->workspace + (int64_t)A.tq * 16);
+  A.splits = seq_attn_dkv_splits(bf16, A);
+  A.part = (float*)((char*)args->workspace + ((int64_t)A.hq * A.tq * 4 + (int64_t)A.tq * 16 + 16 + 255) / 256 * 256);
   return code(launch_seq_attn_backward(str(stream), bf16, A));
 }
 

@@ -10,6 +10,8 @@ hipError_t launch_seq_attn_forward(hipStream_t s, int bf16, const SeqAttnArgs& A
 hipError_t launch_seq_attn_backward(hipStream_t s, int bf16, const SeqAttnArgs& A);
 // how many shares of the keys a forward launch is split into (1: none), from what the host knows
 int seq_attn_splits(int bf16, const SeqAttnArgs& A);
+// ... and a backward launch's work on a key tile
+int seq_attn_dkv_splits(int bf16, const SeqAttnArgs& A);
 // joins partial outputs [split][head][row][d] + [split][head][row][2].  lens (device, per row) and chunk: only the shares that a
 // row's length fills were written (lens == nullptr: all of them)
 hipError_t launch_seq_attn_join(hipStream_t s, int bf16, const SeqAttnArgs& A, const int* lens, int chunk, int capacity);

@@ -62,19 +62,19 @@ seq_attn_fwd_kernel(SeqAttnArgs A) {
   const int kvh = head / (A.hq / A.hk), dh = C::DS == 2 ? (w & 1) : 0;
   const int row0 = tile * C::RB + 32 * (w / C::DS), row = row0 + (lane & 31);
   const int dbytes = A.d * C::ES;
+  SeqMover mv;
+  mv.init<C>(dbytes);
 
   const SeqRow me = seq_row(A, row);
   int lo = me.hi > me.lo ? me.lo : INT_MAX, hi = me.hi;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    lo = min(lo, __shfl_xor(lo, o));
-    hi = max(hi, __shfl_xor(hi, o));
-  }
+  seq_wave_range(lo, hi);
   const int wlo = lo, whi = hi;                                     // what this wave's rows see
   if (lane == 0) { red[2 * w] = lo; red[2 * w + 1] = hi; }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < C::NW; ++i) { lo = min(lo, red[2 * i]); hi = max(hi, red[2 * i + 1]); }
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  hi = __builtin_amdgcn_readfirstlane(hi);
   int beg = lo, end = max(hi, lo);
   if (hi <= 0) beg = end = 0;
   if (A.splits > 1) {                                               // this workgroup's share of the keys, whole tiles
@@ -98,17 +98,17 @@ seq_attn_fwd_kernel(SeqAttnArgs A) {
   m = -INFINITY; l = 0.f;
   seq_u32x4 kr[C::NL], vr[C::NL];
   if (beg < end) {
-    seq_tile_load<C>(kr, kp, A.k_t, beg, end, dbytes);
-    seq_tile_load<C>(vr, vp, A.v_t, beg, end, dbytes);
+    seq_tile_load<C>(mv, kr, kp, A.k_t, beg, end, dbytes);
+    seq_tile_load<C>(mv, vr, vp, A.v_t, beg, end, dbytes);
   }
   for (int kt = beg; kt < end; kt += C::BR) {
     __syncthreads();
-    seq_tile_store<C>(kr, kt_lds, dbytes);
-    seq_tile_store<C>(vr, vt_lds, dbytes);
+    seq_tile_store<C>(mv, kr, kt_lds);
+    seq_tile_store<C>(mv, vr, vt_lds);
     __syncthreads();
     if (kt + C::BR < end) {
-      seq_tile_load<C>(kr, kp, A.k_t, kt + C::BR, end, dbytes);
-      seq_tile_load<C>(vr, vp, A.v_t, kt + C::BR, end, dbytes);
+      seq_tile_load<C>(mv, kr, kp, A.k_t, kt + C::BR, end, dbytes);
+      seq_tile_load<C>(mv, vr, vp, A.v_t, kt + C::BR, end, dbytes);
     }
     const bool active = wlo < min(kt + C::BR, end) && whi > kt;
     seq_f32x16 s[C::NSUB];
@@ -275,7 +275,7 @@ static hipError_t pick(hipStream_t s, const SeqAttnArgs& A) {
 
 hipError_t launch_seq_attn_forward(hipStream_t s, int bf16, const SeqAttnArgs& A) {
   if (A.tq == 0) return hipSuccess;
-  const bool vec = A.aln >= 4 && A.d * (bf16 ? 2 : 4) >= 16;
+  const bool vec = A.aln >= 4;
   if (bf16) return vec ? pick<__bf16, true>(s, A) : pick<__bf16, false>(s, A);
   return vec ? pick<float, true>(s, A) : pick<float, false>(s, A);
 }

@@ -5,6 +5,7 @@
 // Two passes over the score blocks, each writing every output row once from one workgroup: nothing is added atomically, so
 // results do not depend on the order of workgroups (the price: 7 products where one pass with atomic adds takes 5).  Key heads
 // that several query heads share sum over them inside the workgroup.
+#include <algorithm>
 #include <type_traits>
 
 #include "kernels_seq.h"
@@ -121,6 +122,8 @@ seq_attn_dq_kernel(SeqAttnArgs A) {
   const int kvh = head / (A.hq / A.hk), dh = C::DS == 2 ? (w & 1) : 0;
   const int row0 = tile * C::RB + 32 * (w / C::DS), row = row0 + (lane & 31);
   const int dbytes = A.d * C::ES;
+  SeqMover mv;
+  mv.init<C>(dbytes);
 
   SeqRow me{0, 0, 0};
   float lse = INFINITY, delta = 0.f;
@@ -131,16 +134,14 @@ seq_attn_dq_kernel(SeqAttnArgs A) {
     delta = A.delta[(int64_t)head * A.tq + row];
   }
   int lo = me.hi > me.lo ? me.lo : INT_MAX, hi = me.hi;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    lo = min(lo, __shfl_xor(lo, o));
-    hi = max(hi, __shfl_xor(hi, o));
-  }
+  seq_wave_range(lo, hi);
   const int wlo = lo, whi = hi;
   if (lane == 0) { red[2 * w] = lo; red[2 * w + 1] = hi; }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < C::NW; ++i) { lo = min(lo, red[2 * i]); hi = max(hi, red[2 * i + 1]); }
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  hi = __builtin_amdgcn_readfirstlane(hi);
   int beg = lo, end = max(hi, lo);
   if (hi <= 0) beg = end = 0;
 
@@ -156,17 +157,17 @@ seq_attn_dq_kernel(SeqAttnArgs A) {
     for (int e = 0; e < 16; ++e) acc[nb][e] = 0.f;
   seq_u32x4 kr[C::NL], vr[C::NL];
   if (beg < end) {
-    seq_tile_load<C>(kr, kp, A.k_t, beg, end, dbytes);
-    seq_tile_load<C>(vr, vp, A.v_t, beg, end, dbytes);
+    seq_tile_load<C>(mv, kr, kp, A.k_t, beg, end, dbytes);
+    seq_tile_load<C>(mv, vr, vp, A.v_t, beg, end, dbytes);
   }
   for (int kt = beg; kt < end; kt += C::BR) {
     __syncthreads();
-    seq_tile_store<C>(kr, kt_lds, dbytes);
-    seq_tile_store<C>(vr, vt_lds, dbytes);
+    seq_tile_store<C>(mv, kr, kt_lds);
+    seq_tile_store<C>(mv, vr, vt_lds);
     __syncthreads();
     if (kt + C::BR < end) {
-      seq_tile_load<C>(kr, kp, A.k_t, kt + C::BR, end, dbytes);
-      seq_tile_load<C>(vr, vp, A.v_t, kt + C::BR, end, dbytes);
+      seq_tile_load<C>(mv, kr, kp, A.k_t, kt + C::BR, end, dbytes);
+      seq_tile_load<C>(mv, vr, vp, A.v_t, kt + C::BR, end, dbytes);
     }
 #pragma unroll 1
     for (int u = 0; u < C::NSUB; ++u) {
@@ -185,15 +186,22 @@ seq_attn_dq_kernel(SeqAttnArgs A) {
         seq_exchange2<C>(s, dp, xch);
         if (!active) continue;
       }
+      const bool full = __all(me.lo <= kb && me.hi >= kb + 32);
       seq_by_score(A, [&](auto cap, auto slope) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const int key = kb + 4 * h + 8 * (e >> 2) + (e & 3);
           float x = s[e], y = dp[e];
-          seq_pair<T, cap.value, slope.value>(sc, x, y, key >= me.lo && key < me.hi, lse, delta, me.base - key);
+          seq_pair<T, cap.value, slope.value>(sc, x, y, true, lse, delta, me.base - kb - 4 * h - 8 * (e >> 2) - (e & 3));
           dp[e] = y;
         }
       });
+      if (!full) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int key = kb + 4 * h + 8 * (e >> 2) + (e & 3);
+          dp[e] = key >= me.lo && key < me.hi ? dp[e] : 0.f;
+        }
+      }
       seq_reduce<C>(acc, kt_lds, u, dh, dp);
     }
   }
@@ -204,10 +212,13 @@ seq_attn_dq_kernel(SeqAttnArgs A) {
 }
 
 // ---- dk, dv: own rows = keys, queries and dout stream ---------------------------------------------------------------------
+// The work of a key tile -- (query head of the group, tile of query rows) in this order -- may be cut into A.splits shares of equal
+// length, one workgroup each: i0 .. i1 here
 template <class C>
-__device__ __forceinline__ void seq_attn_dkv_again(const SeqAttnArgs& A, uint32_t rows, int row0, int kvh, int qbeg, int qend, int dh) {
+__device__ __forceinline__ void seq_attn_dkv_again(const SeqAttnArgs& A, uint32_t rows, int row0, int kvh, int qbeg, int qend, int i0, int i1,
+                                                   int dh, float* part) {
   using T = typename C::E;
-  const int grp = A.hq / A.hk;
+  const int grp = A.hq / A.hk, nt = (qend - qbeg + C::BR - 1) / C::BR;
 #pragma unroll 1
   for (int n = 0; n < 32; ++n) {
     const int key = row0 + n;
@@ -216,11 +227,11 @@ __device__ __forceinline__ void seq_attn_dkv_again(const SeqAttnArgs& A, uint32_
     const SeqSpread v = seq_spread<T>(A.v + kvh * A.v_h + (int64_t)key * A.v_t, A.d);
     float dk[4] = {0.f, 0.f, 0.f, 0.f}, dv[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
-    for (int g = 0; g < grp; ++g) {
-      const int head = kvh * grp + g;
+    for (int it = i0; it < i1; ++it) {
+      const int head = kvh * grp + it / nt, q0 = qbeg + it % nt * C::BR, q1 = min(q0 + C::BR, qend);
       const SeqScore sc(A, head);
 #pragma unroll 1
-      for (int row = qbeg; row < qend; ++row) {
+      for (int row = q0; row < q1; ++row) {
         const int4 r = A.rows[row];
         if (key < r.x || key >= r.y) continue;
         const SeqSpread q = seq_spread<T>(A.q + head * A.q_h + (int64_t)row * A.q_t, A.d);
@@ -234,14 +245,19 @@ __device__ __forceinline__ void seq_attn_dkv_again(const SeqAttnArgs& A, uint32_
         }
       }
     }
-    const int64_t at = ((int64_t)key * A.hk + kvh) * A.d * C::ES;
-    seq_spread_store<T>(A.dk + at, nullptr, dk, A.scale, A.d);
-    seq_spread_store<T>(A.dv + at, nullptr, dv, 1.f, A.d);
+    const int64_t at = ((int64_t)key * A.hk + kvh) * A.d;
+    if (part) {
+      seq_spread_store<float>((char*)(part + at), nullptr, dk, A.scale, A.d);
+      seq_spread_store<float>((char*)(part + (int64_t)A.tk * A.hk * A.d + at), nullptr, dv, 1.f, A.d);
+    } else {
+      seq_spread_store<T>(A.dk + at * C::ES, nullptr, dk, A.scale, A.d);
+      seq_spread_store<T>(A.dv + at * C::ES, nullptr, dv, 1.f, A.d);
+    }
   }
 }
 
 template <class C>
-__global__ void __launch_bounds__(C::NT) __attribute__((amdgpu_waves_per_eu(C::ES == 4 && C::DS == 2 ? 1 : 2, C::ES == 4 && C::DS == 2 ? 1 : 2)))
+__global__ void __launch_bounds__(C::NT) __attribute__((amdgpu_waves_per_eu(C::DH == 128 ? 1 : 2, C::DH == 128 ? 1 : 2)))
 seq_attn_dkv_kernel(SeqAttnArgs A) {
   using T = typename C::E;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -255,6 +271,8 @@ seq_attn_dkv_kernel(SeqAttnArgs A) {
   const int kvh = id / tiles, tile = id % tiles, dh = C::DS == 2 ? (w & 1) : 0;
   const int first = tile * C::RB, row0 = first + 32 * (w / C::DS), key = row0 + (lane & 31);
   const int dbytes = A.d * C::ES;
+  SeqMover mv;
+  mv.init<C>(dbytes);
 
   // query rows that may see a key of this tile: those of the sequences that the tile touches
   int qbeg = 0, qend = 0;
@@ -268,7 +286,8 @@ seq_attn_dkv_kernel(SeqAttnArgs A) {
         const int lq = A.off_q[s0 + 1] - qbeg, lk = A.off_k[s0 + 1] - A.off_k[s0];
         qbeg += min(max(at - (lk - lq), 0), max(lq, 0));
       }
-      qbeg = min(max(qbeg, 0), A.tq);
+      qbeg = __builtin_amdgcn_readfirstlane(min(max(qbeg, 0), A.tq));
+      qend = __builtin_amdgcn_readfirstlane(qend);
     }
   }
 
@@ -281,31 +300,39 @@ seq_attn_dkv_kernel(SeqAttnArgs A) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) { dk[nb][e] = 0.f; dv[nb][e] = 0.f; }
 
-  for (int g = 0; g < grp; ++g) {
-    const int head = kvh * grp + g;
-    const char *qp = A.q + head * A.q_h, *gp = A.dout + head * A.do_h;
-    const float *lse = A.lse + (int64_t)head * A.tq, *delta = A.delta + (int64_t)head * A.tq;
-    const SeqScore sc(A, head);
+  const int nt = (qend - qbeg + C::BR - 1) / C::BR;
+  int i0 = 0, i1 = qbeg < qend ? grp * nt : 0;
+  if (A.splits > 1) {
+    const int64_t all = i1;
+    i0 = (int)(all * blockIdx.y / A.splits);
+    i1 = (int)(all * (blockIdx.y + 1) / A.splits);
+  }
+  {
     seq_u32x4 qr[C::NL], gr[C::NL];
     float rf[2] = {INFINITY, 0.f};
     int4 ri = make_int4(0, 0, 0, 0);
-    const auto load = [&](int qt) {
-      seq_tile_load<C>(qr, qp, A.q_t, qt, qend, dbytes);
-      seq_tile_load<C>(gr, gp, A.do_t, qt, qend, dbytes);
+    const auto load = [&](int it) {
+      const int head = kvh * grp + it / nt, qt = qbeg + it % nt * C::BR;
+      seq_tile_load<C>(mv, qr, A.q + head * A.q_h, A.q_t, qt, qend, dbytes);
+      seq_tile_load<C>(mv, gr, A.dout + head * A.do_h, A.do_t, qt, qend, dbytes);
       rf[0] = INFINITY; rf[1] = 0.f; ri = make_int4(0, 0, 0, 0);
-      if (tid < C::BR && qt + tid < qend) { rf[0] = lse[qt + tid]; rf[1] = delta[qt + tid]; ri = A.rows[qt + tid]; }
+      if (tid < C::BR && qt + tid < qend) {
+        const int64_t at = (int64_t)head * A.tq + qt + tid;
+        rf[0] = A.lse[at]; rf[1] = A.delta[at]; ri = A.rows[qt + tid];
+      }
     };
-    if (qbeg < qend) load(qbeg);
-    for (int qt = qbeg; qt < qend; qt += C::BR) {
+    if (i0 < i1) load(i0);
+    for (int it = i0; it < i1; ++it) {
+      const SeqScore sc(A, kvh * grp + it / nt);
       __syncthreads();
-      seq_tile_store<C>(qr, qt_lds, dbytes);
-      seq_tile_store<C>(gr, gt_lds, dbytes);
+      seq_tile_store<C>(mv, qr, qt_lds);
+      seq_tile_store<C>(mv, gr, gt_lds);
       if (tid < C::BR) {
         rowf[tid] = rf[0]; rowf[C::BR + tid] = rf[1];
         rowi[tid] = ri.x; rowi[C::BR + tid] = ri.y; rowi[2 * C::BR + tid] = ri.z;
       }
       __syncthreads();
-      if (qt + C::BR < qend) load(qt + C::BR);
+      if (it + 1 < i1) load(it + 1);
 #pragma unroll 1
       for (int u = 0; u < C::NSUB; ++u) {
         const int rl = rowi[32 * u + (lane & 31)], rh = rowi[C::BR + 32 * u + (lane & 31)];
@@ -323,22 +350,41 @@ seq_attn_dkv_kernel(SeqAttnArgs A) {
           seq_exchange2<C>(s, dp, xch);
           if (!active) continue;
         }
+        const bool full = __all(rl <= row0 && rh >= row0 + 32);
         seq_by_score(A, [&](auto cap, auto slope) {
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             const int at = 32 * u + 8 * q + 4 * h;
             const seq_f32x4 l4 = *reinterpret_cast<const seq_f32x4*>(rowf + at), d4 = *reinterpret_cast<const seq_f32x4*>(rowf + C::BR + at);
-            const int4 lo4 = *reinterpret_cast<const int4*>(rowi + at), hi4 = *reinterpret_cast<const int4*>(rowi + C::BR + at),
-                       b4 = *reinterpret_cast<const int4*>(rowi + 2 * C::BR + at);
-            const int lo[4] = {lo4.x, lo4.y, lo4.z, lo4.w}, hi[4] = {hi4.x, hi4.y, hi4.z, hi4.w}, ba[4] = {b4.x, b4.y, b4.z, b4.w};
+            int ba[4] = {0, 0, 0, 0};
+            if constexpr (slope.value) {
+              const int4 b4 = *reinterpret_cast<const int4*>(rowi + 2 * C::BR + at);
+              ba[0] = b4.x; ba[1] = b4.y; ba[2] = b4.z; ba[3] = b4.w;
+            }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               float x = s[4 * q + i], y = dp[4 * q + i];
-              seq_pair<T, cap.value, slope.value>(sc, x, y, key >= lo[i] && key < hi[i], l4[i], d4[i], ba[i] - key);
+              seq_pair<T, cap.value, slope.value>(sc, x, y, true, l4[i], d4[i], ba[i] - key);
               s[4 * q + i] = x; dp[4 * q + i] = y;
             }
+            __builtin_amdgcn_sched_barrier(0);                           // or all four groups' statistics are fetched at once
           }
         });
+        if (!full) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int at = 32 * u + 8 * q + 4 * h;
+            const int4 lo4 = *reinterpret_cast<const int4*>(rowi + at), hi4 = *reinterpret_cast<const int4*>(rowi + C::BR + at);
+            const int lo[4] = {lo4.x, lo4.y, lo4.z, lo4.w}, hi[4] = {hi4.x, hi4.y, hi4.z, hi4.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const bool seen = key >= lo[i] && key < hi[i];
+              s[4 * q + i] = seen ? s[4 * q + i] : 0.f;
+              dp[4 * q + i] = seen ? dp[4 * q + i] : 0.f;
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
         seq_reduce<C>(dv, gt_lds, u, dh, s);
         seq_reduce<C>(dk, qt_lds, u, dh, dp);
       }
@@ -346,11 +392,51 @@ seq_attn_dkv_kernel(SeqAttnArgs A) {
   }
   uint32_t bad = seq_bad_rows<C>(dk, 0, red);
   bad = seq_bad_rows<C>(dv, bad, red);
-  if (bad) seq_attn_dkv_again<C>(A, bad, row0, kvh, qbeg, qend, dh);
+  float* part = A.splits > 1 ? A.part + 2 * blockIdx.y * ((int64_t)A.tk * A.hk * A.d) : nullptr;
+  if (bad) seq_attn_dkv_again<C>(A, bad, row0, kvh, qbeg, qend, i0, i1, dh, part);
   if (key >= A.tk || (bad >> (lane & 31) & 1)) return;
+  if (part) {
+    const int64_t to = ((int64_t)key * A.hk + kvh) * A.d;
+    seq_store_part<C>(dk, A.scale, part + to, dh, A.d, 4);
+    seq_store_part<C>(dv, 1.f, part + (int64_t)A.tk * A.hk * A.d + to, dh, A.d, 4);
+    return;
+  }
   const int64_t at = ((int64_t)key * A.hk + kvh) * dbytes;
   seq_store_own<C>(dk, A.scale, A.dk + at, nullptr, dh, A.d, A.aln);
   seq_store_own<C>(dv, 1.f, A.dv + at, nullptr, dh, A.d, A.aln);
+}
+
+// dk, dv from the shares' partial sums, in the order of the shares: four elements a thread (n: elements of one of them)
+template <class T>
+__global__ void __launch_bounds__(256) seq_attn_dkv_join_kernel(SeqAttnArgs A, int64_t n) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  const int left = (int)min((int64_t)4, n - i);
+  const float* p = A.part + blockIdx.y * n + i;
+  float x[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < A.splits; ++s, p += 2 * n) {
+    const seq_u32x4 r = seq_load16((const char*)p, 4 * left, 4);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) x[u] += __uint_as_float(r[u]);
+  }
+  T* out = reinterpret_cast<T*>(blockIdx.y ? A.dv : A.dk) + i;
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    if (u < left) out[u] = (T)x[u];
+}
+
+// into how many shares a key tile's work is cut: none with 1024 workgroups or more (4 a CU: as the order masks, their work differs by
+// up to the whole length), else as many as bring it there, 8 at most, within 512 MB of partial sums
+int seq_attn_dkv_splits(int bf16, const SeqAttnArgs& A) {
+  const int rb = A.d > 128 ? 64 : 128;
+  const int64_t wgs = ((int64_t)A.tk + rb - 1) / rb * A.hk, bytes = (int64_t)A.tk * A.hk * A.d * 8;
+  if (wgs == 0 || wgs >= 1024) return 1;
+  const int64_t work = (int64_t)(A.hq / A.hk) * ((A.tq / (A.nseq > 0 ? A.nseq : 1) + 31) / 32);       // query tiles a key tile sees, about
+  int64_t n = (1024 + wgs - 1) / wgs;
+  n = std::min<int64_t>(n, 8);
+  n = std::min<int64_t>(n, work / 8);                        // a share is 8 tiles at least
+  n = std::min<int64_t>(n, (int64_t(512) << 20) / std::max<int64_t>(bytes, 1));
+  return (int)std::max<int64_t>(n, 1);
 }
 
 template <class C>
@@ -370,7 +456,11 @@ static hipError_t dkv(hipStream_t s, const SeqAttnArgs& A) {
   auto fn = seq_attn_dkv_kernel<C>;
   hipError_t e = marks.raise_lds(reinterpret_cast<const void*>(fn), lds);
   if (e != hipSuccess) return e;
-  fn<<<(unsigned)((A.tk + C::RB - 1) / C::RB * A.hk), C::NT, lds, s>>>(A);
+  fn<<<dim3((unsigned)((A.tk + C::RB - 1) / C::RB * A.hk), (unsigned)A.splits), C::NT, lds, s>>>(A);
+  e = hipGetLastError();
+  if (e != hipSuccess || A.splits == 1) return e;
+  const int64_t n = (int64_t)A.tk * A.hk * A.d;
+  seq_attn_dkv_join_kernel<typename C::E><<<dim3((unsigned)((n + 1023) / 1024), 2), 256, 0, s>>>(A, n);
   return hipGetLastError();
 }
 template <class T>
@@ -403,7 +493,7 @@ static hipError_t pick(hipStream_t s, const SeqAttnArgs& A) {
 }
 
 hipError_t launch_seq_attn_backward(hipStream_t s, int bf16, const SeqAttnArgs& A) {
-  const bool vec = A.aln >= 4 && A.d * (bf16 ? 2 : 4) >= 16;
+  const bool vec = A.aln >= 4;
   if (bf16) return vec ? pick<__bf16, true>(s, A) : pick<__bf16, false>(s, A);
   return vec ? pick<float, true>(s, A) : pick<float, false>(s, A);
 }

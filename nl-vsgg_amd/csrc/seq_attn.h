@@ -45,56 +45,57 @@ __device__ __forceinline__ int seq_swz(int row) {
   else return (row & 7) | (((row >> 2) & 1) << 3);
 }
 
-// ---- loads.  VEC (addresses and row lengths divisible by 4, a row of 16 bytes or more): buffer loads, whose bounds check turns
-// rows from `hi` on and chunks behind the row's end into zeros (nothing there is read, so what lies behind the last sequence
-// cannot reach a sum).  The last chunk of a row that is no multiple of 16 bytes is read as the row's last 16 bytes and shifted.
-// Otherwise (odd head dims of 2-byte elements): element by element.
+// ---- loads.  VEC (addresses and row lengths divisible by 4): buffer loads, whose bounds check -- dword by dword -- turns rows from
+// `hi` on into zeros (nothing there is read, so what lies behind the last sequence cannot reach a sum); what a row's last chunk
+// reads behind the row's end is masked off.  Otherwise (odd head dims of 2-byte elements): element by element.
 constexpr uint32_t kSeqOob = 0x80000000u;
 __device__ __forceinline__ auto seq_rsrc(const char* base, int64_t stride, int rows, int dbytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, rows > 0 ? (int)((rows - 1) * stride + dbytes) : 0, 0x00027000);
 }
-// byte offset of chunk c within a row, as the load wants it
-__device__ __forceinline__ uint32_t seq_chunk_off(int c, int dbytes) {
-  const int at = 16 * c;
-  return at + 16 <= dbytes ? (uint32_t)at : at < dbytes ? (uint32_t)(dbytes - 16) : kSeqOob;
-}
-// (selects alone: the same as an if / else if chain over the tail's length has been compiled to a path that skips one of them)
-__device__ __forceinline__ seq_u32x4 seq_tail(seq_u32x4 r, int c, int dbytes) {
-  const int rem = dbytes & 15;                       // 4, 8 or 12 where a tail exists
-  const bool t = rem != 0 && c == dbytes >> 4, t4 = t && rem == 4, t8 = t && rem == 8, t12 = t && rem == 12;
-  seq_u32x4 x;
-  x[0] = t4 ? r[3] : t8 ? r[2] : t12 ? r[1] : r[0];
-  x[1] = t4 ? 0u : t8 ? r[3] : t12 ? r[2] : r[1];
-  x[2] = t4 || t8 ? 0u : t12 ? r[3] : r[2];
-  x[3] = t ? 0u : r[3];
-  return x;
+// masks of the four dwords of chunk c: all ones within the row
+__device__ __forceinline__ seq_u32x4 seq_chunk_mask(int c, int dbytes) {
+  seq_u32x4 m;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) m[u] = 16 * c + 4 * u < dbytes ? 0xffffffffu : 0u;
+  return m;
 }
 
-// tile rows row0 .. row0 + BR - 1, global -> registers; rows from `hi` on are zeros.  A thread's chunk is the same in each of its rows
+// what a thread keeps for moving tiles: its chunk column (the same in each of its rows), the offset of its first row's chunk and the
+// chunk's mask
+struct SeqMover {
+  uint32_t row, c;
+  seq_u32x4 mask;
+  template <class C>
+  __device__ __forceinline__ void init(int dbytes) {
+    row = threadIdx.x / C::NC; c = threadIdx.x % C::NC;
+    mask = seq_chunk_mask(c, dbytes);
+  }
+};
+// tile rows row0 .. row0 + BR - 1, global -> registers; rows from `hi` on are zeros (row0, hi: the same in every lane)
 template <class C>
-__device__ __forceinline__ void seq_tile_load(seq_u32x4 (&r)[C::NL], const char* base, int64_t stride, int row0, int hi, int dbytes) {
-  const int rows = min(hi - row0, C::BR), c = threadIdx.x % C::NC;
+__device__ __forceinline__ void seq_tile_load(const SeqMover& mv, seq_u32x4 (&r)[C::NL], const char* base, int64_t stride, int row0, int hi,
+                                              int dbytes) {
+  const int rows = min(hi - row0, C::BR);
   if constexpr (C::VEC) {
     const auto rs = seq_rsrc(base + (int64_t)row0 * stride, stride, rows, dbytes);
-    const uint32_t co = seq_chunk_off(c, dbytes), off = co == kSeqOob ? kSeqOob : (threadIdx.x / C::NC) * (uint32_t)stride + co;
+    const uint32_t at = 16 * mv.c, off = at < (uint32_t)dbytes ? mv.row * (uint32_t)stride + at : kSeqOob;
 #pragma unroll
     for (int i = 0; i < C::NL; ++i)
       r[i] = __builtin_bit_cast(seq_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, off, i * (C::NT / C::NC) * (uint32_t)stride, 0));
   } else {
 #pragma unroll
     for (int i = 0; i < C::NL; ++i) {
-      const int row = threadIdx.x / C::NC + i * (C::NT / C::NC);
-      r[i] = seq_load16(base + (int64_t)(row0 + row) * stride + 16 * c, row < rows ? dbytes - 16 * c : 0, 2);
+      const int row = (int)mv.row + i * (C::NT / C::NC);
+      r[i] = seq_load16(base + (int64_t)(row0 + row) * stride + 16 * mv.c, row < rows ? dbytes - 16 * (int)mv.c : 0, 2);
     }
   }
 }
 template <class C>
-__device__ __forceinline__ void seq_tile_store(const seq_u32x4 (&r)[C::NL], char* tile, int dbytes) {
-  const int c = threadIdx.x % C::NC;
+__device__ __forceinline__ void seq_tile_store(const SeqMover& mv, const seq_u32x4 (&r)[C::NL], char* tile) {
 #pragma unroll
   for (int i = 0; i < C::NL; ++i) {
-    const int row = threadIdx.x / C::NC + i * (C::NT / C::NC);
-    *reinterpret_cast<seq_u32x4*>(tile + row * C::RS + ((c ^ seq_swz<C>(row)) << 4)) = C::VEC ? seq_tail(r[i], c, dbytes) : r[i];
+    const int row = (int)mv.row + i * (C::NT / C::NC);
+    *reinterpret_cast<seq_u32x4*>(tile + row * C::RS + ((mv.c ^ seq_swz<C>(row)) << 4)) = r[i] & mv.mask;
   }
 }
 
@@ -108,11 +109,11 @@ __device__ __forceinline__ void seq_own_load(seq_u32x4 (&f)[C::NF], const char* 
     const auto rs = seq_rsrc(p, stride, left, dbytes);
 #pragma unroll
     for (int i = 0; i < C::NF; ++i) {
-      const int c = c0 + 2 * i;
-      const uint32_t co = seq_chunk_off(c, dbytes);
-      f[i] = seq_tail(__builtin_bit_cast(seq_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, co == kSeqOob ? kSeqOob : n * (uint32_t)stride + co, 0, 0)),
-                      c, dbytes);
+      const int at = 16 * (c0 + 2 * i);
+      f[i] = __builtin_bit_cast(seq_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, at < dbytes ? n * (uint32_t)stride + at : kSeqOob, 0, 0));
     }
+#pragma unroll
+    for (int i = 0; i < C::NF; ++i) f[i] &= seq_chunk_mask(c0 + 2 * i, dbytes);
   } else {
 #pragma unroll
     for (int i = 0; i < C::NF; ++i) {
@@ -120,6 +121,17 @@ __device__ __forceinline__ void seq_own_load(seq_u32x4 (&f)[C::NF], const char* 
       f[i] = seq_load16(p + (int64_t)n * stride + 16 * c, n < left ? dbytes - 16 * c : 0, 2);
     }
   }
+}
+
+// smallest lo and largest hi over the lanes of a wave
+__device__ __forceinline__ void seq_wave_range(int& lo, int& hi) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    lo = min(lo, __shfl_xor(lo, o));
+    hi = max(hi, __shfl_xor(hi, o));
+  }
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  hi = __builtin_amdgcn_readfirstlane(hi);
 }
 
 // acc[stream row][own row] += tile . own
@@ -318,6 +330,23 @@ __device__ __forceinline__ void seq_store_own(const seq_f32x16 (&acc)[C::NB], fl
     }
 }
 
+// ... -> a row of fp32 partial sums
+template <class C>
+__device__ __forceinline__ void seq_store_part(const seq_f32x16 (&acc)[C::NB], float mul, float* out, int dh, int d, int aln) {
+  const int h = (threadIdx.x >> 5) & 1;
+#pragma unroll
+  for (int nb = 0; nb < C::NB; ++nb)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int col = dh * C::DH + 32 * nb + 8 * q + 4 * h;
+      if (col >= d) continue;
+      seq_u32x4 r;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) r[u] = __float_as_uint(acc[nb][4 * q + u] * mul);
+      seq_store16(reinterpret_cast<char*>(out + col), r, 4 * (d - col), aln);
+    }
+}
+
 // ---- score arithmetic: z in base-2 units (z * log2 e), so that exp is one v_exp_f32 --------------------------------------
 // z = cap * tanh(scale * s / cap) - slope * |base - key|; without a cap z = scale * s - slope * |base - key|
 struct SeqScore {
@@ -325,11 +354,23 @@ struct SeqScore {
   __device__ __forceinline__ SeqScore(const SeqAttnArgs& A, int head)
       : mul(A.cap > 0.f ? A.scale / A.cap : A.scale * kSeqLog2e), capl(A.cap * kSeqLog2e), slope(A.slope ? A.slope[head] * kSeqLog2e : 0.f) {}
 };
+// Without branches.  bfloat16: 1 - 2 / (1 + e^2x), absolute error about 1e-7, times a cap of some tens far below the rounding of the
+// scores' inputs.  fp32: that form from |x| = 0.55 on (where it is good to 3 * 2^-24 of itself), below it the Taylor series up to
+// x^15 (its next term is under 2^-24 of x there)
 template <class T>
 __device__ __forceinline__ float seq_tanh(float x) {
-  if constexpr (sizeof(T) == 4) return tanhf(x);
-  // 1 - 2 / (1 + e^2x): absolute error about 1e-7, times a cap of some tens far below the rounding of the scores' inputs
-  else return 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * (2.f * kSeqLog2e)));
+  const float big = 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f((sizeof(T) == 4 ? fabsf(x) : x) * (2.f * kSeqLog2e)));
+  if constexpr (sizeof(T) == 2) return big;
+  const float y = x * x;
+  float p = -929569.f / 638512875.f;
+  p = fmaf(p, y, 21844.f / 6081075.f);
+  p = fmaf(p, y, -1382.f / 155925.f);
+  p = fmaf(p, y, 62.f / 2835.f);
+  p = fmaf(p, y, -17.f / 315.f);
+  p = fmaf(p, y, 2.f / 15.f);
+  p = fmaf(p, y, -1.f / 3.f);
+  const float small = fmaf(p * y, x, x);
+  return fabsf(x) < 0.55f ? small : copysignf(big, x);
 }
 // one pair's z from its scaled-less product; slope_z = dz / d(scale * product) where a cap bends it
 template <class T>
