@@ -15,7 +15,7 @@ __device__ __forceinline__ void seq_attn_fwd_again(const SeqAttnArgs& A, const S
 #pragma unroll 1
   for (int n = 0; n < 32; ++n) {
     const int row = row0 + n;
-    if (!(rows >> n & 1) || row >= A.tq || (C::DS == 2 && (n & 1) != dh)) continue;
+    if (!(rows >> n & 1) || row >= A.tq || n % C::DS != dh) continue;
     const int lo = max(__shfl(me.lo, n), beg), hi = min(__shfl(me.hi, n), end), base = __shfl(me.base, n);
     const SeqSpread q = seq_spread<T>(A.q + head * A.q_h + (int64_t)row * A.q_t, A.d);
     float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f}, unused;
@@ -49,21 +49,24 @@ __device__ __forceinline__ void seq_attn_fwd_again(const SeqAttnArgs& A, const S
 // only when the maximum grows by more than 8 (a factor of 256): p stays below 2^8 and the final division by l undoes any
 // common factor exactly as the textbook form does.
 template <class C>
+struct SeqFwdLds {                                       // DS == 1: two tiles of keys and of values; else one of each and the exchange
+  static constexpr int kBufs = C::DS == 1 ? 2 : 1;
+  static constexpr int kXch = 2 * kBufs * C::kTileBytes, kRed = kXch + (C::DS > 1 ? C::NW * 4096 : 0), kBytes = kRed + C::NW * 8;
+};
+template <class C>
 __global__ void __launch_bounds__(C::NT) __attribute__((amdgpu_waves_per_eu(2, 2)))
 seq_attn_fwd_kernel(SeqAttnArgs A) {
   using T = typename C::E;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  char *kt_lds = smem, *vt_lds = smem + C::kTileBytes, *xch = smem + 2 * C::kTileBytes;
-  int* red = reinterpret_cast<int*>(xch + C::kXchBytes);
+  char* xch = smem + SeqFwdLds<C>::kXch;
+  int* red = reinterpret_cast<int*>(smem + SeqFwdLds<C>::kRed);
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int tiles = (A.tq + C::RB - 1) / C::RB;
   const int id = seq_xcd_order(blockIdx.x, gridDim.x);
   const int head = id / tiles, tile = tiles - 1 - id % tiles;      // rows that see most keys first where the order masks
-  const int kvh = head / (A.hq / A.hk), dh = C::DS == 2 ? (w & 1) : 0;
+  const int kvh = head / (A.hq / A.hk), dh = w % C::DS;
   const int row0 = tile * C::RB + 32 * (w / C::DS), row = row0 + (lane & 31);
   const int dbytes = A.d * C::ES;
-  SeqMover mv;
-  mv.init<C>(dbytes);
 
   const SeqRow me = seq_row(A, row);
   int lo = me.hi > me.lo ? me.lo : INT_MAX, hi = me.hi;
@@ -83,94 +86,116 @@ seq_attn_fwd_kernel(SeqAttnArgs A) {
     end = min(beg + per, end);
   }
 
+  const char *kp = A.k + kvh * A.k_h, *vp = A.v + kvh * A.v_h;
+  SeqMover mk, mv;
+  mk.init<C>(A.k_t, dbytes);
+  mv.init<C>(A.v_t, dbytes);
+  char *kt_lds = smem, *vt_lds = smem + C::kTileBytes;
+  if (beg < end) {
+    seq_tile_move<C>(mk, kt_lds, kp, A.k_t, beg, end, dbytes);
+    seq_tile_move<C>(mv, vt_lds, vp, A.v_t, beg, end, dbytes);
+  }
   seq_u32x4 own[C::NF];
   seq_own_load<C>(own, A.q + head * A.q_h, A.q_t, row0, A.tq, dh, dbytes);
-  const char *kp = A.k + kvh * A.k_h, *vp = A.v + kvh * A.v_h;
   const SeqScore sc(A, head);
   const bool capped = A.cap > 0.f;
-
+  const int rlo = max(me.lo, beg), rhi = min(me.hi, end);           // this lane's visible keys of this workgroup
   seq_f32x16 acc[C::NB];
-  float m, l;
 #pragma unroll
   for (int nb = 0; nb < C::NB; ++nb)
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[nb][e] = 0.f;
-  m = -INFINITY; l = 0.f;
-  seq_u32x4 kr[C::NL], vr[C::NL];
-  if (beg < end) {
-    seq_tile_load<C>(mv, kr, kp, A.k_t, beg, end, dbytes);
-    seq_tile_load<C>(mv, vr, vp, A.v_t, beg, end, dbytes);
-  }
-  for (int kt = beg; kt < end; kt += C::BR) {
-    __syncthreads();
-    seq_tile_store<C>(mv, kr, kt_lds);
-    seq_tile_store<C>(mv, vr, vt_lds);
-    __syncthreads();
-    if (kt + C::BR < end) {
-      seq_tile_load<C>(mv, kr, kp, A.k_t, kt + C::BR, end, dbytes);
-      seq_tile_load<C>(mv, vr, vp, A.v_t, kt + C::BR, end, dbytes);
+  float m = -INFINITY, l = 0.f;
+  seq_tile_done<C>(mk, kt_lds, dbytes);
+  seq_tile_done<C>(mv, vt_lds, dbytes);
+  __syncthreads();
+
+  for (int kt = beg, buf = 0; kt < end; kt += C::BR) {
+    const bool more = kt + C::BR < end, active = wlo < min(kt + C::BR, end) && whi > kt;
+    char *kn = kt_lds, *vn = vt_lds;
+    if constexpr (C::DS == 1) {
+      kn = smem + (buf ^ 1) * 2 * C::kTileBytes;
+      vn = kn + C::kTileBytes;
+      if (more) {
+        seq_tile_move<C>(mk, kn, kp, A.k_t, kt + C::BR, end, dbytes);
+        seq_tile_move<C>(mv, vn, vp, A.v_t, kt + C::BR, end, dbytes);
+      }
     }
-    const bool active = wlo < min(kt + C::BR, end) && whi > kt;
     seq_f32x16 s[C::NSUB];
-    if (active || C::DS == 2) {
+    if (active) {
 #pragma unroll
       for (int u = 0; u < C::NSUB; ++u) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[u][e] = 0.f;
-        if (active) seq_scores<C>(s[u], kt_lds, u, dh, own);
-        if (C::DS == 2) {
-          if (u > 0) __syncthreads();
-          seq_exchange<C>(s[u], xch);
-        }
+        seq_scores<C>(s[u], kt_lds, u, dh, own);
       }
     }
-    if (!active) continue;
-    const int rlo = max(me.lo, beg), rhi = min(me.hi, end);        // this lane's visible keys of this workgroup
-    const bool full = __all(rlo <= kt && rhi >= kt + C::BR);
-    float mt = -INFINITY;
+    if constexpr (C::DS == 2) {
+      static_assert(C::NSUB == 1, "one block is exchanged");
+      if (active) seq_put<C>(s[0], xch, w, 1, 0);
+      seq_tile_done<C>(mv, vt_lds, dbytes);
+      __syncthreads();                                               // keys are free, values and partial scores are there
+      if (more) seq_tile_move<C>(mk, kn, kp, A.k_t, kt + C::BR, end, dbytes);
+      if (active) seq_get<C>(s[0], xch, w, 1, 0);
+    }
+    if (active) {
+      const bool full = __all(rlo <= kt && rhi >= kt + C::BR);
+      float mt = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < C::NSUB; ++u) {
-      if (capped) {
+      for (int u = 0; u < C::NSUB; ++u) {
+        if (capped) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[u][e] = sc.capl * seq_tanh<T>(s[u][e] * sc.mul);
-      } else {
+          for (int e = 0; e < 16; ++e) s[u][e] = sc.capl * seq_tanh<T>(s[u][e] * sc.mul);
+        } else {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[u][e] *= sc.mul;
+          for (int e = 0; e < 16; ++e) s[u][e] *= sc.mul;
+        }
+        const int k0 = kt + 32 * u + 4 * h;
+        if (A.slope) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[u][e] = fmaf(-sc.slope, fabsf((float)(me.base - k0 - 8 * (e >> 2) - (e & 3))), s[u][e]);
+        }
+        if (!full) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int key = k0 + 8 * (e >> 2) + (e & 3);
+            s[u][e] = key >= rlo && key < rhi ? s[u][e] : -INFINITY;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[u][e]);
       }
-      const int k0 = kt + 32 * u + 4 * h;
-      if (A.slope) {
+      mt = fmaxf(mt, __shfl_xor(mt, 32));
+      if (__any(mt > m + 8.f || (m == -INFINITY && mt > -INFINITY))) {
+        const float mn = fmaxf(m, mt);
+        const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        m = mn; l *= al;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[u][e] = fmaf(-sc.slope, fabsf((float)(me.base - k0 - 8 * (e >> 2) - (e & 3))), s[u][e]);
+        for (int nb = 0; nb < C::NB; ++nb)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[nb][e] *= al;
       }
-      if (!full) {
+      const float ms = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int u = 0; u < C::NSUB; ++u) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const int key = k0 + 8 * (e >> 2) + (e & 3);
-          s[u][e] = key >= rlo && key < rhi ? s[u][e] : -INFINITY;
+          s[u][e] = __builtin_amdgcn_exp2f(s[u][e] - ms);
+          l += s[u][e];
         }
+        seq_reduce<C>(acc, vt_lds, u, dh, s[u]);
       }
-#pragma unroll
-      for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[u][e]);
     }
-    mt = fmaxf(mt, __shfl_xor(mt, 32));
-    if (__any(mt > m + 8.f || (m == -INFINITY && mt > -INFINITY))) {
-      const float mn = fmaxf(m, mt);
-      const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-      m = mn; l *= al;
-#pragma unroll
-      for (int nb = 0; nb < C::NB; ++nb)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) acc[nb][e] *= al;
+    if (more) {
+      seq_tile_done<C>(mk, kn, dbytes);
+      if constexpr (C::DS == 1) seq_tile_done<C>(mv, vn, dbytes);
     }
-    const float ms = m == -INFINITY ? 0.f : m;
-#pragma unroll
-    for (int u = 0; u < C::NSUB; ++u) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        s[u][e] = __builtin_amdgcn_exp2f(s[u][e] - ms);
-        l += s[u][e];
-      }
-      seq_reduce<C>(acc, vt_lds, u, dh, s[u]);
+    __syncthreads();
+    if constexpr (C::DS == 1) {
+      buf ^= 1;
+      kt_lds = kn; vt_lds = vn;
+    } else {
+      if (more) seq_tile_move<C>(mv, vt_lds, vp, A.v_t, kt + C::BR, end, dbytes);
     }
   }
   const uint32_t bad = seq_bad_rows<C>(acc, 0, red);
@@ -255,7 +280,7 @@ int seq_attn_splits(int bf16, const SeqAttnArgs& A) {
 
 template <class C>
 static hipError_t fwd(hipStream_t s, const SeqAttnArgs& A) {
-  constexpr int lds = 2 * C::kTileBytes + C::kXchBytes + C::NW * 8;
+  constexpr int lds = SeqFwdLds<C>::kBytes;
   static DeviceMarks marks;
   auto fn = seq_attn_fwd_kernel<C>;
   hipError_t e = marks.raise_lds(reinterpret_cast<const void*>(fn), lds);

@@ -89,7 +89,7 @@ __device__ __forceinline__ void seq_attn_dq_again(const SeqAttnArgs& A, const Se
 #pragma unroll 1
   for (int n = 0; n < 32; ++n) {
     const int row = row0 + n;
-    if (!(rows >> n & 1) || row >= A.tq || (C::DS == 2 && (n & 1) != dh)) continue;
+    if (!(rows >> n & 1) || row >= A.tq || n % C::DS != dh) continue;
     const int lo = __shfl(me.lo, n), hi = __shfl(me.hi, n), base = __shfl(me.base, n);
     const SeqSpread q = seq_spread<T>(A.q + head * A.q_h + (int64_t)row * A.q_t, A.d);
     const SeqSpread g = seq_spread<T>(A.dout + head * A.do_h + (int64_t)row * A.do_t, A.d);
@@ -109,21 +109,25 @@ __device__ __forceinline__ void seq_attn_dq_again(const SeqAttnArgs& A, const Se
 }
 
 template <class C>
-__global__ void __launch_bounds__(C::NT) __attribute__((amdgpu_waves_per_eu(C::NT / 256, C::NT / 256)))
+struct SeqDqLds {                                        // as SeqFwdLds, with two partial blocks a wave
+  static constexpr int kBufs = C::DS == 1 ? 2 : 1;
+  static constexpr int kXch = 2 * kBufs * C::kTileBytes, kFin = kXch + (C::DS > 1 ? C::NW * 8192 : 0);
+  static constexpr int kRed = kFin + (C::DS > 1 ? C::NW / C::DS * 4096 : 0), kBytes = kRed + C::NW * 8;
+};
+template <class C>
+__global__ void __launch_bounds__(C::NT) __attribute__((amdgpu_waves_per_eu(2, 2)))
 seq_attn_dq_kernel(SeqAttnArgs A) {
   using T = typename C::E;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  char *kt_lds = smem, *vt_lds = smem + C::kTileBytes, *xch = smem + 2 * C::kTileBytes;
-  int* red = reinterpret_cast<int*>(xch + 2 * C::kXchBytes);
+  char *xch = smem + SeqDqLds<C>::kXch, *fin = smem + SeqDqLds<C>::kFin;
+  int* red = reinterpret_cast<int*>(smem + SeqDqLds<C>::kRed);
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int tiles = (A.tq + C::RB - 1) / C::RB;
   const int id = seq_xcd_order(blockIdx.x, gridDim.x);
   const int head = id / tiles, tile = tiles - 1 - id % tiles;
-  const int kvh = head / (A.hq / A.hk), dh = C::DS == 2 ? (w & 1) : 0;
+  const int kvh = head / (A.hq / A.hk), dh = w % C::DS;
   const int row0 = tile * C::RB + 32 * (w / C::DS), row = row0 + (lane & 31);
   const int dbytes = A.d * C::ES;
-  SeqMover mv;
-  mv.init<C>(dbytes);
 
   SeqRow me{0, 0, 0};
   float lse = INFINITY, delta = 0.f;
@@ -145,64 +149,131 @@ seq_attn_dq_kernel(SeqAttnArgs A) {
   int beg = lo, end = max(hi, lo);
   if (hi <= 0) beg = end = 0;
 
+  const char *kp = A.k + kvh * A.k_h, *vp = A.v + kvh * A.v_h;
+  SeqMover mk, mv;
+  mk.init<C>(A.k_t, dbytes);
+  mv.init<C>(A.v_t, dbytes);
+  char *kt_lds = smem, *vt_lds = smem + C::kTileBytes;
+  if (beg < end) {
+    seq_tile_move<C>(mk, kt_lds, kp, A.k_t, beg, end, dbytes);
+    seq_tile_move<C>(mv, vt_lds, vp, A.v_t, beg, end, dbytes);
+  }
   seq_u32x4 oq[C::NF], og[C::NF];
   seq_own_load<C>(oq, A.q + head * A.q_h, A.q_t, row0, A.tq, dh, dbytes);
   seq_own_load<C>(og, A.dout + head * A.do_h, A.do_t, row0, A.tq, dh, dbytes);
-  const char *kp = A.k + kvh * A.k_h, *vp = A.v + kvh * A.v_h;
   const SeqScore sc(A, head);
   seq_f32x16 acc[C::NB];
 #pragma unroll
   for (int nb = 0; nb < C::NB; ++nb)
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[nb][e] = 0.f;
-  seq_u32x4 kr[C::NL], vr[C::NL];
-  if (beg < end) {
-    seq_tile_load<C>(mv, kr, kp, A.k_t, beg, end, dbytes);
-    seq_tile_load<C>(mv, vr, vp, A.v_t, beg, end, dbytes);
-  }
-  for (int kt = beg; kt < end; kt += C::BR) {
-    __syncthreads();
-    seq_tile_store<C>(mv, kr, kt_lds);
-    seq_tile_store<C>(mv, vr, vt_lds);
-    __syncthreads();
-    if (kt + C::BR < end) {
-      seq_tile_load<C>(mv, kr, kp, A.k_t, kt + C::BR, end, dbytes);
-      seq_tile_load<C>(mv, vr, vp, A.v_t, kt + C::BR, end, dbytes);
+  seq_tile_done<C>(mk, kt_lds, dbytes);
+  seq_tile_done<C>(mv, vt_lds, dbytes);
+  __syncthreads();
+
+  for (int kt = beg, buf = 0; kt < end; kt += C::BR) {
+    const bool more = kt + C::BR < end;
+    char *kn = kt_lds, *vn = vt_lds;
+    if constexpr (C::DS == 1) {
+      kn = smem + (buf ^ 1) * 2 * C::kTileBytes;
+      vn = kn + C::kTileBytes;
+      if (more) {
+        seq_tile_move<C>(mk, kn, kp, A.k_t, kt + C::BR, end, dbytes);
+        seq_tile_move<C>(mv, vn, vp, A.v_t, kt + C::BR, end, dbytes);
+      }
     }
 #pragma unroll 1
     for (int u = 0; u < C::NSUB; ++u) {
       const int kb = kt + 32 * u;
       const bool active = wlo < min(kb + 32, end) && whi > kb;
-      if (C::DS == 1 && !active) continue;
       seq_f32x16 s, dp;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) { s[e] = 0.f; dp[e] = 0.f; }
       if (active) {
-        seq_scores<C>(s, kt_lds, u, dh, oq);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dp[e] = 0.f;
         seq_scores<C>(dp, vt_lds, u, dh, og);
       }
-      if constexpr (C::DS == 2) {
-        if (u > 0) __syncthreads();
-        seq_exchange2<C>(s, dp, xch);
-        if (!active) continue;
+      if constexpr (C::DS > 1) {                     // the keys' tile was still on its way while the values' was used
+        if (kt > beg) {
+          seq_tile_done<C>(mk, kt_lds, dbytes);
+          __syncthreads();
+        }
+      }
+      if (active) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = 0.f;
+        seq_scores<C>(s, kt_lds, u, dh, oq);
+      }
+      if constexpr (C::DS > 1) {
+        static_assert(C::NSUB == 1 && (C::DS == 2 || C::DS == 4), "one pair of blocks is exchanged");
+        if (active) {
+          seq_put<C>(s, xch, w, 2, 0);
+          seq_put<C>(dp, xch, w, 2, 1);
+        }
+        __syncthreads();                             // the values' tile is free
+        if (more) seq_tile_move<C>(mv, vt_lds, vp, A.v_t, kt + C::BR, end, dbytes);
       }
       const bool full = __all(me.lo <= kb && me.hi >= kb + 32);
-      seq_by_score(A, [&](auto cap, auto slope) {
+      // ds of quads g0 .. g1 of the block, in dp
+      const auto pairs = [&](int g0, int g1) {
+        seq_by_score(A, [&](auto cap, auto slope) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            if (e < 4 * g0 || e >= 4 * g1) continue;
+            float x = s[e], y = dp[e];
+            seq_pair<T, cap.value, slope.value>(sc, x, y, true, lse, delta, me.base - kb - 4 * h - 8 * (e >> 2) - (e & 3));
+            dp[e] = y;
+          }
+        });
+        if (full) return;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          float x = s[e], y = dp[e];
-          seq_pair<T, cap.value, slope.value>(sc, x, y, true, lse, delta, me.base - kb - 4 * h - 8 * (e >> 2) - (e & 3));
-          dp[e] = y;
-        }
-      });
-      if (!full) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
+          if (e < 4 * g0 || e >= 4 * g1) continue;
           const int key = kb + 4 * h + 8 * (e >> 2) + (e & 3);
           dp[e] = key >= me.lo && key < me.hi ? dp[e] : 0.f;
         }
+      };
+      if constexpr (C::DS == 1) {
+        if (!active) continue;
+        pairs(0, 4);
+      } else {
+        // each wave of the team sums and finishes its share of the block's quads, then all take the whole
+        constexpr int GP = 4 / C::DS;
+        if (active) {
+#pragma unroll
+          for (int j = 0; j < C::DS; ++j) {
+            if (j != dh) continue;                   // the registers' numbers must be constants
+#pragma unroll
+            for (int g = j * GP; g < (j + 1) * GP; ++g) {
+              const seq_f32x4 a = seq_sum_quad<C>(xch, w, 2, 0, g), b = seq_sum_quad<C>(xch, w, 2, 1, g);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) { s[4 * g + i] = a[i]; dp[4 * g + i] = b[i]; }
+            }
+            pairs(j * GP, (j + 1) * GP);
+#pragma unroll
+            for (int g = j * GP; g < (j + 1) * GP; ++g) seq_xch<C>(fin, w / C::DS, 1, 0)[g * 64] = seq_quad(dp, g);
+          }
+        }
+        __syncthreads();
+        if (!active) continue;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const seq_f32x4 b = seq_xch<C>(fin, w / C::DS, 1, 0)[g * 64];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) dp[4 * g + i] = b[i];
+        }
       }
       seq_reduce<C>(acc, kt_lds, u, dh, dp);
+    }
+    if (more) {
+      if constexpr (C::DS == 1) seq_tile_done<C>(mk, kn, dbytes);
+      seq_tile_done<C>(mv, vn, dbytes);
+    }
+    __syncthreads();
+    if constexpr (C::DS == 1) {
+      buf ^= 1;
+      kt_lds = kn; vt_lds = vn;
+    } else {
+      if (more) seq_tile_move<C>(mk, kt_lds, kp, A.k_t, kt + C::BR, end, dbytes);
     }
   }
   const uint32_t bad = seq_bad_rows<C>(acc, 0, red);
@@ -222,7 +293,7 @@ __device__ __forceinline__ void seq_attn_dkv_again(const SeqAttnArgs& A, uint32_
 #pragma unroll 1
   for (int n = 0; n < 32; ++n) {
     const int key = row0 + n;
-    if (!(rows >> n & 1) || key >= A.tk || (C::DS == 2 && (n & 1) != dh)) continue;
+    if (!(rows >> n & 1) || key >= A.tk || n % C::DS != dh) continue;
     const SeqSpread k = seq_spread<T>(A.k + kvh * A.k_h + (int64_t)key * A.k_t, A.d);
     const SeqSpread v = seq_spread<T>(A.v + kvh * A.v_h + (int64_t)key * A.v_t, A.d);
     float dk[4] = {0.f, 0.f, 0.f, 0.f}, dv[4] = {0.f, 0.f, 0.f, 0.f};
@@ -257,22 +328,31 @@ __device__ __forceinline__ void seq_attn_dkv_again(const SeqAttnArgs& A, uint32_
 }
 
 template <class C>
-__global__ void __launch_bounds__(C::NT) __attribute__((amdgpu_waves_per_eu(C::DH == 128 ? 1 : 2, C::DH == 128 ? 1 : 2)))
+struct SeqDkvLds {                                       // tiles, statistics of the tile's rows, partial and whole score blocks
+  // bfloat16 at 128 columns a wave: keys, values and both accumulators are 192 registers of the 256 that two waves a SIMD leave each,
+  // too many next to a pair of blocks (spilled, the kernel took 2.4 ms where it now takes DKV_MS): the values' fragments and PK of the
+  // keys' are read from LDS instead, as many as leave room for two workgroups a CU
+  static constexpr bool kPark = C::ES == 2 && C::DH == 128;
+  static constexpr int PK = 3, kParked = kPark ? (PK + C::NF) * 1024 : 0;          // bytes a wave
+  static constexpr int kBufs = C::DS == 1 ? 2 : 1, kStat = 5 * C::BR * 4;
+  static constexpr int kRows = 2 * kBufs * C::kTileBytes, kXch = kRows + kBufs * kStat;
+  static constexpr int kFin = kXch + (C::DS > 1 ? C::NW * 8192 : 0), kRed = kFin + (C::DS > 1 ? C::NW / C::DS * 8192 : 0);
+  static constexpr int kOwn = (kRed + C::NW * 8 + 15) / 16 * 16, kBytes = kOwn + C::NW * kParked;
+};
+template <class C>
+__global__ void __launch_bounds__(C::NT) __attribute__((amdgpu_waves_per_eu(2, 2)))
 seq_attn_dkv_kernel(SeqAttnArgs A) {
   using T = typename C::E;
+  using L = SeqDkvLds<C>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  char *qt_lds = smem, *gt_lds = smem + C::kTileBytes, *xch = smem + 2 * C::kTileBytes;
-  float* rowf = reinterpret_cast<float*>(xch + 2 * C::kXchBytes);       // [2][BR]: lse, delta
-  int* rowi = reinterpret_cast<int*>(rowf + 2 * C::BR);                 // [3][BR]: lo, hi, base
-  int* red = rowi + 3 * C::BR;
+  char *xch = smem + L::kXch, *fin = smem + L::kFin;
+  int* red = reinterpret_cast<int*>(smem + L::kRed);
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int tiles = (A.tk + C::RB - 1) / C::RB, grp = A.hq / A.hk;
   const int id = seq_xcd_order(blockIdx.x, gridDim.x);
-  const int kvh = id / tiles, tile = id % tiles, dh = C::DS == 2 ? (w & 1) : 0;
+  const int kvh = id / tiles, tile = id % tiles, dh = w % C::DS;
   const int first = tile * C::RB, row0 = first + 32 * (w / C::DS), key = row0 + (lane & 31);
   const int dbytes = A.d * C::ES;
-  SeqMover mv;
-  mv.init<C>(dbytes);
 
   // query rows that may see a key of this tile: those of the sequences that the tile touches
   int qbeg = 0, qend = 0;
@@ -286,20 +366,11 @@ seq_attn_dkv_kernel(SeqAttnArgs A) {
         const int lq = A.off_q[s0 + 1] - qbeg, lk = A.off_k[s0 + 1] - A.off_k[s0];
         qbeg += min(max(at - (lk - lq), 0), max(lq, 0));
       }
-      qbeg = __builtin_amdgcn_readfirstlane(min(max(qbeg, 0), A.tq));
-      qend = __builtin_amdgcn_readfirstlane(qend);
+      qbeg = min(max(qbeg, 0), A.tq);
     }
+    qbeg = __builtin_amdgcn_readfirstlane(qbeg);
+    qend = __builtin_amdgcn_readfirstlane(qend);
   }
-
-  seq_u32x4 ok[C::NF], ov[C::NF];
-  seq_own_load<C>(ok, A.k + kvh * A.k_h, A.k_t, row0, A.tk, dh, dbytes);
-  seq_own_load<C>(ov, A.v + kvh * A.v_h, A.v_t, row0, A.tk, dh, dbytes);
-  seq_f32x16 dk[C::NB], dv[C::NB];
-#pragma unroll
-  for (int nb = 0; nb < C::NB; ++nb)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) { dk[nb][e] = 0.f; dv[nb][e] = 0.f; }
-
   const int nt = (qend - qbeg + C::BR - 1) / C::BR;
   int i0 = 0, i1 = qbeg < qend ? grp * nt : 0;
   if (A.splits > 1) {
@@ -307,87 +378,206 @@ seq_attn_dkv_kernel(SeqAttnArgs A) {
     i0 = (int)(all * blockIdx.y / A.splits);
     i1 = (int)(all * (blockIdx.y + 1) / A.splits);
   }
-  {
-    seq_u32x4 qr[C::NL], gr[C::NL];
-    float rf[2] = {INFINITY, 0.f};
-    int4 ri = make_int4(0, 0, 0, 0);
-    const auto load = [&](int it) {
-      const int head = kvh * grp + it / nt, qt = qbeg + it % nt * C::BR;
-      seq_tile_load<C>(mv, qr, A.q + head * A.q_h, A.q_t, qt, qend, dbytes);
-      seq_tile_load<C>(mv, gr, A.dout + head * A.do_h, A.do_t, qt, qend, dbytes);
-      rf[0] = INFINITY; rf[1] = 0.f; ri = make_int4(0, 0, 0, 0);
-      if (tid < C::BR && qt + tid < qend) {
-        const int64_t at = (int64_t)head * A.tq + qt + tid;
-        rf[0] = A.lse[at]; rf[1] = A.delta[at]; ri = A.rows[qt + tid];
+
+  SeqMover mq, mg;
+  mq.init<C>(A.q_t, dbytes);
+  mg.init<C>(A.do_t, dbytes);
+  const auto head_of = [&](int it) { return kvh * grp + it / nt; };
+  const auto row_of = [&](int it) { return qbeg + it % nt * C::BR; };
+  float sf[2];
+  int4 si;
+  const auto load_stat = [&](int it) {                    // threads tid < BR: their row's statistics
+    const int r = row_of(it) + tid;
+    sf[0] = INFINITY; sf[1] = 0.f; si = make_int4(0, 0, 0, 0);
+    if (tid < C::BR && r < qend) {
+      const int64_t at = (int64_t)head_of(it) * A.tq + r;
+      sf[0] = A.lse[at]; sf[1] = A.delta[at]; si = A.rows[r];
+    }
+  };
+  const auto store_stat = [&](char* to) {                 // [lse | delta | lo | hi | base][BR]
+    if (tid < C::BR) {
+      float* f = reinterpret_cast<float*>(to);
+      int* n = reinterpret_cast<int*>(to);
+      f[tid] = sf[0]; f[C::BR + tid] = sf[1];
+      n[2 * C::BR + tid] = si.x; n[3 * C::BR + tid] = si.y; n[4 * C::BR + tid] = si.z;
+    }
+  };
+
+  char *qt_lds = smem, *gt_lds = smem + C::kTileBytes, *st = smem + L::kRows;
+  if (i0 < i1) {
+    seq_tile_move<C>(mq, qt_lds, A.q + head_of(i0) * A.q_h, A.q_t, row_of(i0), qend, dbytes);
+    seq_tile_move<C>(mg, gt_lds, A.dout + head_of(i0) * A.do_h, A.do_t, row_of(i0), qend, dbytes);
+    load_stat(i0);
+    store_stat(st);
+  }
+  seq_u32x4 ok[C::NF], ov[C::NF];
+  seq_own_load<C>(ok, A.k + kvh * A.k_h, A.k_t, row0, A.tk, dh, dbytes);
+  seq_own_load<C>(ov, A.v + kvh * A.v_h, A.v_t, row0, A.tk, dh, dbytes);
+  char* parked = smem + L::kOwn + w * L::kParked;       // read by this wave alone
+  if constexpr (L::kPark) {
+#pragma unroll
+    for (int f = 0; f < C::NF; ++f) {
+      if (f < L::PK) *reinterpret_cast<seq_u32x4*>(parked + f * 1024 + lane * 16) = ok[f];
+      *reinterpret_cast<seq_u32x4*>(parked + (L::PK + f) * 1024 + lane * 16) = ov[f];
+    }
+  }
+  seq_f32x16 dk[C::NB], dv[C::NB];
+#pragma unroll
+  for (int nb = 0; nb < C::NB; ++nb)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) { dk[nb][e] = 0.f; dv[nb][e] = 0.f; }
+  seq_tile_done<C>(mq, qt_lds, dbytes);
+  seq_tile_done<C>(mg, gt_lds, dbytes);
+  __syncthreads();
+
+  for (int it = i0, buf = 0; it < i1; ++it) {
+    const bool more = it + 1 < i1;
+    const SeqScore sc(A, head_of(it));
+    char *qn = qt_lds, *gn = gt_lds, *sn = st;
+    if constexpr (C::DS == 1) {
+      qn = smem + (buf ^ 1) * 2 * C::kTileBytes;
+      gn = qn + C::kTileBytes;
+      sn = smem + L::kRows + (buf ^ 1) * L::kStat;
+    }
+    if (more) {
+      load_stat(it + 1);
+      if constexpr (C::DS == 1) {
+        seq_tile_move<C>(mq, qn, A.q + head_of(it + 1) * A.q_h, A.q_t, row_of(it + 1), qend, dbytes);
+        seq_tile_move<C>(mg, gn, A.dout + head_of(it + 1) * A.do_h, A.do_t, row_of(it + 1), qend, dbytes);
+      }
+    }
+    const float* rowf = reinterpret_cast<const float*>(st);
+    const int* rowi = reinterpret_cast<const int*>(st) + 2 * C::BR;
+    // p and ds of quads g0 .. g1 of a score block in place
+    const auto pairs = [&](seq_f32x16& s, seq_f32x16& dp, int u, int g0, int g1, bool full) {
+      seq_by_score(A, [&](auto cap, auto slope) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if (q < g0 || q >= g1) continue;
+          const int at = 32 * u + 8 * q + 4 * h;
+          const seq_f32x4 l4 = *reinterpret_cast<const seq_f32x4*>(rowf + at), d4 = *reinterpret_cast<const seq_f32x4*>(rowf + C::BR + at);
+          int ba[4] = {0, 0, 0, 0};
+          if constexpr (slope.value) {
+            const int4 b4 = *reinterpret_cast<const int4*>(rowi + 2 * C::BR + at);
+            ba[0] = b4.x; ba[1] = b4.y; ba[2] = b4.z; ba[3] = b4.w;
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float x = s[4 * q + i], y = dp[4 * q + i];
+            seq_pair<T, cap.value, slope.value>(sc, x, y, true, l4[i], d4[i], ba[i] - key);
+            s[4 * q + i] = x; dp[4 * q + i] = y;
+          }
+          __builtin_amdgcn_sched_barrier(0);                             // or all the quads' statistics are fetched at once
+        }
+      });
+      if (full) return;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (q < g0 || q >= g1) continue;
+        const int at = 32 * u + 8 * q + 4 * h;
+        const int4 lo4 = *reinterpret_cast<const int4*>(rowi + at), hi4 = *reinterpret_cast<const int4*>(rowi + C::BR + at);
+        const int lo[4] = {lo4.x, lo4.y, lo4.z, lo4.w}, hi[4] = {hi4.x, hi4.y, hi4.z, hi4.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool seen = key >= lo[i] && key < hi[i];
+          s[4 * q + i] = seen ? s[4 * q + i] : 0.f;
+          dp[4 * q + i] = seen ? dp[4 * q + i] : 0.f;
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
     };
-    if (i0 < i1) load(i0);
-    for (int it = i0; it < i1; ++it) {
-      const SeqScore sc(A, kvh * grp + it / nt);
-      __syncthreads();
-      seq_tile_store<C>(mv, qr, qt_lds);
-      seq_tile_store<C>(mv, gr, gt_lds);
-      if (tid < C::BR) {
-        rowf[tid] = rf[0]; rowf[C::BR + tid] = rf[1];
-        rowi[tid] = ri.x; rowi[C::BR + tid] = ri.y; rowi[2 * C::BR + tid] = ri.z;
-      }
-      __syncthreads();
-      if (it + 1 < i1) load(it + 1);
 #pragma unroll 1
-      for (int u = 0; u < C::NSUB; ++u) {
-        const int rl = rowi[32 * u + (lane & 31)], rh = rowi[C::BR + 32 * u + (lane & 31)];
-        const bool active = __any(rl < row0 + 32 && rh > row0);
-        if (C::DS == 1 && !active) continue;
-        seq_f32x16 s, dp;
+    for (int u = 0; u < C::NSUB; ++u) {
+      const int rl = rowi[32 * u + (lane & 31)], rh = rowi[C::BR + 32 * u + (lane & 31)];
+      const bool active = __any(rl < row0 + 32 && rh > row0), full = __all(rl <= row0 && rh >= row0 + 32);
+      seq_f32x16 s, dp;
+      if (active) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) { s[e] = 0.f; dp[e] = 0.f; }
-        if (active) {
-          seq_scores<C>(s, qt_lds, u, dh, ok);
-          seq_scores<C>(dp, gt_lds, u, dh, ov);
+        for (int e = 0; e < 16; ++e) s[e] = 0.f;
+        if constexpr (L::kPark) seq_scores_parked<C, L::PK>(s, qt_lds, u, dh, parked, ok);
+        else seq_scores<C>(s, qt_lds, u, dh, ok);
+      }
+      if constexpr (C::DS > 1) {                     // dout's tile was still on its way while q's was used
+        if (it > i0) {
+          seq_tile_done<C>(mg, gt_lds, dbytes);
+          __syncthreads();
         }
-        if constexpr (C::DS == 2) {
-          if (u > 0) __syncthreads();
-          seq_exchange2<C>(s, dp, xch);
-          if (!active) continue;
-        }
-        const bool full = __all(rl <= row0 && rh >= row0 + 32);
-        seq_by_score(A, [&](auto cap, auto slope) {
+      }
+      if (active) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int at = 32 * u + 8 * q + 4 * h;
-            const seq_f32x4 l4 = *reinterpret_cast<const seq_f32x4*>(rowf + at), d4 = *reinterpret_cast<const seq_f32x4*>(rowf + C::BR + at);
-            int ba[4] = {0, 0, 0, 0};
-            if constexpr (slope.value) {
-              const int4 b4 = *reinterpret_cast<const int4*>(rowi + 2 * C::BR + at);
-              ba[0] = b4.x; ba[1] = b4.y; ba[2] = b4.z; ba[3] = b4.w;
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              float x = s[4 * q + i], y = dp[4 * q + i];
-              seq_pair<T, cap.value, slope.value>(sc, x, y, true, l4[i], d4[i], ba[i] - key);
-              s[4 * q + i] = x; dp[4 * q + i] = y;
-            }
-            __builtin_amdgcn_sched_barrier(0);                           // or all four groups' statistics are fetched at once
-          }
-        });
-        if (!full) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int at = 32 * u + 8 * q + 4 * h;
-            const int4 lo4 = *reinterpret_cast<const int4*>(rowi + at), hi4 = *reinterpret_cast<const int4*>(rowi + C::BR + at);
-            const int lo[4] = {lo4.x, lo4.y, lo4.z, lo4.w}, hi[4] = {hi4.x, hi4.y, hi4.z, hi4.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const bool seen = key >= lo[i] && key < hi[i];
-              s[4 * q + i] = seen ? s[4 * q + i] : 0.f;
-              dp[4 * q + i] = seen ? dp[4 * q + i] : 0.f;
-            }
-            __builtin_amdgcn_sched_barrier(0);
-          }
-        }
+        for (int e = 0; e < 16; ++e) dp[e] = 0.f;
+        if constexpr (L::kPark) seq_scores_parked<C, C::NF>(dp, gt_lds, u, dh, parked + L::PK * 1024, ov);
+        else seq_scores<C>(dp, gt_lds, u, dh, ov);
+      }
+      if constexpr (C::DS == 1) {
+        if (!active) continue;
+        pairs(s, dp, u, 0, 4, full);
         seq_reduce<C>(dv, gt_lds, u, dh, s);
         seq_reduce<C>(dk, qt_lds, u, dh, dp);
+      } else {
+        // each wave of the team sums and finishes its share of the block's quads, then all take the whole
+        static_assert(C::NSUB == 1 && (C::DS == 2 || C::DS == 4), "one pair of blocks is exchanged");
+        constexpr int GP = 4 / C::DS;
+        if (active) {
+          seq_put<C>(s, xch, w, 2, 0);
+          seq_put<C>(dp, xch, w, 2, 1);
+        }
+        __syncthreads();
+        if (active) {
+#pragma unroll
+          for (int j = 0; j < C::DS; ++j) {
+            if (j != dh) continue;                   // the registers' numbers must be constants
+#pragma unroll
+            for (int g = j * GP; g < (j + 1) * GP; ++g) {
+              const seq_f32x4 a = seq_sum_quad<C>(xch, w, 2, 0, g), b = seq_sum_quad<C>(xch, w, 2, 1, g);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) { s[4 * g + i] = a[i]; dp[4 * g + i] = b[i]; }
+            }
+            pairs(s, dp, u, j * GP, (j + 1) * GP, full);
+#pragma unroll
+            for (int g = j * GP; g < (j + 1) * GP; ++g) {
+              seq_xch<C>(fin, w / C::DS, 2, 0)[g * 64] = seq_quad(s, g);
+              seq_xch<C>(fin, w / C::DS, 2, 1)[g * 64] = seq_quad(dp, g);
+            }
+          }
+        }
+        __syncthreads();                             // also: the statistics' last reader has passed
+        if (more) store_stat(st);
+        if (active) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const seq_f32x4 b = seq_xch<C>(fin, w / C::DS, 2, 1)[g * 64];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dp[4 * g + i] = b[i];
+          }
+          seq_reduce<C>(dk, qt_lds, u, dh, dp);
+        }
+        __syncthreads();                             // q's tile is free
+        if (more) seq_tile_move<C>(mq, qt_lds, A.q + head_of(it + 1) * A.q_h, A.q_t, row_of(it + 1), qend, dbytes);
+        if (active) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const seq_f32x4 a = seq_xch<C>(fin, w / C::DS, 2, 0)[g * 64];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[4 * g + i] = a[i];
+          }
+          seq_reduce<C>(dv, gt_lds, u, dh, s);
+        }
       }
+    }
+    if (more) {
+      seq_tile_done<C>(mq, qn, dbytes);
+      if constexpr (C::DS == 1) {
+        seq_tile_done<C>(mg, gn, dbytes);
+        store_stat(sn);
+      }
+    }
+    __syncthreads();
+    if constexpr (C::DS == 1) {
+      buf ^= 1;
+      qt_lds = qn; gt_lds = gn; st = sn;
+    } else {
+      if (more) seq_tile_move<C>(mg, gt_lds, A.dout + head_of(it + 1) * A.do_h, A.do_t, row_of(it + 1), qend, dbytes);
     }
   }
   uint32_t bad = seq_bad_rows<C>(dk, 0, red);
@@ -428,7 +618,7 @@ __global__ void __launch_bounds__(256) seq_attn_dkv_join_kernel(SeqAttnArgs A, i
 // into how many shares a key tile's work is cut: none with 1024 workgroups or more (4 a CU: as the order masks, their work differs by
 // up to the whole length), else as many as bring it there, 8 at most, within 512 MB of partial sums
 int seq_attn_dkv_splits(int bf16, const SeqAttnArgs& A) {
-  const int rb = A.d > 128 ? 64 : 128;
+  const int rb = A.d > 128 && !bf16 ? 64 : 128;
   const int64_t wgs = ((int64_t)A.tk + rb - 1) / rb * A.hk, bytes = (int64_t)A.tk * A.hk * A.d * 8;
   if (wgs == 0 || wgs >= 1024) return 1;
   const int64_t work = (int64_t)(A.hq / A.hk) * ((A.tq / (A.nseq > 0 ? A.nseq : 1) + 31) / 32);       // query tiles a key tile sees, about
@@ -441,7 +631,7 @@ int seq_attn_dkv_splits(int bf16, const SeqAttnArgs& A) {
 
 template <class C>
 static hipError_t dq(hipStream_t s, const SeqAttnArgs& A) {
-  constexpr int lds = 2 * C::kTileBytes + 2 * C::kXchBytes + C::NW * 8;
+  constexpr int lds = SeqDqLds<C>::kBytes;
   static DeviceMarks marks;
   auto fn = seq_attn_dq_kernel<C>;
   hipError_t e = marks.raise_lds(reinterpret_cast<const void*>(fn), lds);
@@ -451,7 +641,7 @@ static hipError_t dq(hipStream_t s, const SeqAttnArgs& A) {
 }
 template <class C>
 static hipError_t dkv(hipStream_t s, const SeqAttnArgs& A) {
-  constexpr int lds = 2 * C::kTileBytes + 2 * C::kXchBytes + 5 * C::BR * 4 + C::NW * 8;
+  constexpr int lds = SeqDkvLds<C>::kBytes;
   static DeviceMarks marks;
   auto fn = seq_attn_dkv_kernel<C>;
   hipError_t e = marks.raise_lds(reinterpret_cast<const void*>(fn), lds);
@@ -482,14 +672,14 @@ static hipError_t pick(hipStream_t s, const SeqAttnArgs& A) {
     e = delta<T>(s, A);
     if (e != hipSuccess) return e;
     if (A.d <= 64) e = dq<SeqTile<T, 64, 1, 4, 64, VEC>>(s, A);
-    else if (A.d <= 128) e = dq<SeqTile<T, 128, 1, 4, sizeof(T) == 2 ? 64 : 32, VEC>>(s, A);
-    else e = dq<SeqTile<T, 256, 2, 4, 32, VEC>>(s, A);
+    else if (A.d <= 128) e = dq<SeqTile<T, 128, sizeof(T) == 2 ? 1 : 2, sizeof(T) == 2 ? 4 : 8, sizeof(T) == 2 ? 64 : 32, VEC>>(s, A);
+    else e = dq<SeqTile<T, 256, sizeof(T) == 2 ? 2 : 4, 8, 32, VEC>>(s, A);
     if (e != hipSuccess) return e;
   }
   if (A.tk == 0) return e;
   if (A.d <= 64) return dkv<SeqTile<T, 64, 1, 4, 64, VEC>>(s, A);
-  if (A.d <= 128) return dkv<SeqTile<T, 128, 1, 4, 32, VEC>>(s, A);
-  return dkv<SeqTile<T, 256, 2, 4, 32, VEC>>(s, A);
+  if (A.d <= 128) return dkv<SeqTile<T, 128, sizeof(T) == 2 ? 1 : 2, sizeof(T) == 2 ? 4 : 8, 32, VEC>>(s, A);
+  return dkv<SeqTile<T, 256, sizeof(T) == 2 ? 2 : 4, 8, 32, VEC>>(s, A);
 }
 
 hipError_t launch_seq_attn_backward(hipStream_t s, int bf16, const SeqAttnArgs& A) {

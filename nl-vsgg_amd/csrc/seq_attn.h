@@ -9,8 +9,9 @@
 // once the contraction index is permuted, so probabilities go from the exponential into the next matrix instruction without
 // leaving their lane; row statistics of an own row live in one lane (plus its partner 32 lanes further).
 // bfloat16: v_mfma_f32_32x32x16_bf16, transposed reads by ds_read_b64_tr_b16; fp32: v_mfma_f32_32x32x2_f32 (exact products).
-// Head dims are padded to DP = 64 / 128 / 256 with zeros.  At DP = 256 two waves share 32 own rows, each contracting (scores)
-// and accumulating (reductions) one half of d; the partial scores are exchanged through LDS (DS = 2).
+// Head dims are padded to DP = 64 / 128 / 256 with zeros.  Where 32 own rows and their accumulators would not fit half of a SIMD's
+// registers (so that two waves share it), a team of DS = 2 or 4 waves shares 32 own rows, each contracting (scores) and accumulating
+// (reductions) its part of d; the partial scores meet in LDS.
 #pragma once
 #include "seq_common.h"
 
@@ -32,8 +33,9 @@ struct SeqTile {
   static constexpr int RB = 32 * NW / DS;            // own rows of a workgroup
   static constexpr int NL = BR * NC / NT;            // chunks a thread moves per tile
   static constexpr int kTileBytes = BR * RS;
-  static constexpr int kXchBytes = DS == 2 ? NW * 4096 : 0;      // one 32x32 block of partial scores a wave
-  static_assert(BR * NC % NT == 0 && NT % NC == 0, "whole chunks, one chunk column a thread");
+  static constexpr int kStep = NT / NC;              // tile rows between a thread's chunks
+  static_assert(BR * NC % NT == 0 && NT % NC == 0, "whole chunks");
+  static_assert(kStep % 8 == 0, "two source offsets: the layout's XOR repeats every 16 rows");
 };
 
 // chunk position of (row, chunk): an XOR that spreads both access patterns over the banks -- eight consecutive rows at one
@@ -60,42 +62,60 @@ __device__ __forceinline__ seq_u32x4 seq_chunk_mask(int c, int dbytes) {
   return m;
 }
 
-// what a thread keeps for moving tiles: its chunk column (the same in each of its rows), the offset of its first row's chunk and the
-// chunk's mask
+// Moving tiles.  VEC: straight from memory into LDS (16 bytes a lane, no registers), lane i of a wave to 16 i behind the wave's
+// base; the XOR of the layout is applied to the SOURCE chunk.  A tile's mover is done with seq_tile_done: its own loads have
+// landed and the tail of a row that is no multiple of 16 bytes is cleared (a load reads on behind the row there); a barrier then
+// shows the tile to the others.  The copy into a tile may only start behind a barrier that every reader of its old content passed.
 struct SeqMover {
-  uint32_t row, c;
-  seq_u32x4 mask;
+  uint32_t off[2];                                  // source offset of an even / odd chunk's row and chunk, or kSeqOob
+  uint32_t tail;                                    // bit i: this thread moves the last, partial chunk in its i-th row
+  int wave;
   template <class C>
-  __device__ __forceinline__ void init(int dbytes) {
-    row = threadIdx.x / C::NC; c = threadIdx.x % C::NC;
-    mask = seq_chunk_mask(c, dbytes);
+  __device__ __forceinline__ void init(int64_t stride, int dbytes) {
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    tail = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = threadIdx.x / C::NC + i * C::kStep, c = (threadIdx.x % C::NC) ^ seq_swz<C>(row);
+      off[i] = 16 * c < dbytes ? (threadIdx.x / C::NC) * (uint32_t)stride + 16 * c : kSeqOob;
+      if ((dbytes & 15) && c == dbytes >> 4) tail |= 1u << i;
+    }
   }
 };
-// tile rows row0 .. row0 + BR - 1, global -> registers; rows from `hi` on are zeros (row0, hi: the same in every lane)
 template <class C>
-__device__ __forceinline__ void seq_tile_load(const SeqMover& mv, seq_u32x4 (&r)[C::NL], const char* base, int64_t stride, int row0, int hi,
-                                              int dbytes) {
+__device__ __forceinline__ void seq_tile_move(const SeqMover& mv, char* tile, const char* base, int64_t stride, int row0, int hi, int dbytes) {
+#ifdef __HIP_DEVICE_COMPILE__                              // the host pass refuses 16-byte copies into LDS
   const int rows = min(hi - row0, C::BR);
   if constexpr (C::VEC) {
     const auto rs = seq_rsrc(base + (int64_t)row0 * stride, stride, rows, dbytes);
-    const uint32_t at = 16 * mv.c, off = at < (uint32_t)dbytes ? mv.row * (uint32_t)stride + at : kSeqOob;
 #pragma unroll
     for (int i = 0; i < C::NL; ++i)
-      r[i] = __builtin_bit_cast(seq_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, off, i * (C::NT / C::NC) * (uint32_t)stride, 0));
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(tile + (i * C::NT + mv.wave * 64) * 16), 16,
+                                               mv.off[i & 1], i * C::kStep * (uint32_t)stride, 0, 0);
   } else {
 #pragma unroll
     for (int i = 0; i < C::NL; ++i) {
-      const int row = (int)mv.row + i * (C::NT / C::NC);
-      r[i] = seq_load16(base + (int64_t)(row0 + row) * stride + 16 * mv.c, row < rows ? dbytes - 16 * (int)mv.c : 0, 2);
+      const int row = threadIdx.x / C::NC + i * C::kStep, c = threadIdx.x % C::NC;
+      const seq_u32x4 r = seq_load16(base + (int64_t)(row0 + row) * stride + 16 * c, row < rows ? dbytes - 16 * c : 0, 2);
+      *reinterpret_cast<seq_u32x4*>(tile + row * C::RS + ((c ^ seq_swz<C>(row)) << 4)) = r;
     }
   }
+#endif
 }
 template <class C>
-__device__ __forceinline__ void seq_tile_store(const SeqMover& mv, const seq_u32x4 (&r)[C::NL], char* tile) {
+__device__ __forceinline__ void seq_tile_done(const SeqMover& mv, char* tile, int dbytes) {
+  if constexpr (C::VEC) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (dbytes & 15) {
 #pragma unroll
-  for (int i = 0; i < C::NL; ++i) {
-    const int row = (int)mv.row + i * (C::NT / C::NC);
-    *reinterpret_cast<seq_u32x4*>(tile + row * C::RS + ((mv.c ^ seq_swz<C>(row)) << 4)) = r[i] & mv.mask;
+      for (int i = 0; i < C::NL; ++i)
+        if (mv.tail >> (i & 1) & 1) {
+          uint32_t* p = reinterpret_cast<uint32_t*>(tile + (i * C::NT + threadIdx.x) * 16);
+          if ((dbytes & 15) <= 4) p[1] = 0;
+          if ((dbytes & 15) <= 8) p[2] = 0;
+          p[3] = 0;
+        }
+    }
   }
 }
 
@@ -153,6 +173,20 @@ __device__ __forceinline__ void seq_scores(seq_f32x16& acc, const char* tile, in
   }
 }
 
+// the same with the first P of the own rows' fragments parked in LDS (`parked`: this wave's, fragment by fragment, 16 bytes a lane)
+template <class C, int P>
+__device__ __forceinline__ void seq_scores_parked(seq_f32x16& acc, const char* tile, int sub, int dh, const char* parked, const seq_u32x4 (&own)[C::NF]) {
+  const int lane = threadIdx.x & 63, row = 32 * sub + (lane & 31), h = lane >> 5;
+  const char* p = tile + row * C::RS;
+  const int x = (h ^ seq_swz<C>(row)) << 4;
+#pragma unroll
+  for (int f = 0; f < C::NF; ++f) {
+    const seq_u32x4 a = *reinterpret_cast<const seq_u32x4*>(p + ((dh * C::DH * C::ES + 32 * f) ^ x));
+    const seq_u32x4 b = f < P ? *reinterpret_cast<const seq_u32x4*>(parked + f * 1024 + lane * 16) : own[f];
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(seq_bf16x8, a), __builtin_bit_cast(seq_bf16x8, b), acc, 0, 0, 0);
+  }
+}
+
 // acc[d][own row] += tile^T . w, w = a score block's registers.  bfloat16: w is rounded to 8 bits of mantissa here, the one
 // rounding of probabilities (or of their derivatives) on the way into the matrix instruction; sums stay in fp32
 template <class C>
@@ -195,7 +229,7 @@ __device__ __forceinline__ void seq_reduce(seq_f32x16 (&acc)[C::NB], const char*
 
 // Own rows (bits of the answer) whose sums are not finite.  A matrix instruction multiplies what a mask hides by an exact 0,
 // which is right unless that row holds an infinity or NaN (0 * inf): such own rows are done again, pair by pair over the
-// visible rows alone, so that what a mask hides cannot spread.  With DS == 2 the two waves of a pair share the answer.
+// visible rows alone, so that what a mask hides cannot spread.  The waves of a team share the answer.
 // Every wave of the workgroup calls this (barriers inside).
 template <class C>
 __device__ __forceinline__ uint32_t seq_bad_rows(const seq_f32x16 (&acc)[C::NB], uint32_t more, int* red) {
@@ -206,14 +240,15 @@ __device__ __forceinline__ uint32_t seq_bad_rows(const seq_f32x16 (&acc)[C::NB],
     for (int e = 0; e < 16; ++e) bad |= !(fabsf(acc[nb][e]) < INFINITY);
   const uint64_t b = __ballot(bad);
   uint32_t rows = (uint32_t)b | (uint32_t)(b >> 32) | more;
-  if constexpr (C::DS == 2) {
-    const int w = threadIdx.x >> 6;
+  if constexpr (C::DS > 1) {
+    const int w = threadIdx.x >> 6, first = w - w % C::DS;
     __syncthreads();
     if ((threadIdx.x & 63) == 0) red[w] = (int)rows;
     __syncthreads();
-    rows |= (uint32_t)red[w ^ 1];
+#pragma unroll
+    for (int m = 0; m < C::DS; ++m) rows |= (uint32_t)red[first + m];
   }
-  return rows;
+  return __builtin_amdgcn_readfirstlane(rows);
 }
 
 // one row spread over a wave: lane holds columns lane, lane + 64, ...
@@ -251,42 +286,40 @@ __device__ __forceinline__ void seq_spread_store(char* out, char* out_lo, const 
   }
 }
 
-// DS == 2: add the partner wave's partial block.  Every wave of the workgroup calls this (barrier inside)
+// ---- partial score blocks of the DS waves (a team) that share own rows.  Every wave of the workgroup passes the barrier between
+// put and get / share.
 template <class C>
-__device__ __forceinline__ void seq_exchange(seq_f32x16& s, char* xch) {
-  if constexpr (C::DS == 2) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    seq_f32x4* mine = reinterpret_cast<seq_f32x4*>(xch + w * 4096);
-    const seq_f32x4* other = reinterpret_cast<const seq_f32x4*>(xch + (w ^ 1) * 4096);
+__device__ __forceinline__ seq_f32x4* seq_xch(char* xch, int wave, int blocks, int block) {
+  return reinterpret_cast<seq_f32x4*>(xch) + (wave * blocks + block) * 256 + (threadIdx.x & 63);
+}
+__device__ __forceinline__ seq_f32x4 seq_quad(const seq_f32x16& s, int g) {
+  return seq_f32x4{s[4 * g], s[4 * g + 1], s[4 * g + 2], s[4 * g + 3]};
+}
+template <class C>
+__device__ __forceinline__ void seq_put(const seq_f32x16& s, char* xch, int wave, int blocks, int block) {
+  seq_f32x4* to = seq_xch<C>(xch, wave, blocks, block);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) mine[i * 64 + lane] = seq_f32x4{s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]};
-    __syncthreads();
+  for (int g = 0; g < 4; ++g) to[g * 64] = seq_quad(s, g);
+}
+// DS == 2: add the partner's block.  Both waves add the same two numbers, so both hold the same sum
+template <class C>
+__device__ __forceinline__ void seq_get(seq_f32x16& s, char* xch, int wave, int blocks, int block) {
+  const seq_f32x4* from = seq_xch<C>(xch, wave ^ 1, blocks, block);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const seq_f32x4 o = other[i * 64 + lane];
+  for (int g = 0; g < 4; ++g) {
+    const seq_f32x4 o = from[g * 64];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) s[4 * i + u] += o[u];
-    }
+    for (int u = 0; u < 4; ++u) s[4 * g + u] += o[u];
   }
 }
-
+// the whole sum of quad g (registers 4g .. 4g + 3), members in order
 template <class C>
-__device__ __forceinline__ void seq_exchange2(seq_f32x16& a, seq_f32x16& b, char* xch) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  seq_f32x4* mine = reinterpret_cast<seq_f32x4*>(xch + w * 8192);
-  const seq_f32x4* other = reinterpret_cast<const seq_f32x4*>(xch + (w ^ 1) * 8192);
+__device__ __forceinline__ seq_f32x4 seq_sum_quad(char* xch, int wave, int blocks, int block, int g) {
+  const int first = wave - wave % C::DS;
+  seq_f32x4 r = seq_xch<C>(xch, first, blocks, block)[g * 64];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    mine[i * 64 + lane] = seq_f32x4{a[4 * i], a[4 * i + 1], a[4 * i + 2], a[4 * i + 3]};
-    mine[256 + i * 64 + lane] = seq_f32x4{b[4 * i], b[4 * i + 1], b[4 * i + 2], b[4 * i + 3]};
-  }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const seq_f32x4 x = other[i * 64 + lane], y = other[256 + i * 64 + lane];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) { a[4 * i + u] += x[u]; b[4 * i + u] += y[u]; }
-  }
+  for (int m = 1; m < C::DS; ++m) r += seq_xch<C>(xch, first + m, blocks, block)[g * 64];
+  return r;
 }
 
 // Z[d][own row] registers -> a contiguous output row
