@@ -281,6 +281,7 @@ int seq_attn_splits(int bf16, const SeqAttnArgs& A) {
 template <class C>
 static hipError_t fwd(hipStream_t s, const SeqAttnArgs& A) {
   constexpr int lds = SeqFwdLds<C>::kBytes;
+  static_assert(lds <= 160 * 1024, "LDS of a CU");
   static DeviceMarks marks;
   auto fn = seq_attn_fwd_kernel<C>;
   hipError_t e = marks.raise_lds(reinterpret_cast<const void*>(fn), lds);

@@ -618,7 +618,7 @@ __global__ void __launch_bounds__(256) seq_attn_dkv_join_kernel(SeqAttnArgs A, i
 // into how many shares a key tile's work is cut: none with 1024 workgroups or more (4 a CU: as the order masks, their work differs by
 // up to the whole length), else as many as bring it there, 8 at most, within 512 MB of partial sums
 int seq_attn_dkv_splits(int bf16, const SeqAttnArgs& A) {
-  const int rb = A.d > 128 && !bf16 ? 64 : 128;
+  const int rb = A.d > 128 ? 64 : 128;
   const int64_t wgs = ((int64_t)A.tk + rb - 1) / rb * A.hk, bytes = (int64_t)A.tk * A.hk * A.d * 8;
   if (wgs == 0 || wgs >= 1024) return 1;
   const int64_t work = (int64_t)(A.hq / A.hk) * ((A.tq / (A.nseq > 0 ? A.nseq : 1) + 31) / 32);       // query tiles a key tile sees, about
@@ -632,6 +632,7 @@ int seq_attn_dkv_splits(int bf16, const SeqAttnArgs& A) {
 template <class C>
 static hipError_t dq(hipStream_t s, const SeqAttnArgs& A) {
   constexpr int lds = SeqDqLds<C>::kBytes;
+  static_assert(lds <= 160 * 1024, "LDS of a CU");
   static DeviceMarks marks;
   auto fn = seq_attn_dq_kernel<C>;
   hipError_t e = marks.raise_lds(reinterpret_cast<const void*>(fn), lds);
@@ -642,6 +643,7 @@ static hipError_t dq(hipStream_t s, const SeqAttnArgs& A) {
 template <class C>
 static hipError_t dkv(hipStream_t s, const SeqAttnArgs& A) {
   constexpr int lds = SeqDkvLds<C>::kBytes;
+  static_assert(lds <= 160 * 1024, "LDS of a CU");
   static DeviceMarks marks;
   auto fn = seq_attn_dkv_kernel<C>;
   hipError_t e = marks.raise_lds(reinterpret_cast<const void*>(fn), lds);
@@ -679,7 +681,7 @@ static hipError_t pick(hipStream_t s, const SeqAttnArgs& A) {
   if (A.tk == 0) return e;
   if (A.d <= 64) return dkv<SeqTile<T, 64, 1, 4, 64, VEC>>(s, A);
   if (A.d <= 128) return dkv<SeqTile<T, 128, sizeof(T) == 2 ? 1 : 2, sizeof(T) == 2 ? 4 : 8, 32, VEC>>(s, A);
-  return dkv<SeqTile<T, 256, sizeof(T) == 2 ? 2 : 4, 8, 32, VEC>>(s, A);
+  return dkv<SeqTile<T, 256, 4, 8, 32, VEC>>(s, A);
 }
 
 hipError_t launch_seq_attn_backward(hipStream_t s, int bf16, const SeqAttnArgs& A) {
