@@ -51,7 +51,10 @@ __device__ __forceinline__ void seq_attn_fwd_again(const SeqAttnArgs& A, const S
 template <class C>
 struct SeqFwdLds {                                       // DS == 1: two tiles of keys and of values; else one of each and the exchange
   static constexpr int kBufs = C::DS == 1 ? 2 : 1;
-  static constexpr int kXch = 2 * kBufs * C::kTileBytes, kRed = kXch + (C::DS > 1 ? C::NW * 4096 : 0), kBytes = kRed + C::NW * 8;
+  // the workgroup's small notes before and after the loop lie where the exchange is during it: at DP = 256 in fp32 a workgroup then
+  // takes exactly half of a CU's 160 KB
+  static constexpr int kXch = 2 * kBufs * C::kTileBytes, kRed = kXch;
+  static constexpr int kBytes = kXch + (C::DS > 1 ? C::NW * 4096 : C::NW * 8);
 };
 template <class C>
 __global__ void __launch_bounds__(C::NT) __attribute__((amdgpu_waves_per_eu(2, 2)))
@@ -130,13 +133,16 @@ seq_attn_fwd_kernel(SeqAttnArgs A) {
         seq_scores<C>(s[u], kt_lds, u, dh, own);
       }
     }
-    if constexpr (C::DS == 2) {
+    if constexpr (C::DS > 1) {
       static_assert(C::NSUB == 1, "one block is exchanged");
-      if (active) seq_put<C>(s[0], xch, w, 1, 0);
+      if (active) SeqShare<C, 1>::put(s[0], xch, w, 0);
       seq_tile_done<C>(mv, vt_lds, dbytes);
       __syncthreads();                                               // keys are free, values and partial scores are there
       if (more) seq_tile_move<C>(mk, kn, kp, A.k_t, kt + C::BR, end, dbytes);
-      if (active) seq_get<C>(s[0], xch, w, 1, 0);
+      if (active) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) seq_set_quad(s[0], g, SeqShare<C, 1>::sum(xch, w - dh, 0, g));
+      }
     }
     if (active) {
       const bool full = __all(rlo <= kt && rhi >= kt + C::BR);
@@ -296,7 +302,7 @@ template <class T, bool VEC>
 static hipError_t pick(hipStream_t s, const SeqAttnArgs& A) {
   if (A.d <= 64) return fwd<SeqTile<T, 64, 1, 4, 64, VEC>>(s, A);
   if (A.d <= 128) return fwd<SeqTile<T, 128, 1, 4, sizeof(T) == 2 ? 64 : 32, VEC>>(s, A);
-  return fwd<SeqTile<T, 256, 2, 8, 32, VEC>>(s, A);
+  return fwd<SeqTile<T, 256, sizeof(T) == 2 ? 2 : 4, 4, 32, VEC>>(s, A);
 }
 
 hipError_t launch_seq_attn_forward(hipStream_t s, int bf16, const SeqAttnArgs& A) {

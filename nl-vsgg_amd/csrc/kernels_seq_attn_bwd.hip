@@ -111,15 +111,18 @@ __device__ __forceinline__ void seq_attn_dq_again(const SeqAttnArgs& A, const Se
 template <class C>
 struct SeqDqLds {                                        // as SeqFwdLds, with two partial blocks a wave
   static constexpr int kBufs = C::DS == 1 ? 2 : 1;
-  static constexpr int kXch = 2 * kBufs * C::kTileBytes, kFin = kXch + (C::DS > 1 ? C::NW * 8192 : 0);
-  static constexpr int kRed = kFin + (C::DS > 1 ? C::NW / C::DS * 4096 : 0), kBytes = kRed + C::NW * 8;
+  // the partial blocks go where the values' tile was (it is used up before them), where it is large enough
+  static constexpr int kNeed = C::DS > 1 ? C::NW * SeqShare<C, 2>::kWave : 0;
+  static constexpr bool kOver = C::DS > 1 && kNeed <= C::kTileBytes;
+  static constexpr int kXch = kOver ? C::kTileBytes : 2 * kBufs * C::kTileBytes;
+  static constexpr int kRed = 2 * kBufs * C::kTileBytes + (kOver ? 0 : kNeed), kBytes = kRed + C::NW * 8;
 };
 template <class C>
 __global__ void __launch_bounds__(C::NT) __attribute__((amdgpu_waves_per_eu(2, 2)))
 seq_attn_dq_kernel(SeqAttnArgs A) {
   using T = typename C::E;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  char *xch = smem + SeqDqLds<C>::kXch, *fin = smem + SeqDqLds<C>::kFin;
+  char* xch = smem + SeqDqLds<C>::kXch;
   int* red = reinterpret_cast<int*>(smem + SeqDqLds<C>::kRed);
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int tiles = (A.tq + C::RB - 1) / C::RB;
@@ -193,10 +196,8 @@ seq_attn_dq_kernel(SeqAttnArgs A) {
         seq_scores<C>(dp, vt_lds, u, dh, og);
       }
       if constexpr (C::DS > 1) {                     // the keys' tile was still on its way while the values' was used
-        if (kt > beg) {
-          seq_tile_done<C>(mk, kt_lds, dbytes);
-          __syncthreads();
-        }
+        if (kt > beg) seq_tile_done<C>(mk, kt_lds, dbytes);
+        __syncthreads();
       }
       if (active) {
 #pragma unroll
@@ -204,63 +205,59 @@ seq_attn_dq_kernel(SeqAttnArgs A) {
         seq_scores<C>(s, kt_lds, u, dh, oq);
       }
       if constexpr (C::DS > 1) {
-        static_assert(C::NSUB == 1 && (C::DS == 2 || C::DS == 4), "one pair of blocks is exchanged");
+        static_assert(C::NSUB == 1, "one pair of blocks is exchanged");
         if (active) {
-          seq_put<C>(s, xch, w, 2, 0);
-          seq_put<C>(dp, xch, w, 2, 1);
+          SeqShare<C, 2>::put(s, xch, w, 0);
+          SeqShare<C, 2>::put(dp, xch, w, 1);
         }
         __syncthreads();                             // the values' tile is free
-        if (more) seq_tile_move<C>(mv, vt_lds, vp, A.v_t, kt + C::BR, end, dbytes);
+        if (!SeqDqLds<C>::kOver && more) seq_tile_move<C>(mv, vt_lds, vp, A.v_t, kt + C::BR, end, dbytes);
       }
       const bool full = __all(me.lo <= kb && me.hi >= kb + 32);
-      // ds of quads g0 .. g1 of the block, in dp
-      const auto pairs = [&](int g0, int g1) {
-        seq_by_score(A, [&](auto cap, auto slope) {
+      if constexpr (C::DS == 1) {
+        if (!active) continue;
+        seq_by_score(A, [&](auto cap, auto slope) __attribute__((always_inline)) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            if (e < 4 * g0 || e >= 4 * g1) continue;
             float x = s[e], y = dp[e];
             seq_pair<T, cap.value, slope.value>(sc, x, y, true, lse, delta, me.base - kb - 4 * h - 8 * (e >> 2) - (e & 3));
             dp[e] = y;
           }
         });
-        if (full) return;
+        if (!full) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          if (e < 4 * g0 || e >= 4 * g1) continue;
-          const int key = kb + 4 * h + 8 * (e >> 2) + (e & 3);
-          dp[e] = key >= me.lo && key < me.hi ? dp[e] : 0.f;
-        }
-      };
-      if constexpr (C::DS == 1) {
-        if (!active) continue;
-        pairs(0, 4);
-      } else {
-        // each wave of the team sums and finishes its share of the block's quads, then all take the whole
-        constexpr int GP = 4 / C::DS;
-        if (active) {
-#pragma unroll
-          for (int j = 0; j < C::DS; ++j) {
-            if (j != dh) continue;                   // the registers' numbers must be constants
-#pragma unroll
-            for (int g = j * GP; g < (j + 1) * GP; ++g) {
-              const seq_f32x4 a = seq_sum_quad<C>(xch, w, 2, 0, g), b = seq_sum_quad<C>(xch, w, 2, 1, g);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) { s[4 * g + i] = a[i]; dp[4 * g + i] = b[i]; }
-            }
-            pairs(j * GP, (j + 1) * GP);
-#pragma unroll
-            for (int g = j * GP; g < (j + 1) * GP; ++g) seq_xch<C>(fin, w / C::DS, 1, 0)[g * 64] = seq_quad(dp, g);
+          for (int e = 0; e < 16; ++e) {
+            const int key = kb + 4 * h + 8 * (e >> 2) + (e & 3);
+            dp[e] = key >= me.lo && key < me.hi ? dp[e] : 0.f;
           }
         }
+      } else {
+        // each wave of the team sums and finishes its share of the block's quads, then all take the whole
+        using S = SeqShare<C, 2>;
+        if (active)
+          seq_by_score(A, [&](auto cap, auto slope) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < S::GP; ++i) {
+              const int g = dh * S::GP + i;
+              const seq_f32x4 a = S::sum(xch, w - dh, 0, g);
+              seq_f32x4 b = S::sum(xch, w - dh, 1, g);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int key = kb + 8 * g + 4 * h + e;
+                float x = a[e], y = b[e];
+                seq_pair<T, cap.value, slope.value>(sc, x, y, full || (key >= me.lo && key < me.hi), lse, delta, me.base - key);
+                b[e] = y;
+              }
+              *S::slot(xch, w, 1, g) = b;
+            }
+          });
         __syncthreads();
-        if (!active) continue;
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const seq_f32x4 b = seq_xch<C>(fin, w / C::DS, 1, 0)[g * 64];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) dp[4 * g + i] = b[i];
+        if (active) S::take(dp, xch, w - dh, 1);
+        if constexpr (SeqDqLds<C>::kOver) {
+          __syncthreads();                           // the blocks are read: the next values may come
+          if (more) seq_tile_move<C>(mv, vt_lds, vp, A.v_t, kt + C::BR, end, dbytes);
         }
+        if (!active) continue;
       }
       seq_reduce<C>(acc, kt_lds, u, dh, dp);
     }
@@ -336,7 +333,7 @@ struct SeqDkvLds {                                       // tiles, statistics of
   static constexpr int PK = 3, kParked = kPark ? (PK + C::NF) * 1024 : 0;          // bytes a wave
   static constexpr int kBufs = C::DS == 1 ? 2 : 1, kStat = 5 * C::BR * 4;
   static constexpr int kRows = 2 * kBufs * C::kTileBytes, kXch = kRows + kBufs * kStat;
-  static constexpr int kFin = kXch + (C::DS > 1 ? C::NW * 8192 : 0), kRed = kFin + (C::DS > 1 ? C::NW / C::DS * 8192 : 0);
+  static constexpr int kRed = kXch + (C::DS > 1 ? C::NW * SeqShare<C, 2>::kWave : 0);
   static constexpr int kOwn = (kRed + C::NW * 8 + 15) / 16 * 16, kBytes = kOwn + C::NW * kParked;
 };
 template <class C>
@@ -345,7 +342,7 @@ seq_attn_dkv_kernel(SeqAttnArgs A) {
   using T = typename C::E;
   using L = SeqDkvLds<C>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  char *xch = smem + L::kXch, *fin = smem + L::kFin;
+  char* xch = smem + L::kXch;
   int* red = reinterpret_cast<int*>(smem + L::kRed);
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int tiles = (A.tk + C::RB - 1) / C::RB, grp = A.hq / A.hk;
@@ -448,42 +445,31 @@ seq_attn_dkv_kernel(SeqAttnArgs A) {
     }
     const float* rowf = reinterpret_cast<const float*>(st);
     const int* rowi = reinterpret_cast<const int*>(st) + 2 * C::BR;
-    // p and ds of quads g0 .. g1 of a score block in place
-    const auto pairs = [&](seq_f32x16& s, seq_f32x16& dp, int u, int g0, int g1, bool full) {
-      seq_by_score(A, [&](auto cap, auto slope) {
+    // p and ds of quad g of block u in place of its products
+    const auto quad = [&](auto cap, auto slope, int u, int g, seq_f32x4& s4, seq_f32x4& p4) __attribute__((always_inline)) {
+      const int at = 32 * u + 8 * g + 4 * h;
+      const seq_f32x4 l4 = *reinterpret_cast<const seq_f32x4*>(rowf + at), d4 = *reinterpret_cast<const seq_f32x4*>(rowf + C::BR + at);
+      int ba[4] = {0, 0, 0, 0};
+      if constexpr (slope.value) {
+        const int4 b4 = *reinterpret_cast<const int4*>(rowi + 2 * C::BR + at);
+        ba[0] = b4.x; ba[1] = b4.y; ba[2] = b4.z; ba[3] = b4.w;
+      }
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          if (q < g0 || q >= g1) continue;
-          const int at = 32 * u + 8 * q + 4 * h;
-          const seq_f32x4 l4 = *reinterpret_cast<const seq_f32x4*>(rowf + at), d4 = *reinterpret_cast<const seq_f32x4*>(rowf + C::BR + at);
-          int ba[4] = {0, 0, 0, 0};
-          if constexpr (slope.value) {
-            const int4 b4 = *reinterpret_cast<const int4*>(rowi + 2 * C::BR + at);
-            ba[0] = b4.x; ba[1] = b4.y; ba[2] = b4.z; ba[3] = b4.w;
-          }
+      for (int i = 0; i < 4; ++i) {
+        float x = s4[i], y = p4[i];
+        seq_pair<T, cap.value, slope.value>(sc, x, y, true, l4[i], d4[i], ba[i] - key);
+        s4[i] = x; p4[i] = y;
+      }
+    };
+    const auto hide = [&](int u, int g, seq_f32x4& s4, seq_f32x4& p4) __attribute__((always_inline)) {
+      const int at = 32 * u + 8 * g + 4 * h;
+      const int4 lo4 = *reinterpret_cast<const int4*>(rowi + at), hi4 = *reinterpret_cast<const int4*>(rowi + C::BR + at);
+      const int lo[4] = {lo4.x, lo4.y, lo4.z, lo4.w}, hi[4] = {hi4.x, hi4.y, hi4.z, hi4.w};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float x = s[4 * q + i], y = dp[4 * q + i];
-            seq_pair<T, cap.value, slope.value>(sc, x, y, true, l4[i], d4[i], ba[i] - key);
-            s[4 * q + i] = x; dp[4 * q + i] = y;
-          }
-          __builtin_amdgcn_sched_barrier(0);                             // or all the quads' statistics are fetched at once
-        }
-      });
-      if (full) return;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        if (q < g0 || q >= g1) continue;
-        const int at = 32 * u + 8 * q + 4 * h;
-        const int4 lo4 = *reinterpret_cast<const int4*>(rowi + at), hi4 = *reinterpret_cast<const int4*>(rowi + C::BR + at);
-        const int lo[4] = {lo4.x, lo4.y, lo4.z, lo4.w}, hi[4] = {hi4.x, hi4.y, hi4.z, hi4.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const bool seen = key >= lo[i] && key < hi[i];
-          s[4 * q + i] = seen ? s[4 * q + i] : 0.f;
-          dp[4 * q + i] = seen ? dp[4 * q + i] : 0.f;
-        }
-        __builtin_amdgcn_sched_barrier(0);
+      for (int i = 0; i < 4; ++i) {
+        const bool seen = key >= lo[i] && key < hi[i];
+        s4[i] = seen ? s4[i] : 0.f;
+        p4[i] = seen ? p4[i] : 0.f;
       }
     };
 #pragma unroll 1
@@ -511,56 +497,59 @@ seq_attn_dkv_kernel(SeqAttnArgs A) {
       }
       if constexpr (C::DS == 1) {
         if (!active) continue;
-        pairs(s, dp, u, 0, 4, full);
+        seq_by_score(A, [&](auto cap, auto slope) __attribute__((always_inline)) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            seq_f32x4 a = seq_quad(s, g), b = seq_quad(dp, g);
+            quad(cap, slope, u, g, a, b);
+            seq_set_quad(s, g, a);
+            seq_set_quad(dp, g, b);
+            __builtin_amdgcn_sched_barrier(0);       // or all the quads' statistics are fetched at once
+          }
+        });
+        if (!full) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            seq_f32x4 a = seq_quad(s, g), b = seq_quad(dp, g);
+            hide(u, g, a, b);
+            seq_set_quad(s, g, a);
+            seq_set_quad(dp, g, b);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
         seq_reduce<C>(dv, gt_lds, u, dh, s);
         seq_reduce<C>(dk, qt_lds, u, dh, dp);
       } else {
         // each wave of the team sums and finishes its share of the block's quads, then all take the whole
-        static_assert(C::NSUB == 1 && (C::DS == 2 || C::DS == 4), "one pair of blocks is exchanged");
-        constexpr int GP = 4 / C::DS;
+        static_assert(C::NSUB == 1, "one pair of blocks is exchanged");
+        using S = SeqShare<C, 2>;
         if (active) {
-          seq_put<C>(s, xch, w, 2, 0);
-          seq_put<C>(dp, xch, w, 2, 1);
+          S::put(s, xch, w, 0);
+          S::put(dp, xch, w, 1);
         }
         __syncthreads();
-        if (active) {
+        if (active)
+          seq_by_score(A, [&](auto cap, auto slope) __attribute__((always_inline)) {
 #pragma unroll
-          for (int j = 0; j < C::DS; ++j) {
-            if (j != dh) continue;                   // the registers' numbers must be constants
-#pragma unroll
-            for (int g = j * GP; g < (j + 1) * GP; ++g) {
-              const seq_f32x4 a = seq_sum_quad<C>(xch, w, 2, 0, g), b = seq_sum_quad<C>(xch, w, 2, 1, g);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) { s[4 * g + i] = a[i]; dp[4 * g + i] = b[i]; }
+            for (int i = 0; i < S::GP; ++i) {
+              const int g = dh * S::GP + i;
+              seq_f32x4 a = S::sum(xch, w - dh, 0, g), b = S::sum(xch, w - dh, 1, g);
+              quad(cap, slope, u, g, a, b);
+              if (!full) hide(u, g, a, b);
+              *S::slot(xch, w, 0, g) = a;
+              *S::slot(xch, w, 1, g) = b;
             }
-            pairs(s, dp, u, j * GP, (j + 1) * GP, full);
-#pragma unroll
-            for (int g = j * GP; g < (j + 1) * GP; ++g) {
-              seq_xch<C>(fin, w / C::DS, 2, 0)[g * 64] = seq_quad(s, g);
-              seq_xch<C>(fin, w / C::DS, 2, 1)[g * 64] = seq_quad(dp, g);
-            }
-          }
-        }
+          });
         __syncthreads();                             // also: the statistics' last reader has passed
         if (more) store_stat(st);
         if (active) {
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const seq_f32x4 b = seq_xch<C>(fin, w / C::DS, 2, 1)[g * 64];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) dp[4 * g + i] = b[i];
-          }
+          S::take(dp, xch, w - dh, 1);
           seq_reduce<C>(dk, qt_lds, u, dh, dp);
         }
         __syncthreads();                             // q's tile is free
         if (more) seq_tile_move<C>(mq, qt_lds, A.q + head_of(it + 1) * A.q_h, A.q_t, row_of(it + 1), qend, dbytes);
         if (active) {
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const seq_f32x4 a = seq_xch<C>(fin, w / C::DS, 2, 0)[g * 64];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[4 * g + i] = a[i];
-          }
+          S::take(s, xch, w - dh, 0);
           seq_reduce<C>(dv, gt_lds, u, dh, s);
         }
       }
@@ -618,7 +607,8 @@ __global__ void __launch_bounds__(256) seq_attn_dkv_join_kernel(SeqAttnArgs A, i
 // into how many shares a key tile's work is cut: none with 1024 workgroups or more (4 a CU: as the order masks, their work differs by
 // up to the whole length), else as many as bring it there, 8 at most, within 512 MB of partial sums
 int seq_attn_dkv_splits(int bf16, const SeqAttnArgs& A) {
-  const int rb = A.d > 128 ? 64 : 128;
+  const int rb = A.d <= (bf16 ? 128 : 64) ? 128 : A.d > 128 && bf16 ? 32 : 64;       // own rows of a workgroup
+
   const int64_t wgs = ((int64_t)A.tk + rb - 1) / rb * A.hk, bytes = (int64_t)A.tk * A.hk * A.d * 8;
   if (wgs == 0 || wgs >= 1024) return 1;
   const int64_t work = (int64_t)(A.hq / A.hk) * ((A.tq / (A.nseq > 0 ? A.nseq : 1) + 31) / 32);       // query tiles a key tile sees, about
@@ -674,14 +664,14 @@ static hipError_t pick(hipStream_t s, const SeqAttnArgs& A) {
     e = delta<T>(s, A);
     if (e != hipSuccess) return e;
     if (A.d <= 64) e = dq<SeqTile<T, 64, 1, 4, 64, VEC>>(s, A);
-    else if (A.d <= 128) e = dq<SeqTile<T, 128, sizeof(T) == 2 ? 1 : 2, sizeof(T) == 2 ? 4 : 8, sizeof(T) == 2 ? 64 : 32, VEC>>(s, A);
-    else e = dq<SeqTile<T, 256, sizeof(T) == 2 ? 2 : 4, 8, 32, VEC>>(s, A);
+    else if (A.d <= 128) e = dq<SeqTile<T, 128, sizeof(T) == 2 ? 1 : 2, 4, sizeof(T) == 2 ? 64 : 32, VEC>>(s, A);
+    else e = dq<SeqTile<T, 256, sizeof(T) == 2 ? 2 : 4, 4, 32, VEC>>(s, A);
     if (e != hipSuccess) return e;
   }
   if (A.tk == 0) return e;
   if (A.d <= 64) return dkv<SeqTile<T, 64, 1, 4, 64, VEC>>(s, A);
-  if (A.d <= 128) return dkv<SeqTile<T, 128, sizeof(T) == 2 ? 1 : 2, sizeof(T) == 2 ? 4 : 8, 32, VEC>>(s, A);
-  return dkv<SeqTile<T, 256, 4, 8, 32, VEC>>(s, A);
+  if (A.d <= 128) return dkv<SeqTile<T, 128, sizeof(T) == 2 ? 1 : 2, 4, 32, VEC>>(s, A);
+  return dkv<SeqTile<T, 256, 4, sizeof(T) == 2 ? 4 : 8, 32, VEC>>(s, A);
 }
 
 hipError_t launch_seq_attn_backward(hipStream_t s, int bf16, const SeqAttnArgs& A) {

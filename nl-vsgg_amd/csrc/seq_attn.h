@@ -13,6 +13,8 @@
 // registers (so that two waves share it), a team of DS = 2 or 4 waves shares 32 own rows, each contracting (scores) and accumulating
 // (reductions) its part of d; the partial scores meet in LDS.
 #pragma once
+#include <type_traits>
+
 #include "seq_common.h"
 
 namespace sttran {
@@ -35,7 +37,7 @@ struct SeqTile {
   static constexpr int kTileBytes = BR * RS;
   static constexpr int kStep = NT / NC;              // tile rows between a thread's chunks
   static_assert(BR * NC % NT == 0 && NT % NC == 0, "whole chunks");
-  static_assert(kStep % 8 == 0, "two source offsets: the layout's XOR repeats every 16 rows");
+  static_assert(2 * kStep % (ES == 4 ? 8 : 16) == 0, "two source offsets: the layout's XOR repeats every 8 (fp32) or 16 rows");
 };
 
 // chunk position of (row, chunk): an XOR that spreads both access patterns over the banks -- eight consecutive rows at one
@@ -286,41 +288,40 @@ __device__ __forceinline__ void seq_spread_store(char* out, char* out_lo, const 
   }
 }
 
-// ---- partial score blocks of the DS waves (a team) that share own rows.  Every wave of the workgroup passes the barrier between
-// put and get / share.
-template <class C>
-__device__ __forceinline__ seq_f32x4* seq_xch(char* xch, int wave, int blocks, int block) {
-  return reinterpret_cast<seq_f32x4*>(xch) + (wave * blocks + block) * 256 + (threadIdx.x & 63);
-}
+// ---- partial score blocks of the DS waves (a team) that share own rows.  A wave stores its block as four quads (registers
+// 4g .. 4g + 3), a quad as 16 bytes a lane; the barrier between writing and reading is the caller's.
 __device__ __forceinline__ seq_f32x4 seq_quad(const seq_f32x16& s, int g) {
   return seq_f32x4{s[4 * g], s[4 * g + 1], s[4 * g + 2], s[4 * g + 3]};
 }
-template <class C>
-__device__ __forceinline__ void seq_put(const seq_f32x16& s, char* xch, int wave, int blocks, int block) {
-  seq_f32x4* to = seq_xch<C>(xch, wave, blocks, block);
+__device__ __forceinline__ void seq_set_quad(seq_f32x16& s, int g, seq_f32x4 x) {
 #pragma unroll
-  for (int g = 0; g < 4; ++g) to[g * 64] = seq_quad(s, g);
+  for (int i = 0; i < 4; ++i) s[4 * g + i] = x[i];
 }
-// DS == 2: add the partner's block.  Both waves add the same two numbers, so both hold the same sum
-template <class C>
-__device__ __forceinline__ void seq_get(seq_f32x16& s, char* xch, int wave, int blocks, int block) {
-  const seq_f32x4* from = seq_xch<C>(xch, wave ^ 1, blocks, block);
+__device__ __forceinline__ seq_f32x4* seq_slot(char* at, int slot) {
+  return reinterpret_cast<seq_f32x4*>(at + slot * 1024) + (threadIdx.x & 63);
+}
+// B blocks a wave.  Member j of a team finishes quads j * GP .. (j + 1) * GP - 1: everyone puts its blocks; after a barrier the
+// finisher sums its quads over the members, in their order, and leaves what it made of them in its OWN slot of that quad, which
+// nobody else reads before the next barrier; after that, take() has the whole blocks.
+template <class C, int B>
+struct SeqShare {
+  static constexpr int GP = 4 / C::DS, kWave = B * 4096;
+  static __device__ __forceinline__ seq_f32x4* slot(char* xch, int wave, int block, int g) { return seq_slot(xch, (wave * B + block) * 4 + g); }
+  static __device__ __forceinline__ void put(const seq_f32x16& s, char* xch, int wave, int block) {
 #pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    const seq_f32x4 o = from[g * 64];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) s[4 * g + u] += o[u];
+    for (int g = 0; g < 4; ++g) *slot(xch, wave, block, g) = seq_quad(s, g);
   }
-}
-// the whole sum of quad g (registers 4g .. 4g + 3), members in order
-template <class C>
-__device__ __forceinline__ seq_f32x4 seq_sum_quad(char* xch, int wave, int blocks, int block, int g) {
-  const int first = wave - wave % C::DS;
-  seq_f32x4 r = seq_xch<C>(xch, first, blocks, block)[g * 64];
+  static __device__ __forceinline__ seq_f32x4 sum(char* xch, int first, int block, int g) {
+    seq_f32x4 r = *slot(xch, first, block, g);
 #pragma unroll
-  for (int m = 1; m < C::DS; ++m) r += seq_xch<C>(xch, first + m, blocks, block)[g * 64];
-  return r;
-}
+    for (int m = 1; m < C::DS; ++m) r += *slot(xch, first + m, block, g);
+    return r;
+  }
+  static __device__ __forceinline__ void take(seq_f32x16& s, char* xch, int first, int block) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) seq_set_quad(s, g, *slot(xch, first + g / GP, block, g));
+  }
+};
 
 // Z[d][own row] registers -> a contiguous output row
 template <class C>
