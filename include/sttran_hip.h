@@ -349,7 +349,7 @@ int sttran_attention_backward(const SttranAttention* args, void* stream);
 
 /* One new token a sequence: q [num_seq, num_q_heads, head_dim] over the first lengths[s] rows (clamped to capacity) of the caches
  * k / v [num_seq, capacity, num_kv_heads, head_dim]; the token's place is lengths[s] - 1.  Same z as above; length 0 gives zeros.
- * Rows from lengths[s] on are not read.  num_seq <= 65535.  Workspace: sttran_attention_step_workspace_bytes(args). */
+ * Rows from lengths[s] on are not read.  num_seq <= 65535; a row stride is at most 2^22 bytes.  Workspace: sttran_attention_step_workspace_bytes(args). */
 typedef struct SttranAttentionStep {
   uint32_t struct_size;            /* = sizeof(SttranAttentionStep) */
   int32_t dtype;

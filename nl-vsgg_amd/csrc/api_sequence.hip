@@ -9,7 +9,7 @@ using namespace sttran;
 
 namespace {
 
-constexpr int64_t kMaxRows = (int64_t(1) << 31) - 1024, kMaxRowBytes = int64_t(1) << 24;
+constexpr int64_t kMaxRows = (int64_t(1) << 31) - 1024, kMaxRowBytes = int64_t(1) << 24, kMaxCacheRowBytes = int64_t(1) << 22;
 
 bool dtype_ok(int32_t t) { return t == STTRAN_DTYPE_F32 || t == STTRAN_DTYPE_BF16; }
 int elt(int32_t t) { return t == STTRAN_DTYPE_BF16 ? 2 : 4; }
@@ -28,7 +28,7 @@ struct Alignment {
   }
 };
 
-bool row_stride_ok(int64_t s, int es) { return s >= 0 && s * es <= kMaxRowBytes; }
+bool row_stride_ok(int64_t s, int es, int64_t most = kMaxRowBytes) { return s >= 0 && s <= most && s * es <= most; }
 bool head_stride_ok(int64_t s) { return s >= 0 && s < (int64_t(1) << 40); }
 
 hipStream_t str(void* s) { return reinterpret_cast<hipStream_t>(s); }
@@ -77,7 +77,7 @@ bool step_args(const SttranAttentionStep* a, SeqStepArgs& A) {
   if (a->num_seq < 0 || a->num_seq > 65535 || a->capacity < 0 || a->capacity > kMaxRows) return false;
   if (!number(a->score_cap) || a->score_cap < 0.f || !number(a->scale)) return false;
   const int es = elt(a->dtype);
-  if (!row_stride_ok(a->k_row_stride, es) || !row_stride_ok(a->v_row_stride, es) || !head_stride_ok(a->q_seq_stride) ||
+  if (!row_stride_ok(a->k_row_stride, es, kMaxCacheRowBytes) || !row_stride_ok(a->v_row_stride, es, kMaxCacheRowBytes) || !head_stride_ok(a->q_seq_stride) ||
       !head_stride_ok(a->q_head_stride) || !head_stride_ok(a->k_seq_stride) || !head_stride_ok(a->k_head_stride) ||
       !head_stride_ok(a->v_seq_stride) || !head_stride_ok(a->v_head_stride))
     return false;

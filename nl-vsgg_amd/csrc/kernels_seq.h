@@ -42,6 +42,7 @@ struct SeqRotaryArgs {
   const float* freq;               // [rot / 2] angle a position step
   int64_t tokens;
   int heads[2], d, rot, interleaved, aln;
+  uint32_t per_head;               // the launch's own
   float eps;
 };
 int seq_rotary_groups(const SeqRotaryArgs& A);          // workgroups of a backward launch

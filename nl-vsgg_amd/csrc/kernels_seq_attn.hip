@@ -231,49 +231,66 @@ seq_attn_fwd_kernel(SeqAttnArgs A) {
   if (A.lse && dh == 0 && h == 0) A.lse[(int64_t)head * A.tq + row] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
-// joins the shares of a launch that was split over the keys, in the order of the splits: one wave a (row, head)
+// joins the shares of a launch that was split over the keys: one workgroup a (row, head).  The waves take the shares in turn, their
+// sums are added in the order of the waves
 template <class T>
 __global__ void __launch_bounds__(256) seq_attn_join_kernel(SeqAttnArgs A, const int* lens, int chunk, int capacity) {
-  const int lane = threadIdx.x & 63;
-  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);         // head * tq + row
-  if (i >= (int64_t)A.hq * A.tq) return;
+  __shared__ float sm[4][256], wt[256], red[8];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int64_t i = blockIdx.x;                                            // head * tq + row
   const int head = (int)(i / A.tq), row = (int)(i % A.tq);
   const int64_t step = (int64_t)A.hq * A.tq;
   const int shares = lens ? min((min(max(lens[row], 1), capacity) + chunk - 1) / chunk, A.splits) : A.splits;
-  const float* ps = A.part + (int64_t)A.splits * step * A.d;
+  const float *ps = A.part + (int64_t)A.splits * step * A.d + i * 2, *po = A.part + i * A.d;
   float m = -INFINITY;
-  for (int s = 0; s < shares; ++s) m = fmaxf(m, ps[(s * step + i) * 2]);
+  for (int s = tid; s < shares; s += 256) m = fmaxf(m, ps[s * step * 2]);
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+  if (lane == 0) red[w] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
   const float ms = m == -INFINITY ? 0.f : m;
   float o[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
-  for (int s = 0; s < shares; ++s) {
-    const float mx = ps[(s * step + i) * 2], lx = ps[(s * step + i) * 2 + 1];
-    if (lx == 0.f) continue;                                               // nothing visible there
-    const float f = __builtin_amdgcn_exp2f(mx - ms);
-    l = fmaf(lx, f, l);
-    const float* po = A.part + (s * step + i) * A.d;
+  for (int s0 = 0; s0 < shares; s0 += 256) {                               // a share that saw nothing weighs exp(-inf) = 0
+    float f = 0.f;
+    if (s0 + tid < shares) {
+      f = __builtin_amdgcn_exp2f(ps[(s0 + tid) * step * 2] - ms);
+      l = fmaf(ps[(s0 + tid) * step * 2 + 1], f, l);
+    }
+    __syncthreads();
+    wt[tid] = f;
+    __syncthreads();
+    const int n = min(shares - s0, 256);
+#pragma unroll 8
+    for (int s = w; s < n; s += 4) {
+      const float* p = po + (s0 + s) * step * A.d;
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (lane + 64 * u < A.d) o[u] = fmaf(po[lane + 64 * u], f, o[u]);
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  const int64_t at = ((int64_t)row * A.hq + head) * A.d;
-#pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    if (lane + 64 * u >= A.d) continue;
-    const float x = o[u] * inv;
-    if constexpr (sizeof(T) == 4) {
-      reinterpret_cast<float*>(A.out)[at + lane + 64 * u] = x;
-    } else {
-      const float y = SeqElt<T>::round(x);
-      reinterpret_cast<uint16_t*>(A.out)[at + lane + 64 * u] = (uint16_t)SeqElt<T>::bits(y);
-      if (A.out_lo) reinterpret_cast<uint16_t*>(A.out_lo)[at + lane + 64 * u] = (uint16_t)SeqElt<T>::bits(x - y);
+      for (int u = 0; u < 4; ++u) o[u] = fmaf(lane + 64 * u < A.d ? p[lane + 64 * u] : 0.f, wt[s], o[u]);
     }
   }
-  if (A.lse && lane == 0) A.lse[i] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+  l = seq_group_sum<64>(l);
+  if (lane == 0) red[4 + w] = l;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) sm[w][lane + 64 * u] = o[u];
+  __syncthreads();
+  l = ((red[4] + red[5]) + red[6]) + red[7];
+  const int col = threadIdx.x;
+  if (col < A.d) {
+    const float x = (((sm[0][col] + sm[1][col]) + sm[2][col]) + sm[3][col]) * (l == 0.f ? 0.f : 1.f / l);
+    const int64_t at = ((int64_t)row * A.hq + head) * A.d + col;
+    if constexpr (sizeof(T) == 4) {
+      reinterpret_cast<float*>(A.out)[at] = x;
+    } else {
+      const float y = SeqElt<T>::round(x);
+      reinterpret_cast<uint16_t*>(A.out)[at] = (uint16_t)SeqElt<T>::bits(y);
+      if (A.out_lo) reinterpret_cast<uint16_t*>(A.out_lo)[at] = (uint16_t)SeqElt<T>::bits(x - y);
+    }
+  }
+  if (A.lse && threadIdx.x == 0) A.lse[i] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
 hipError_t launch_seq_attn_join(hipStream_t s, int bf16, const SeqAttnArgs& A, const int* lens, int chunk, int capacity) {
-  const unsigned grid = (unsigned)(((int64_t)A.hq * A.tq + 3) / 4);
+  const unsigned grid = (unsigned)((int64_t)A.hq * A.tq);
   if (bf16) seq_attn_join_kernel<__bf16><<<grid, 256, 0, s>>>(A, lens, chunk, capacity);
   else seq_attn_join_kernel<float><<<grid, 256, 0, s>>>(A, lens, chunk, capacity);
   return hipGetLastError();

@@ -21,17 +21,15 @@ __global__ void __launch_bounds__(256) seq_attn_delta_kernel(SeqAttnArgs A) {
   const int c = threadIdx.x % LPR;
   if (item >= (int64_t)A.tq * A.hq) return;
   const int row = (int)(item / A.hq), head = (int)(item % A.hq), dbytes = A.d * (int)sizeof(T);
-  const int valid = dbytes - 16 * c;
-  const seq_u32x4 g = seq_load16(A.dout + row * A.do_t + head * A.do_h + 16 * c, valid, A.aln);
-  const seq_u32x4 o = seq_load16(A.out + item * dbytes + 16 * c, valid, A.aln);
+  const seq_u32x4 g = seq_row_chunk(A.dout + row * A.do_t + head * A.do_h, c, dbytes, A.aln);
+  const seq_u32x4 o = seq_row_chunk(A.out + item * dbytes, c, dbytes, A.aln);
   seq_u32x4 r = {0, 0, 0, 0};
-  if (A.out_lo) r = seq_load16(A.out_lo + item * dbytes + 16 * c, valid, A.aln);
+  if (A.out_lo) r = seq_row_chunk(A.out_lo + item * dbytes, c, dbytes, A.aln);
   float s = 0.f;
 #pragma unroll
   for (int i = 0; i < SeqElt<T>::kPer16; ++i)
     s = fmaf(SeqElt<T>::get(g, i), SeqElt<T>::get(o, i) + (sizeof(T) == 2 ? SeqElt<T>::get(r, i) : 0.f), s);
-#pragma unroll
-  for (int x = 1; x < LPR; x <<= 1) s += __shfl_xor(s, x);
+  s = seq_group_sum<LPR>(s);
   if (c) return;
   A.delta[(int64_t)head * A.tq + row] = s;
   if (head == 0) {

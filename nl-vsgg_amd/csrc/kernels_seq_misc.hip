@@ -5,195 +5,217 @@ namespace sttran {
 
 // ---- rotary positions ------------------------------------------------------------------------------------------------------
 // y = R(pos) x' with x' = w * x / sqrt(mean(x^2) + eps) (or x' = x without a norm).  R turns pair i of the first `rot` columns by
-// pos * freq_i; the pair is (2i, 2i + 1) (interleaved) or (i, i + rot / 2) (halves); columns from rot on pass.
-// Bound by memory: one read and one write of q and k.  A workgroup takes TT tokens at a time with all their heads, so an
-// angle's cosine and sine are taken once a token: in 64 bits up to the turn's fraction (a far position times a frequency
-// has no exact fraction in 32), then in fp32.  LPR lanes hold one row, 16 bytes each; a pair's other half comes through LDS.
-template <int LPR>
-struct SeqRot {
-  static constexpr int kRows = 256 / LPR;                 // rows in flight
-  int rot, half;
-  bool inter;
-  float* row;                                             // this row's LDS copy, rounded up to whole chunks
-  // out[i] = the turned value of column e0 + i; sign -1: the turn back
-  template <int EPL>
-  __device__ __forceinline__ void turn(float (&x)[EPL], const float* cs, float sign, int c) const {
-    const int e0 = c * EPL;
-    if (inter) {
-#pragma unroll
-      for (int j = 0; j < EPL / 2; ++j) {
-        const int i = e0 / 2 + j;
-        if (i >= half) continue;
-        const float co = cs[2 * i], si = sign * cs[2 * i + 1], a = x[2 * j], b = x[2 * j + 1];
-        x[2 * j] = a * co - b * si;
-        x[2 * j + 1] = b * co + a * si;
-      }
-      return;
-    }
-    // rows live in one wave: its own LDS writes are visible to it once they are done
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-    for (int j = 0; j < EPL; ++j) row[e0 + j] = x[j];
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#pragma unroll
-    for (int j = 0; j < EPL; ++j) {
-      const int e = e0 + j;
-      if (e >= rot) continue;
-      const bool first = e < half;
-      const int i = first ? e : e - half;
-      const float other = row[first ? e + half : i], co = cs[2 * i], si = sign * cs[2 * i + 1];
-      x[j] = first ? x[j] * co - other * si : x[j] * co + other * si;
-    }
-    __builtin_amdgcn_wave_barrier();
-  }
-};
-
-__device__ __forceinline__ void seq_angles(const SeqRotaryArgs& A, float* cs, int64_t t0, int tt) {
-  const int half = A.rot / 2;
-  for (int i = threadIdx.x; i < tt * half; i += 256) {
-    const int t = i / half, f = i % half;
-    float co = 1.f, si = 0.f;
-    if (t0 + t < A.tokens) {
-      const double turns = (double)A.pos[t0 + t] * ((double)A.freq[f] * 0.15915494309189533577);   // 1 / (2 pi)
-      const float frac = (float)(turns - rint(turns));
-      sincospif(2.f * frac, &si, &co);
-    }
-    cs[2 * i] = co; cs[2 * i + 1] = si;
-  }
-}
-
+// pos * freq_i; the pair is (2i, 2i + 1) (interleaved) or (i, i + rot / 2) (halves); columns from rot on pass:
+//   y[e] = x'[e] * C[e] + x'[partner(e)] * S[e],   C = cos, S = -sin / +sin on a pair's first / second column, 1 and 0 behind rot.
+// The backward pass turns dy back (S negated) and takes the norm's gradient from it.
+// Bound by memory: one read and one write of q and k (and of their gradients).  A workgroup takes TT tokens at a time with all
+// their heads, so C and S are made once a token: the angle in 64 bits up to the turn's fraction (a far position times a frequency
+// has no exact fraction in 32), then in fp32.  LPR lanes hold one row, 16 bytes each; the halves' partners come through LDS.
+// What bounds it is the bytes in flight, so registers are kept low for more waves: 8 a SIMD forward (110 us at 7), 5 backward (166 us
+// at 4); the rows' next pass fetched ahead cost registers and was slower (135 / 266 us), and so were larger grids.
+// Measured (32768 tokens, 16 + 4 heads of 128 columns, 96 turned, bfloat16, norm): 93 us forward (3.6 TB/s), 150 us backward (3.4 TB/s) and
+// 6 us for the weights' gradients.
 template <class T, int LPR, bool BWD>
-__global__ void __launch_bounds__(256) seq_rotary_kernel(SeqRotaryArgs A, int TT) {
-  constexpr int EPL = SeqElt<T>::kPer16, ROWS = 256 / LPR;
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(BWD ? 5 : 8, 8))) seq_rotary_kernel(SeqRotaryArgs A, int TT) {
+  constexpr int EPL = SeqElt<T>::kPer16, ROWS = 256 / LPR, ROW = LPR * EPL;
   extern __shared__ __attribute__((aligned(16))) float sm[];
-  float* cs = sm;                                          // [TT][rot / 2][2]
-  const int rowlen = LPR * EPL, c = threadIdx.x % LPR, r0 = threadIdx.x / LPR;
-  SeqRot<LPR> R{A.rot, A.rot / 2, A.interleaved != 0, sm + (TT * A.rot + 3) / 4 * 4 + r0 * rowlen};
+  const int c = threadIdx.x % LPR, r0 = threadIdx.x / LPR, e0 = c * EPL, half = A.rot / 2;
+  float* const wts = sm + TT * 2 * ROW;                    // behind the angles [TT][C | S][ROW]: the weights of q and of k,
+  float* const row = wts + 2 * ROW + r0 * ROW;             // then a copy of this lane's row
   const int heads = A.heads[0] + A.heads[1], dbytes = A.d * (int)sizeof(T), valid = dbytes - 16 * c;
+  const bool norm = A.w[0] != nullptr, swap = !A.interleaved && A.rot > 0, chunked = half % EPL == 0;
   float dw[2][EPL];
 #pragma unroll
   for (int j = 0; j < EPL; ++j) dw[0][j] = dw[1][j] = 0.f;
+  if (norm)
+    for (int i = threadIdx.x; i < 2 * ROW; i += 256) wts[i] = i % ROW < A.d ? A.w[i / ROW][i % ROW] : 0.f;
+  const float per_d = 1.f / (float)A.d;
+  for (int i = threadIdx.x; i < TT * (ROW - A.rot); i += 256) {              // the columns that pass
+    const int t = i / (ROW - A.rot), e = A.rot + i % (ROW - A.rot);
+    sm[t * 2 * ROW + e] = 1.f;
+    sm[t * 2 * ROW + ROW + e] = 0.f;
+  }
 
+  const int rows = TT * heads;
+  struct Where { int t, which, head; int64_t token; bool on; };
+  const auto where = [&](int64_t t0, int b) __attribute__((always_inline)) {
+    const int r = min(b + r0, rows - 1);
+    Where p;
+    p.t = heads > 1 ? (int)__umulhi((uint32_t)r, A.per_head) : r;
+    const int hh = r - p.t * heads;
+    p.which = hh >= A.heads[0] ? 1 : 0;
+    p.head = p.which ? hh - A.heads[0] : hh;
+    p.token = t0 + p.t < A.tokens ? t0 + p.t : A.tokens - 1;
+    p.on = b + r0 < rows && t0 + p.t < A.tokens;
+    return p;
+  };
   for (int64_t t0 = (int64_t)blockIdx.x * TT; t0 < A.tokens; t0 += (int64_t)gridDim.x * TT) {
     __syncthreads();
-    seq_angles(A, cs, t0, TT);
+    for (int i = threadIdx.x; i < TT * half; i += 256) {
+      const int t = i / half, f = i % half;
+      const int64_t token = t0 + t < A.tokens ? t0 + t : A.tokens - 1;
+      const double turns = (double)A.pos[token] * ((double)A.freq[f] * 0.15915494309189533577);   // 1 / (2 pi)
+      float co, si;
+      sincospif(2.f * (float)(turns - rint(turns)), &si, &co);
+      float* C = sm + t * 2 * ROW;
+      const int a = A.interleaved ? 2 * f : f, b = A.interleaved ? a + 1 : f + half;
+      C[a] = co; C[b] = co;
+      C[ROW + a] = BWD ? si : -si; C[ROW + b] = BWD ? -si : si;
+    }
     __syncthreads();
-    const int rows = TT * heads;
     for (int b = 0; b < rows; b += ROWS) {
-      const int r = b + r0, t = min(r, rows - 1) / heads, hh = min(r, rows - 1) % heads;
-      const int which = hh >= A.heads[0] ? 1 : 0, head = which ? hh - A.heads[0] : hh;
-      const int64_t token = t0 + t;
-      const bool on = r < rows && token < A.tokens;
-      const float* cst = cs + t * A.rot;
-      const float* w = A.w[which];
-      const int64_t at = (token * A.heads[which] + head) * dbytes + 16 * c;
-      float x[EPL], inv = 1.f;
-      const bool need_x = !BWD || w;
-      seq_u32x4 xr = {0, 0, 0, 0};
-      if (need_x) xr = seq_load16(A.x[which] + token * A.x_t[which] + head * A.x_h[which] + 16 * c, on ? valid : 0, A.aln);
+      const Where p = where(t0, b);
+      seq_u32x4 xr = {0, 0, 0, 0}, gr = {0, 0, 0, 0};
+      if (!BWD || norm) xr = seq_row_chunk(A.x[p.which] + p.token * A.x_t[p.which] + p.head * A.x_h[p.which], c, dbytes, A.aln);
+      if (BWD) gr = seq_row_chunk(A.dy[p.which] + p.token * A.dy_t[p.which] + p.head * A.dy_h[p.which], c, dbytes, A.aln);
+      const int t = p.t, which = p.which;
+      const bool on = p.on;
+      const int64_t at = (p.token * A.heads[which] + p.head) * dbytes;
+      float x[EPL], y[EPL], wj[EPL], inv = 1.f;
 #pragma unroll
-      for (int j = 0; j < EPL; ++j) x[j] = SeqElt<T>::get(xr, j);
-      float wj[EPL];
-      if (w) {
+      for (int j = 0; j < EPL; ++j) {
+        x[j] = SeqElt<T>::get(xr, j);
+        wj[j] = 1.f;
+      }
+      if (norm) {
+#pragma unroll
+        for (int j = 0; j < EPL; j += 4) {
+          const seq_f32x4 a = *reinterpret_cast<const seq_f32x4*>(wts + which * ROW + e0 + j);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) wj[j + u] = a[u];
+        }
         float s = 0.f;
 #pragma unroll
-        for (int j = 0; j < EPL; ++j) {
-          s = fmaf(x[j], x[j], s);
-          wj[j] = c * EPL + j < A.d ? w[c * EPL + j] : 0.f;
-        }
-#pragma unroll
-        for (int o = 1; o < LPR; o <<= 1) s += __shfl_xor(s, o);
-        inv = 1.f / sqrtf(s / (float)A.d + A.eps);
+        for (int j = 0; j < EPL; ++j) s = fmaf(x[j], x[j], s);
+        inv = rsqrtf(seq_group_sum<LPR>(s) * per_d + A.eps);
 #pragma unroll
         for (int j = 0; j < EPL; ++j) x[j] *= inv;
       }
-      float y[EPL];
-      if constexpr (!BWD) {
 #pragma unroll
-        for (int j = 0; j < EPL; ++j) y[j] = w ? x[j] * wj[j] : x[j];
-        R.template turn<EPL>(y, cst, 1.f, c);
-      } else {
-        const seq_u32x4 gr = seq_load16(A.dy[which] + token * A.dy_t[which] + head * A.dy_h[which] + 16 * c, on ? valid : 0, A.aln);
-        float g[EPL];
+      for (int j = 0; j < EPL; ++j) y[j] = BWD ? SeqElt<T>::get(gr, j) : x[j] * wj[j];
+      // the turn
+      const float* C = sm + t * 2 * ROW + e0;
+      float co[EPL], si[EPL], z[EPL];
 #pragma unroll
-        for (int j = 0; j < EPL; ++j) g[j] = SeqElt<T>::get(gr, j);
-        R.template turn<EPL>(g, cst, -1.f, c);
-        if (w) {
-          float s = 0.f;
+      for (int j = 0; j < EPL; j += 4) {
+        const seq_f32x4 a = *reinterpret_cast<const seq_f32x4*>(C + j), b4 = *reinterpret_cast<const seq_f32x4*>(C + ROW + j);
 #pragma unroll
-          for (int j = 0; j < EPL; ++j) {
-            const float gx = g[j] * x[j];
-            if (which) dw[1][j] += gx; else dw[0][j] += gx;
-            s = fmaf(gx, wj[j], s);
+        for (int u = 0; u < 4; ++u) { co[j + u] = a[u]; si[j + u] = b4[u]; }
+      }
+      if (swap) {
+        // a row lives in one wave, whose LDS accesses keep their order: only the compiler must
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int j = 0; j < EPL; j += 4) *reinterpret_cast<seq_f32x4*>(row + e0 + j) = seq_f32x4{y[j], y[j + 1], y[j + 2], y[j + 3]};
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        if (chunked) {
+          const float* p = row + (e0 < half ? e0 + half : e0 < A.rot ? e0 - half : e0);
+#pragma unroll
+          for (int j = 0; j < EPL; j += 4) {
+            const seq_f32x4 a = *reinterpret_cast<const seq_f32x4*>(p + j);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) z[j + u] = a[u];
           }
-#pragma unroll
-          for (int o = 1; o < LPR; o <<= 1) s += __shfl_xor(s, o);
-          s /= (float)A.d;
-#pragma unroll
-          for (int j = 0; j < EPL; ++j) y[j] = inv * (g[j] * wj[j] - x[j] * s);
         } else {
 #pragma unroll
-          for (int j = 0; j < EPL; ++j) y[j] = g[j];
+          for (int j = 0; j < EPL; ++j) {
+            const int e = e0 + j;
+            z[j] = row[e < half ? e + half : e < A.rot ? e - half : e];
+          }
         }
+        __builtin_amdgcn_wave_barrier();
+      } else {
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) z[j] = y[j ^ 1];
       }
       seq_u32x4 out = {0, 0, 0, 0};
 #pragma unroll
+      for (int j = 0; j < EPL; ++j) y[j] = fmaf(z[j], si[j], y[j] * co[j]);
+      if (BWD && norm) {
+        float s = 0.f;
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) {
+          const float gx = on ? y[j] * x[j] : 0.f;
+          dw[0][j] += which ? 0.f : gx;
+          dw[1][j] += which ? gx : 0.f;
+          s = fmaf(y[j] * x[j], wj[j], s);
+        }
+        s = seq_group_sum<LPR>(s) * per_d;
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) y[j] = inv * (y[j] * wj[j] - x[j] * s);
+      }
+#pragma unroll
       for (int j = 0; j < EPL; ++j) SeqElt<T>::put(out, j, y[j]);
-      if (on) seq_store16((BWD ? A.dx[which] : A.y[which]) + at, out, valid, A.aln);
+      if (on) seq_store16((BWD ? A.dx[which] : A.y[which]) + at + 16 * c, out, valid, A.aln);
     }
   }
   if constexpr (BWD) {
     if (!A.part) return;
     // this workgroup's share of the weight gradients: rows in the order r0 = 0, 1, ...
-    float* buf = sm;                                       // [ROWS][rowlen]
     for (int which = 0; which < 2; ++which) {
       __syncthreads();
 #pragma unroll
-      for (int j = 0; j < EPL; ++j) buf[r0 * rowlen + c * EPL + j] = dw[which][j];
+      for (int j = 0; j < EPL; ++j) sm[r0 * ROW + e0 + j] = dw[which][j];
       __syncthreads();
       for (int e = threadIdx.x; e < A.d; e += 256) {
         float s = 0.f;
-        for (int r = 0; r < ROWS; ++r) s += buf[r * rowlen + e];
+        for (int r = 0; r < ROWS; ++r) s += sm[r * ROW + e];
         A.part[((int64_t)blockIdx.x * 2 + which) * A.d + e] = s;
       }
     }
   }
 }
 
-// joins the workgroups' shares in a fixed order, in 64 bits: one workgroup 64 columns, four partial sums a column
-__global__ void __launch_bounds__(256) seq_rotary_dw_kernel(SeqRotaryArgs A, int groups) {
-  __shared__ double sm[256];
+// joins the workgroups' shares in a fixed order, in 64 bits: one workgroup 64 columns, sixteen partial sums a column
+__global__ void __launch_bounds__(1024) seq_rotary_dw_kernel(SeqRotaryArgs A, int groups) {
+  __shared__ double sm[1024];
   const int which = blockIdx.y, e = blockIdx.x * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6;
   double s = 0.;
-  if (e < A.d)
-    for (int g = q; g < groups; g += 4) s += A.part[((int64_t)g * 2 + which) * A.d + e];
+  if (e < A.d) {
+    const float* p = A.part + (int64_t)which * A.d + e;
+#pragma unroll 8
+    for (int g = q; g < groups; g += 16) s += p[(int64_t)g * 2 * A.d];
+  }
   sm[threadIdx.x] = s;
   __syncthreads();
-  if (q == 0 && e < A.d && A.dw[which]) A.dw[which][e] = (float)(((sm[threadIdx.x] + sm[threadIdx.x + 64]) + sm[threadIdx.x + 128]) + sm[threadIdx.x + 192]);
+  if (q == 0 && e < A.d && A.dw[which]) {
+    for (int i = 1; i < 16; ++i) s += sm[threadIdx.x + 64 * i];
+    A.dw[which][e] = (float)s;
+  }
 }
 
 static int rotary_tt(const SeqRotaryArgs& A) { return A.tokens >= 4096 ? 4 : 1; }
 int seq_rotary_groups(const SeqRotaryArgs& A) {
   const int64_t tiles = (A.tokens + rotary_tt(A) - 1) / rotary_tt(A);
-  return (int)(tiles < 1024 ? tiles : 1024);
+  return (int)(tiles < 1280 ? tiles : 1280);
 }
 
+template <class T, int LPR, bool BWD>
+static hipError_t rotary_lpr(hipStream_t s, SeqRotaryArgs A) {
+  const int tt = rotary_tt(A), heads = A.heads[0] + A.heads[1];
+  A.per_head = heads > 1 ? (uint32_t)(((uint64_t)1 << 32) / heads + 1) : 0;      // r / heads = high half of r * per_head
+  const int64_t tiles = (A.tokens + tt - 1) / tt;
+  const unsigned grid = BWD ? (unsigned)seq_rotary_groups(A) : (unsigned)(tiles < 2048 ? tiles : 2048);
+  constexpr int row = LPR * SeqElt<T>::kPer16;
+  const int lds = (tt * 2 * row + 2 * row + 256 / LPR * row) * 4;                // angles, weights, rows (or the gradient's shares)
+  seq_rotary_kernel<T, LPR, BWD><<<grid, 256, lds, s>>>(A, tt);
+  return hipGetLastError();
+}
+static hipError_t rotary_dw(hipStream_t s, const SeqRotaryArgs& A, int groups) {
+  seq_rotary_dw_kernel<<<dim3((unsigned)((A.d + 63) / 64), 2), 1024, 0, s>>>(A, groups);
+  return hipGetLastError();
+}
 template <class T, bool BWD>
 static hipError_t rotary(hipStream_t s, const SeqRotaryArgs& A) {
-  const int tt = rotary_tt(A), chunks = (A.d * (int)sizeof(T) + 15) / 16;
-  const int64_t tiles = (A.tokens + tt - 1) / tt;
-  const unsigned grid = BWD ? (unsigned)seq_rotary_groups(A) : (unsigned)(tiles < 16384 ? tiles : 16384);
-  const int lds = ((tt * A.rot + 3) / 4 * 4 + 256 * SeqElt<T>::kPer16) * 4;        // angles + rows (or the gradient's shares)
-  if (chunks <= 8) seq_rotary_kernel<T, 8, BWD><<<grid, 256, lds, s>>>(A, tt);
-  else if (chunks <= 16) seq_rotary_kernel<T, 16, BWD><<<grid, 256, lds, s>>>(A, tt);
-  else if (chunks <= 32) seq_rotary_kernel<T, 32, BWD><<<grid, 256, lds, s>>>(A, tt);
-  else if constexpr (sizeof(T) == 4) seq_rotary_kernel<T, 64, BWD><<<grid, 256, lds, s>>>(A, tt);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || !BWD || !A.part) return e;
-  seq_rotary_dw_kernel<<<dim3((unsigned)((A.d + 63) / 64), 2), 256, 0, s>>>(A, (int)grid);
-  return hipGetLastError();
+  const int chunks = (A.d * (int)sizeof(T) + 15) / 16;
+  hipError_t e = hipSuccess;
+  if (chunks <= 8) e = rotary_lpr<T, 8, BWD>(s, A);
+  else if (chunks <= 16) e = rotary_lpr<T, 16, BWD>(s, A);
+  else if (chunks <= 32) e = rotary_lpr<T, 32, BWD>(s, A);
+  else if constexpr (sizeof(T) == 4) e = rotary_lpr<T, 64, BWD>(s, A);
+  return e != hipSuccess || !BWD || !A.part ? e : rotary_dw(s, A, seq_rotary_groups(A));
 }
 
 hipError_t launch_seq_rotary_forward(hipStream_t s, int bf16, const SeqRotaryArgs& A) {
@@ -202,9 +224,7 @@ hipError_t launch_seq_rotary_forward(hipStream_t s, int bf16, const SeqRotaryArg
 }
 hipError_t launch_seq_rotary_backward(hipStream_t s, int bf16, const SeqRotaryArgs& A) {
   if (A.tokens == 0) {                                     // no rows: the weights' gradients are zeros all the same
-    if (!A.part) return hipSuccess;
-    seq_rotary_dw_kernel<<<dim3((unsigned)((A.d + 63) / 64), 2), 256, 0, s>>>(A, 0);
-    return hipGetLastError();
+    return A.part ? rotary_dw(s, A, 0) : hipSuccess;
   }
   return bf16 ? rotary<__bf16, true>(s, A) : rotary<float, true>(s, A);
 }

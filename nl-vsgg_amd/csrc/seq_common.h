@@ -33,6 +33,23 @@ __device__ __forceinline__ seq_u32x4 seq_load16(const char* p, int valid, int al
   return r;
 }
 
+// chunk c of a row at `row`, what lies behind the row's dbytes as zeros, without branches between lanes (a divergent tail makes
+// every load of a loop wait by itself): chunks at the row's end read its last 16 bytes and shift them (selects alone: the same as
+// an if / else if chain over the tail's length has been compiled to a path that skips one of them)
+__device__ __forceinline__ seq_u32x4 seq_row_chunk(const char* row, int c, int dbytes, int aln) {
+  if (aln < 4 || dbytes < 16) return seq_load16(row + 16 * c, dbytes - 16 * c, aln);
+  const int at = min(16 * c, dbytes - 16), skip = (16 * c - at) >> 2;          // dwords of it that lie before the chunk
+  const seq_u32x4 r = *reinterpret_cast<const seq_u32x4_a4*>(row + at);
+  if ((dbytes & 15) == 0 && dbytes >= 16 * 64) return r;
+  const bool s1 = skip == 1, s2 = skip == 2, s3 = skip == 3, s0 = skip == 0;
+  seq_u32x4 x;
+  x[0] = s0 ? r[0] : s1 ? r[1] : s2 ? r[2] : s3 ? r[3] : 0u;
+  x[1] = s0 ? r[1] : s1 ? r[2] : s2 ? r[3] : 0u;
+  x[2] = s0 ? r[2] : s1 ? r[3] : 0u;
+  x[3] = s0 ? r[3] : 0u;
+  return x;
+}
+
 __device__ __forceinline__ void seq_store16(char* p, seq_u32x4 r, int valid, int aln) {
   if (valid >= 16 && aln >= 4) {
     *reinterpret_cast<seq_u32x4_a4*>(p) = r;
@@ -70,6 +87,34 @@ template <> struct SeqElt<__bf16> {
   }
   static __device__ __forceinline__ float round(float x) { return (float)(__bf16)x; }
 };
+
+// ---- lane exchanges without LDS traffic (DPP: within rows of 16 lanes; permlane swaps: between rows)
+template <int CTRL>
+__device__ __forceinline__ float seq_dpp(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, false));
+}
+constexpr int kDppXor1 = 0xB1, kDppXor3 = 0x1B, kDppXor7 = 0x141, kDppXor15 = 0x140;    // quad_perm, row_half_mirror, row_mirror
+template <int N> __device__ __forceinline__ float seq_ror(float x) { return seq_dpp<0x120 + N>(x); }         // lane i from i - N of 16
+template <int N> __device__ __forceinline__ float seq_bcast(float x) { return seq_dpp<0x150 + N>(x); }       // lane N of the row
+__device__ __forceinline__ float seq_add16(float x) {                                                        // x + lane ^ 16
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float seq_add32(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// sum over groups of N lanes, the same bits in each of them
+template <int N>
+__device__ __forceinline__ float seq_group_sum(float x) {
+  x += seq_dpp<kDppXor1>(x);
+  if constexpr (N > 2) x += seq_dpp<kDppXor3>(x);
+  if constexpr (N > 4) x += seq_dpp<kDppXor7>(x);
+  if constexpr (N > 8) x += seq_dpp<kDppXor15>(x);
+  if constexpr (N > 16) x = seq_add16(x);
+  if constexpr (N > 32) x = seq_add32(x);
+  return x;
+}
 
 // ---- attention over packed sequences: arguments of the launches (strides in BYTES) ---------------------------------------
 struct SeqAttnArgs {

@@ -23,7 +23,7 @@ from .. import _native as nat
 
 _DTYPES = {torch.float32: nat.DTYPE_F32, torch.bfloat16: nat.DTYPE_BF16}
 _ATT_SIZE, _STEP_SIZE, _ROT_SIZE = (C.sizeof(t) for t in (nat.SttranAttention, nat.SttranAttentionStep, nat.SttranRotary))
-_MAX_ROW_BYTES = 1 << 24
+_MAX_ROW_BYTES, _MAX_CACHE_ROW_BYTES = 1 << 24, 1 << 22
 
 
 def _launch(fn, args, dev):
@@ -219,8 +219,8 @@ def attention_step(q, k_cache, v_cache, lengths, *, distance_slope=None, score_c
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
         raise ValueError(f"{name}: out must be contiguous and like q")
     for what, x in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if d > 1 and x.stride(3) != 1 or x.shape[1] > 1 and x.stride(1) * x.element_size() > _MAX_ROW_BYTES:
-            raise ValueError(f"{name}: {what}'s head dim must be contiguous and its rows at most {_MAX_ROW_BYTES} bytes apart (a cache is never copied)")
+        if d > 1 and x.stride(3) != 1 or x.shape[1] > 1 and x.stride(1) * x.element_size() > _MAX_CACHE_ROW_BYTES:
+            raise ValueError(f"{name}: {what}'s head dim must be contiguous and its rows at most {_MAX_CACHE_ROW_BYTES} bytes apart (a cache is never copied)")
     cap_rows = k_cache.shape[1]
     a = nat.SttranAttentionStep(_STEP_SIZE, _DTYPES[q.dtype], n, hq, hk, d, cap_rows, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
                                 q.stride(0), q.stride(1), k_cache.stride(0), k_cache.stride(1) if cap_rows > 1 else 0, k_cache.stride(2),
