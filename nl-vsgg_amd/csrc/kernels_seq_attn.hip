@@ -48,6 +48,28 @@ __device__ __forceinline__ void seq_attn_fwd_again(const SeqAttnArgs& A, const S
 // One pass over the keys with the running maximum m and sum l of the softmax (both fp32, base 2).  The accumulator is rescaled
 // only when the maximum grows by more than 8 (a factor of 256): p stays below 2^8 and the final division by l undoes any
 // common factor exactly as the textbook form does.
+// keys outside [lo, hi) of a block that starts at key kt
+template <class C>
+__device__ __forceinline__ void seq_hide(seq_f32x16 (&s)[C::NSUB], int kt, int lo, int hi, float with) {
+  const int k0 = kt + 4 * ((threadIdx.x >> 5) & 1);
+#pragma unroll
+  for (int u = 0; u < C::NSUB; ++u)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int key = k0 + 32 * u + 8 * (e >> 2) + (e & 3);
+      s[u][e] = key >= lo && key < hi ? s[u][e] : with;
+    }
+}
+template <class C>
+__device__ __forceinline__ float seq_block_max(const seq_f32x16 (&s)[C::NSUB]) {
+  float m = -INFINITY;
+#pragma unroll
+  for (int u = 0; u < C::NSUB; ++u)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) m = fmaxf(m, s[u][e]);
+  return m;
+}
+
 template <class C>
 struct SeqFwdLds {                                       // DS == 1: two tiles of keys and of values; else one of each and the exchange
   static constexpr int kBufs = C::DS == 1 ? 2 : 1;
@@ -101,7 +123,7 @@ seq_attn_fwd_kernel(SeqAttnArgs A) {
   seq_u32x4 own[C::NF];
   seq_own_load<C>(own, A.q + head * A.q_h, A.q_t, row0, A.tq, dh, dbytes);
   const SeqScore sc(A, head);
-  const bool capped = A.cap > 0.f;
+  const bool capped = A.cap > 0.f, linear = !capped && !A.slope && sc.mul > 0.f, bent = C::ES == 2 && capped && !A.slope;
   const int rlo = max(me.lo, beg), rhi = min(me.hi, end);           // this lane's visible keys of this workgroup
   seq_f32x16 acc[C::NB];
 #pragma unroll
@@ -146,30 +168,42 @@ seq_attn_fwd_kernel(SeqAttnArgs A) {
     }
     if (active) {
       const bool full = __all(rlo <= kt && rhi >= kt + C::BR);
-      float mt = -INFINITY;
+      // s becomes what z is linear in -- z = c1 * s + c0 -- so that one fma stands before the exponential:
+      //   plain: the products (scale > 0);  cap (bfloat16): r = 1 / (1 + e^(2 products)), z = cap - 2 cap r;  else: z itself
+      float mt, c1, c0;
+      if (linear) {
+        c1 = sc.mul; c0 = 0.f;
+        if (!full) seq_hide<C>(s, kt, rlo, rhi, -INFINITY);
+        mt = seq_block_max<C>(s) * c1;
+      } else if (bent) {
+        c1 = -2.f * sc.capl; c0 = sc.capl;
 #pragma unroll
-      for (int u = 0; u < C::NSUB; ++u) {
-        if (capped) {
+        for (int u = 0; u < C::NSUB; ++u)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) s[u][e] = sc.capl * seq_tanh<T>(s[u][e] * sc.mul);
-        } else {
+          for (int e = 0; e < 16; ++e)
+            s[u][e] = -__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[u][e] * (sc.mul * (2.f * kSeqLog2e))));
+        if (!full) seq_hide<C>(s, kt, rlo, rhi, -INFINITY);
+        c1 = -c1;
+        mt = fmaf(seq_block_max<C>(s), c1, c0);
+      } else {
+        c1 = 1.f; c0 = 0.f;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) s[u][e] *= sc.mul;
-        }
-        const int k0 = kt + 32 * u + 4 * h;
-        if (A.slope) {
+        for (int u = 0; u < C::NSUB; ++u) {
+          if (capped) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) s[u][e] = fmaf(-sc.slope, fabsf((float)(me.base - k0 - 8 * (e >> 2) - (e & 3))), s[u][e]);
-        }
-        if (!full) {
+            for (int e = 0; e < 16; ++e) s[u][e] = sc.capl * seq_tanh<T>(s[u][e] * sc.mul);
+          } else {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int key = k0 + 8 * (e >> 2) + (e & 3);
-            s[u][e] = key >= rlo && key < rhi ? s[u][e] : -INFINITY;
+            for (int e = 0; e < 16; ++e) s[u][e] *= sc.mul;
+          }
+          if (A.slope) {
+            const float at = (float)(me.base - kt - 32 * u - 4 * h);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[u][e] = fmaf(-sc.slope, fabsf(at - (float)(8 * (e >> 2) + (e & 3))), s[u][e]);
           }
         }
-#pragma unroll
-        for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[u][e]);
+        if (!full) seq_hide<C>(s, kt, rlo, rhi, -INFINITY);
+        mt = seq_block_max<C>(s);
       }
       mt = fmaxf(mt, __shfl_xor(mt, 32));
       if (__any(mt > m + 8.f || (m == -INFINITY && mt > -INFINITY))) {
@@ -181,12 +215,12 @@ seq_attn_fwd_kernel(SeqAttnArgs A) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) acc[nb][e] *= al;
       }
-      const float ms = m == -INFINITY ? 0.f : m;
+      c0 -= m == -INFINITY ? 0.f : m;
 #pragma unroll
       for (int u = 0; u < C::NSUB; ++u) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          s[u][e] = __builtin_amdgcn_exp2f(s[u][e] - ms);
+          s[u][e] = __builtin_amdgcn_exp2f(fmaf(s[u][e], c1, c0));
           l += s[u][e];
         }
         seq_reduce<C>(acc, vt_lds, u, dh, s[u]);

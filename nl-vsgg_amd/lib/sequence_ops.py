@@ -27,12 +27,13 @@ _MAX_ROW_BYTES, _MAX_CACHE_ROW_BYTES = 1 << 24, 1 << 22
 
 
 def _launch(fn, args, dev):
-    """`fn(args..., stream)` on the device's current stream; the entry points have no handle and so no device of their own."""
-    if torch.cuda.current_device() == dev.index:
-        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    """`fn(args..., stream)` on the device's current stream; the entry points have no handle and so no device of their own.  (The
+    stream's raw handle: building a torch.cuda.Stream costs 2 us of the 11 that a small call takes.)"""
+    if torch._C._cuda_getDevice() == dev.index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
     if rc != nat.STTRAN_OK:
         raise nat.SttranError(rc, f"{fn.__name__} failed")
 
@@ -64,6 +65,11 @@ def _small(name, what, x, dtype, shape, dev):
     if x.dtype != dtype or tuple(x.shape) != shape or x.device != dev:
         raise ValueError(f"{name}: {what} must be {dtype} {list(shape)} on {dev}, got {x.dtype} {list(x.shape)} on {x.device}")
     return x.contiguous()
+
+
+def _like(x):
+    """An uninitialised contiguous tensor of x's shape (half the time of torch.empty with its shape, dtype and device)."""
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
 def _ptr(x):
@@ -102,7 +108,7 @@ def _attention_struct(q, k, v, seq_off, key_off, prefix, slope, causal, cap, sca
 
 def _attention_forward(q, k, v, seq_off, key_off, prefix, slope, causal, cap, scale, train):
     lib = nat.load()
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out = _like(q)
     a = _attention_struct(q, k, v, seq_off, key_off, prefix, slope, causal, cap, scale)
     a.out = out.data_ptr()
     low = lse = None
@@ -133,7 +139,7 @@ class _PackedAttention(torch.autograd.Function):
         lib = nat.load()
         dout = _rows(dout)
         a = _attention_struct(q, k, v, seq_off, key_off, prefix, slope, *ctx.plain)
-        grads = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v)]
+        grads = [_like(x) for x in (q, k, v)]
         a.out, a.out_residual, a.lse = out.data_ptr(), _ptr(low), lse.data_ptr()
         a.dout, a.dout_row_stride, a.dout_head_stride = dout.data_ptr(), dout.stride(0) if dout.shape[0] > 1 else 0, dout.stride(1)
         a.dq, a.dk, a.dv = (g.data_ptr() for g in grads)
@@ -215,7 +221,7 @@ def attention_step(q, k_cache, v_cache, lengths, *, distance_slope=None, score_c
     scale, cap = _score(name, scale, score_cap, d)
     q = _rows(q, limit=False)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        out = _like(q)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
         raise ValueError(f"{name}: out must be contiguous and like q")
     for what, x in (("k_cache", k_cache), ("v_cache", v_cache)):
@@ -295,7 +301,7 @@ class _RotaryQK(torch.autograd.Function):
         lib, dev = nat.load(), q.device
         dyq, dyk = _rows(dyq, limit=False), _rows(dyk, limit=False)
         a = _rotary_struct(q, k, positions, freq, wq, wk, *ctx.plain)
-        dq, dk = torch.empty(q.shape, dtype=q.dtype, device=dev), torch.empty(k.shape, dtype=k.dtype, device=dev)
+        dq, dk = _like(q), _like(k)
         a.dq_out, a.dk_out, a.dq, a.dk = dyq.data_ptr(), dyk.data_ptr(), dq.data_ptr(), dk.data_ptr()
         a.dq_row_stride, a.dq_head_stride, a.dk_row_stride, a.dk_head_stride = dyq.stride(0), dyq.stride(1), dyk.stride(0), dyk.stride(1)
         dwq = dwk = None
@@ -348,7 +354,7 @@ def rotary_qk(q, k, positions, frequencies, q_weight=None, k_weight=None, *, eps
 
 
 def _dropout(x, residual, p, rng_state, key, offset, used):
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _like(x)
     _launch(nat.load().sttran_dropout_add, (x.data_ptr(), _ptr(residual), y.data_ptr(), x.numel(), _DTYPES[x.dtype], p, _ptr(rng_state), key,
                                             offset, _ptr(used)), x.device)
     return y
