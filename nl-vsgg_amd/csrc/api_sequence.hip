@@ -31,6 +31,8 @@ struct Alignment {
 bool row_stride_ok(int64_t s, int es, int64_t most = kMaxRowBytes) { return s >= 0 && s <= most && s * es <= most; }
 bool head_stride_ok(int64_t s) { return s >= 0 && s < (int64_t(1) << 40); }
 
+bool workspace_ok(const void* p, int64_t have, int64_t need) { return p && have >= need && !(reinterpret_cast<uintptr_t>(p) & 15); }
+
 hipStream_t str(void* s) { return reinterpret_cast<hipStream_t>(s); }
 int code(hipError_t e) { return e == hipSuccess ? STTRAN_OK : STTRAN_ERR_HIP; }
 
@@ -51,6 +53,7 @@ bool attention_args(const SttranAttention* a, SeqAttnArgs& A, Alignment& al) {
   A.q_t = a->q_row_stride * es; A.q_h = a->q_head_stride * es;
   A.k_t = a->k_row_stride * es; A.k_h = a->k_head_stride * es;
   A.v_t = a->v_row_stride * es; A.v_h = a->v_head_stride * es;
+  A.raw[0] = {A.q, A.q_t, A.q_h}; A.raw[1] = {A.k, A.k_t, A.k_h}; A.raw[2] = {A.v, A.v_t, A.v_h};
   A.out = (char*)a->out; A.out_lo = a->dtype == STTRAN_DTYPE_BF16 ? (char*)a->out_residual : nullptr; A.lse = a->lse;
   A.off_q = a->seq_off; A.off_k = a->key_off; A.prefix = a->prefix_len; A.slope = a->distance_slope;
   A.nseq = a->num_seq; A.tq = (int)a->q_rows; A.tk = (int)a->kv_rows;
@@ -59,16 +62,6 @@ bool attention_args(const SttranAttention* a, SeqAttnArgs& A, Alignment& al) {
   al.at(a->q); al.at(a->k); al.at(a->v); al.at(a->out); al.at(A.out_lo);
   al.step(A.q_t); al.step(A.q_h); al.step(A.k_t); al.step(A.k_h); al.step(A.v_t); al.step(A.v_h); al.step((int64_t)A.d * es);
   return true;
-}
-
-int64_t attention_workspace(const SeqAttnArgs& A, int bf16, bool backward) {
-  if (backward) {
-    const int64_t rows = ((int64_t)A.hq * A.tq * 4 + (int64_t)A.tq * 16 + 16 + 255) / 256 * 256;      // ranges, delta
-    const int parts = seq_attn_dkv_splits(bf16, A);
-    return rows + (parts > 1 ? (int64_t)parts * 2 * A.tk * A.hk * A.d * 4 : 0);
-  }
-  const int splits = seq_attn_splits(bf16, A);
-  return splits > 1 ? (int64_t)splits * A.hq * A.tq * (A.d + 2) * 4 : 0;
 }
 
 bool step_args(const SttranAttentionStep* a, SeqStepArgs& A) {
@@ -144,7 +137,7 @@ extern "C" {
 int64_t sttran_attention_workspace_bytes(const SttranAttention* args, int32_t backward) {
   SeqAttnArgs A{};
   Alignment al;
-  return attention_args(args, A, al) ? attention_workspace(A, args->dtype == STTRAN_DTYPE_BF16, backward != 0) : 0;
+  return attention_args(args, A, al) ? seq_attn_plan(args->dtype == STTRAN_DTYPE_BF16, A, backward != 0).bytes : 0;
 }
 
 int sttran_attention_forward(const SttranAttention* args, void* stream) {
@@ -154,13 +147,9 @@ int sttran_attention_forward(const SttranAttention* args, void* stream) {
   const int bf16 = args->dtype == STTRAN_DTYPE_BF16;
   A.aln = al.value(elt(args->dtype));
   if (!A.aln) return STTRAN_ERR_INVALID;
-  const int64_t need = attention_workspace(A, bf16, false);
-  if (need > 0) {
-    if (!args->workspace || args->workspace_bytes < need || (reinterpret_cast<uintptr_t>(args->workspace) & 15)) return STTRAN_ERR_INVALID;
-    A.splits = seq_attn_splits(bf16, A);
-    A.part = (float*)args->workspace;
-  }
-  return code(launch_seq_attn_forward(str(stream), bf16, A));
+  const SeqAttnPlan plan = seq_attn_plan(bf16, A, false);
+  if (plan.bytes > 0 && !workspace_ok(args->workspace, args->workspace_bytes, plan.bytes)) return STTRAN_ERR_INVALID;
+  return code(launch_seq_attn_forward(str(stream), bf16, A, plan, (char*)args->workspace));
 }
 
 int sttran_attention_backward(const SttranAttention* args, void* stream) {
@@ -171,19 +160,16 @@ int sttran_attention_backward(const SttranAttention* args, void* stream) {
   if (args->q_rows > 0 && (!args->out || !args->lse || !args->dout || !args->dq)) return STTRAN_ERR_INVALID;
   if (args->kv_rows > 0 && (!args->dk || !args->dv)) return STTRAN_ERR_INVALID;
   if (!row_stride_ok(args->dout_row_stride, es) || !head_stride_ok(args->dout_head_stride)) return STTRAN_ERR_INVALID;
-  const int64_t need = attention_workspace(A, bf16, true);
-  if (!args->workspace || args->workspace_bytes < need || (reinterpret_cast<uintptr_t>(args->workspace) & 15)) return STTRAN_ERR_INVALID;
+  const SeqAttnPlan plan = seq_attn_plan(bf16, A, true);
+  if (plan.bytes > 0 && !workspace_ok(args->workspace, args->workspace_bytes, plan.bytes)) return STTRAN_ERR_INVALID;
   A.dout = (const char*)args->dout;
   A.do_t = args->dout_row_stride * es; A.do_h = args->dout_head_stride * es;
+  A.raw[3] = {A.dout, A.do_t, A.do_h};
   A.dq = (char*)args->dq; A.dk = (char*)args->dk; A.dv = (char*)args->dv;
   al.at(A.dout); al.at(A.dq); al.at(A.dk); al.at(A.dv); al.step(A.do_t); al.step(A.do_h);
   A.aln = al.value(es);
   if (!A.aln) return STTRAN_ERR_INVALID;
-  A.rows = (int4*)args->workspace;
-  A.delta = (float*)((char*)args->workspace + (int64_t)A.tq * 16);
-  A.splits = seq_attn_dkv_splits(bf16, A);
-  A.part = (float*)((char*)args->workspace + ((int64_t)A.hq * A.tq * 4 + (int64_t)A.tq * 16 + 16 + 255) / 256 * 256);
-  return code(launch_seq_attn_backward(str(stream), bf16, A));
+  return code(launch_seq_attn_backward(str(stream), bf16, A, plan, (char*)args->workspace));
 }
 
 int64_t sttran_attention_step_workspace_bytes(const SttranAttentionStep* args) {
@@ -201,7 +187,7 @@ int sttran_attention_step(const SttranAttentionStep* args, void* stream) {
   A.aln = al.value(elt(args->dtype));
   if (!A.aln) return STTRAN_ERR_INVALID;
   const int64_t need = step_workspace(A);
-  if (need > 0 && (!args->workspace || args->workspace_bytes < need || (reinterpret_cast<uintptr_t>(args->workspace) & 15))) return STTRAN_ERR_INVALID;
+  if (need > 0 && !workspace_ok(args->workspace, args->workspace_bytes, need)) return STTRAN_ERR_INVALID;
   A.part = (float*)args->workspace;
   return code(launch_seq_step(str(stream), args->dtype == STTRAN_DTYPE_BF16, A));
 }
@@ -229,7 +215,7 @@ int sttran_rotary_backward(const SttranRotary* args, void* stream) {
   A.aln = al.value(elt(args->dtype));
   if (!A.aln) return STTRAN_ERR_INVALID;
   if (A.dw[0] || A.dw[1]) {
-    if (!args->workspace || args->workspace_bytes < rotary_workspace(A) || (reinterpret_cast<uintptr_t>(args->workspace) & 15)) return STTRAN_ERR_INVALID;
+    if (!workspace_ok(args->workspace, args->workspace_bytes, rotary_workspace(A))) return STTRAN_ERR_INVALID;
     A.part = (float*)args->workspace;
   }
   return code(launch_seq_rotary_backward(str(stream), args->dtype == STTRAN_DTYPE_BF16, A));

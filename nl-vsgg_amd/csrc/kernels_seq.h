@@ -6,12 +6,20 @@
 namespace sttran {
 
 // ---- attention over packed sequences
-hipError_t launch_seq_attn_forward(hipStream_t s, int bf16, const SeqAttnArgs& A);
-hipError_t launch_seq_attn_backward(hipStream_t s, int bf16, const SeqAttnArgs& A);
-// how many shares of the keys a forward launch is split into (1: none), from what the host knows
-int seq_attn_splits(int bf16, const SeqAttnArgs& A);
-// ... and a backward launch's work on a key tile
-int seq_attn_dkv_splits(int bf16, const SeqAttnArgs& A);
+// How a call is run, from what the host knows, and where things lie in its workspace (byte offsets)
+struct SeqAttnPlan {
+  bool planes;               // fp32 as three bfloat16 planes
+  int splits;                // shares of the keys (forward) or of a key tile's work (backward); 1: none
+  int64_t rows, delta, part, plane[4], bytes;
+};
+SeqAttnPlan seq_attn_plan(int bf16, const SeqAttnArgs& A, bool backward);
+hipError_t launch_seq_attn_forward(hipStream_t s, int bf16, const SeqAttnArgs& A, const SeqAttnPlan& P, char* workspace);
+hipError_t launch_seq_attn_backward(hipStream_t s, int bf16, const SeqAttnArgs& A, const SeqAttnPlan& P, char* workspace);
+// their parts: the launches themselves, planes already made; own rows of a forward / key tile workgroup
+hipError_t launch_seq_attn_fwd(hipStream_t s, int bf16, bool planes, const SeqAttnArgs& A);
+hipError_t launch_seq_attn_bwd(hipStream_t s, int bf16, bool planes, const SeqAttnArgs& A);
+int seq_attn_fwd_tile(int bf16, bool planes, int d);
+int seq_attn_dkv_tile(int bf16, bool planes, int d);
 // joins partial outputs [split][head][row][d] + [split][head][row][2].  lens (device, per row) and chunk: only the shares that a
 // row's length fills were written (lens == nullptr: all of them)
 hipError_t launch_seq_attn_join(hipStream_t s, int bf16, const SeqAttnArgs& A, const int* lens, int chunk, int capacity);

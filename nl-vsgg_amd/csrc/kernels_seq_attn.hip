@@ -17,12 +17,12 @@ __device__ __forceinline__ void seq_attn_fwd_again(const SeqAttnArgs& A, const S
     const int row = row0 + n;
     if (!(rows >> n & 1) || row >= A.tq || n % C::DS != dh) continue;
     const int lo = max(__shfl(me.lo, n), beg), hi = min(__shfl(me.hi, n), end), base = __shfl(me.base, n);
-    const SeqSpread q = seq_spread<T>(A.q + head * A.q_h + (int64_t)row * A.q_t, A.d);
+    const SeqSpread q = seq_spread<T>(A.raw[0].p + head * A.raw[0].h + (int64_t)row * A.raw[0].t, A.d);
     float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f}, unused;
 #pragma unroll 1
     for (int key = lo; key < hi; ++key) {
-      const SeqSpread k = seq_spread<T>(A.k + kvh * A.k_h + (int64_t)key * A.k_t, A.d);
-      const SeqSpread v = seq_spread<T>(A.v + kvh * A.v_h + (int64_t)key * A.v_t, A.d);
+      const SeqSpread k = seq_spread<T>(A.raw[1].p + kvh * A.raw[1].h + (int64_t)key * A.raw[1].t, A.d);
+      const SeqSpread v = seq_spread<T>(A.raw[2].p + kvh * A.raw[2].h + (int64_t)key * A.raw[2].t, A.d);
       const float z = seq_z<T>(A, sc, seq_spread_dot(q, k), base, key, unused);
       const float mn = fmaxf(m, z), ms = mn == -INFINITY ? 0.f : mn, al = __builtin_amdgcn_exp2f(m - ms), p = __builtin_amdgcn_exp2f(z - ms);
       l = fmaf(l, al, p);
@@ -39,7 +39,7 @@ __device__ __forceinline__ void seq_attn_fwd_again(const SeqAttnArgs& A, const S
       if (lane == 0) { ps[0] = m; ps[1] = l; }
       continue;
     }
-    const int64_t at = ((int64_t)row * A.hq + head) * A.d * C::ES;
+    const int64_t at = ((int64_t)row * A.hq + head) * A.d * C::OS;
     seq_spread_store<T>(A.out + at, A.out_lo ? A.out_lo + at : nullptr, o, l == 0.f ? 0.f : 1.f / l, A.d);
     if (A.lse && lane == 0) A.lse[(int64_t)head * A.tq + row] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
   }
@@ -48,50 +48,69 @@ __device__ __forceinline__ void seq_attn_fwd_again(const SeqAttnArgs& A, const S
 // One pass over the keys with the running maximum m and sum l of the softmax (both fp32, base 2).  The accumulator is rescaled
 // only when the maximum grows by more than 8 (a factor of 256): p stays below 2^8 and the final division by l undoes any
 // common factor exactly as the textbook form does.
-// keys outside [lo, hi) of a block that starts at key kt
-template <class C>
-__device__ __forceinline__ void seq_hide(seq_f32x16 (&s)[C::NSUB], int kt, int lo, int hi, float with) {
-  const int k0 = kt + 4 * ((threadIdx.x >> 5) & 1);
+// N scores of one row, x[i] of key k0 + 8 (i / 4) + i % 4, become what z is linear in -- z = c1 * x + c0 -- so that one fma stands
+// before the exponential; hidden ones become -inf (c1 > 0); returns the largest z.
+//   plain: the products (scale > 0);  cap (bfloat16): -1 / (1 + e^(2 products)), z = cap - 2 cap / (1 + ..);  else: z itself
+template <class C, int N>
+__device__ __forceinline__ float seq_bend(const SeqAttnArgs& A, const SeqScore& sc, float (&x)[N], int k0, int base, bool full, int lo, int hi,
+                                          float& c1, float& c0) {
+  using T = typename C::E;
+  if (A.cap <= 0.f && !A.slope && sc.mul > 0.f) {
+    c1 = sc.mul; c0 = 0.f;
+  } else if (C::OS == 2 && A.cap > 0.f && !A.slope) {
+    c1 = 2.f * sc.capl; c0 = sc.capl;
 #pragma unroll
-  for (int u = 0; u < C::NSUB; ++u)
+    for (int i = 0; i < N; ++i) x[i] = -__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x[i] * (sc.mul * (2.f * kSeqLog2e))));
+  } else {
+    c1 = 1.f; c0 = 0.f;
+    if (A.cap > 0.f) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int key = k0 + 32 * u + 8 * (e >> 2) + (e & 3);
-      s[u][e] = key >= lo && key < hi ? s[u][e] : with;
+      for (int i = 0; i < N; ++i) x[i] = sc.capl * seq_tanh<T>(x[i] * sc.mul);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] *= sc.mul;
     }
-}
-template <class C>
-__device__ __forceinline__ float seq_block_max(const seq_f32x16 (&s)[C::NSUB]) {
+    if (A.slope) {
+      const float at = (float)(base - k0);
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = fmaf(-sc.slope, fabsf(at - (float)(8 * (i >> 2) + (i & 3))), x[i]);
+    }
+  }
+  if (!full) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int key = k0 + 8 * (i >> 2) + (i & 3);
+      x[i] = key >= lo && key < hi ? x[i] : -INFINITY;
+    }
+  }
   float m = -INFINITY;
 #pragma unroll
-  for (int u = 0; u < C::NSUB; ++u)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) m = fmaxf(m, s[u][e]);
-  return m;
+  for (int i = 0; i < N; ++i) m = fmaxf(m, x[i]);
+  return fmaf(m, c1, c0);
 }
 
 template <class C>
 struct SeqFwdLds {                                       // DS == 1: two tiles of keys and of values; else one of each and the exchange
   static constexpr int kBufs = C::DS == 1 ? 2 : 1;
-  // the workgroup's small notes before and after the loop lie where the exchange is during it: at DP = 256 in fp32 a workgroup then
-  // takes exactly half of a CU's 160 KB
-  static constexpr int kXch = 2 * kBufs * C::kTileBytes, kRed = kXch;
-  static constexpr int kBytes = kXch + (C::DS > 1 ? C::NW * 4096 : C::NW * 8);
+  // the workgroup's small notes before and after the loop lie where the exchange is during it: at DP = 256 in fp32 two workgroups
+  // then share a CU's 160 KB
+  static constexpr int kXch = 2 * kBufs * C::kTileBytes, kRed = kXch, kRefs = kXch + (C::DS > 1 ? C::NW * SeqShare<C, 1>::kWave : 0);
+  static constexpr int kBytes = C::DS > 1 ? kRefs + C::NW * 128 : kXch + C::NW * 8;
 };
 template <class C>
 __global__ void __launch_bounds__(C::NT) __attribute__((amdgpu_waves_per_eu(2, 2)))
 seq_attn_fwd_kernel(SeqAttnArgs A) {
-  using T = typename C::E;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   char* xch = smem + SeqFwdLds<C>::kXch;
   int* red = reinterpret_cast<int*>(smem + SeqFwdLds<C>::kRed);
+  float* refs = reinterpret_cast<float*>(smem + SeqFwdLds<C>::kRefs);
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int tiles = (A.tq + C::RB - 1) / C::RB;
   const int id = seq_xcd_order(blockIdx.x, gridDim.x);
   const int head = id / tiles, tile = tiles - 1 - id % tiles;      // rows that see most keys first where the order masks
   const int kvh = head / (A.hq / A.hk), dh = w % C::DS;
   const int row0 = tile * C::RB + 32 * (w / C::DS), row = row0 + (lane & 31);
-  const int dbytes = A.d * C::ES;
+  const int dbytes = C::row_bytes(A.d);
 
   const SeqRow me = seq_row(A, row);
   int lo = me.hi > me.lo ? me.lo : INT_MAX, hi = me.hi;
@@ -120,10 +139,9 @@ seq_attn_fwd_kernel(SeqAttnArgs A) {
     seq_tile_move<C>(mk, kt_lds, kp, A.k_t, beg, end, dbytes);
     seq_tile_move<C>(mv, vt_lds, vp, A.v_t, beg, end, dbytes);
   }
-  seq_u32x4 own[C::NF];
+  seq_u32x4 own[C::PL * C::NF];
   seq_own_load<C>(own, A.q + head * A.q_h, A.q_t, row0, A.tq, dh, dbytes);
   const SeqScore sc(A, head);
-  const bool capped = A.cap > 0.f, linear = !capped && !A.slope && sc.mul > 0.f, bent = C::ES == 2 && capped && !A.slope;
   const int rlo = max(me.lo, beg), rhi = min(me.hi, end);           // this lane's visible keys of this workgroup
   seq_f32x16 acc[C::NB];
 #pragma unroll
@@ -155,75 +173,102 @@ seq_attn_fwd_kernel(SeqAttnArgs A) {
         seq_scores<C>(s[u], kt_lds, u, dh, own);
       }
     }
-    if constexpr (C::DS > 1) {
+    const bool full = __all(rlo <= kt && rhi >= kt + C::BR);
+    float c1, c0;
+    if constexpr (C::DS == 1) {
+      if (active) {
+        float x[16 * C::NSUB];
+#pragma unroll
+        for (int i = 0; i < 16 * C::NSUB; ++i) x[i] = s[i >> 4][i & 15];
+        float mt = seq_bend<C>(A, sc, x, kt + 4 * h, me.base, full, rlo, rhi, c1, c0);
+        mt = fmaxf(mt, __shfl_xor(mt, 32));
+        if (__any(mt > m + 8.f || (m == -INFINITY && mt > -INFINITY))) {
+          const float mn = fmaxf(m, mt);
+          const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+          m = mn; l *= al;
+#pragma unroll
+          for (int nb = 0; nb < C::NB; ++nb)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[nb][e] *= al;
+        }
+        c0 -= m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int u = 0; u < C::NSUB; ++u) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            s[u][e] = __builtin_amdgcn_exp2f(fmaf(x[16 * u + e], c1, c0));
+            l += s[u][e];
+          }
+          seq_reduce<C>(acc, vt_lds, u, dh, s[u]);
+        }
+      }
+    } else {
+      // Each wave of the team adds up and exponentiates its share of the block's quads, against the team's maximum so far, or its own
+      // where that is 2^30 behind; it tells the others which.  So one barrier brings probabilities, and the rare change of the
+      // maximum is made afterwards by factors.
       static_assert(C::NSUB == 1, "one block is exchanged");
-      if (active) SeqShare<C, 1>::put(s[0], xch, w, 0);
+      using S = SeqShare<C, 1>;
+      const int first = w - dh;
+      if (active) S::put(s[0], xch, first, dh, 0);
       seq_tile_done<C>(mv, vt_lds, dbytes);
       __syncthreads();                                               // keys are free, values and partial scores are there
       if (more) seq_tile_move<C>(mk, kn, kp, A.k_t, kt + C::BR, end, dbytes);
+      float part = 0.f;
       if (active) {
+        float x[4 * S::GP];
 #pragma unroll
-        for (int g = 0; g < 4; ++g) seq_set_quad(s[0], g, SeqShare<C, 1>::sum(xch, w - dh, 0, g));
-      }
-    }
-    if (active) {
-      const bool full = __all(rlo <= kt && rhi >= kt + C::BR);
-      // s becomes what z is linear in -- z = c1 * s + c0 -- so that one fma stands before the exponential:
-      //   plain: the products (scale > 0);  cap (bfloat16): r = 1 / (1 + e^(2 products)), z = cap - 2 cap r;  else: z itself
-      float mt, c1, c0;
-      if (linear) {
-        c1 = sc.mul; c0 = 0.f;
-        if (!full) seq_hide<C>(s, kt, rlo, rhi, -INFINITY);
-        mt = seq_block_max<C>(s) * c1;
-      } else if (bent) {
-        c1 = -2.f * sc.capl; c0 = sc.capl;
+        for (int i = 0; i < S::GP; ++i) {
+          const seq_f32x4 q = S::sum(s[0], xch, first, dh, 0, i);
 #pragma unroll
-        for (int u = 0; u < C::NSUB; ++u)
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            s[u][e] = -__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[u][e] * (sc.mul * (2.f * kSeqLog2e))));
-        if (!full) seq_hide<C>(s, kt, rlo, rhi, -INFINITY);
-        c1 = -c1;
-        mt = fmaf(seq_block_max<C>(s), c1, c0);
-      } else {
-        c1 = 1.f; c0 = 0.f;
-#pragma unroll
-        for (int u = 0; u < C::NSUB; ++u) {
-          if (capped) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) s[u][e] = sc.capl * seq_tanh<T>(s[u][e] * sc.mul);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) s[u][e] *= sc.mul;
-          }
-          if (A.slope) {
-            const float at = (float)(me.base - kt - 32 * u - 4 * h);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) s[u][e] = fmaf(-sc.slope, fabsf(at - (float)(8 * (e >> 2) + (e & 3))), s[u][e]);
-          }
+          for (int e = 0; e < 4; ++e) x[4 * i + e] = q[e];
         }
-        if (!full) seq_hide<C>(s, kt, rlo, rhi, -INFINITY);
-        mt = seq_block_max<C>(s);
-      }
-      mt = fmaxf(mt, __shfl_xor(mt, 32));
-      if (__any(mt > m + 8.f || (m == -INFINITY && mt > -INFINITY))) {
-        const float mn = fmaxf(m, mt);
-        const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-        m = mn; l *= al;
+        float mt = seq_bend<C>(A, sc, x, kt + 8 * dh * S::GP + 4 * h, me.base, full, rlo, rhi, c1, c0);
+        mt = fmaxf(mt, __shfl_xor(mt, 32));
+        const float ref = mt > m + 30.f ? mt : m;
+        c0 -= ref == -INFINITY ? 0.f : ref;
 #pragma unroll
-        for (int nb = 0; nb < C::NB; ++nb)
+        for (int i = 0; i < S::GP; ++i) {
+          seq_f32x4 p;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) acc[nb][e] *= al;
-      }
-      c0 -= m == -INFINITY ? 0.f : m;
-#pragma unroll
-      for (int u = 0; u < C::NSUB; ++u) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          s[u][e] = __builtin_amdgcn_exp2f(fmaf(s[u][e], c1, c0));
-          l += s[u][e];
+          for (int e = 0; e < 4; ++e) {
+            p[e] = __builtin_amdgcn_exp2f(fmaf(x[4 * i + e], c1, c0));
+            part += p[e];
+          }
+          S::leave(p, xch, first, dh, 0, i);
         }
-        seq_reduce<C>(acc, vt_lds, u, dh, s[u]);
+        if (h == 0) refs[w * 32 + lane] = ref;
+      }
+      __syncthreads();
+      if (active) {
+        float r[C::DS], mn = -INFINITY, own = 0.f;
+#pragma unroll
+        for (int j = 0; j < C::DS; ++j) {
+          r[j] = refs[(first + j) * 32 + (lane & 31)];
+          mn = fmaxf(mn, r[j]);
+          own = j == dh ? r[j] : own;
+        }
+        bool same = mn == m;
+#pragma unroll
+        for (int j = 0; j < C::DS; ++j) same = same && r[j] == mn;
+        S::take(s[0], xch, first, 0);
+        if (!__all(same)) {
+          const float al = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+          l *= al;
+#pragma unroll
+          for (int nb = 0; nb < C::NB; ++nb)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[nb][e] *= al;
+          m = mn;
+#pragma unroll
+          for (int j = 0; j < C::DS; ++j) {
+            const float f = r[j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(r[j] - mn);
+#pragma unroll
+            for (int e = 4 * j * S::GP; e < 4 * (j + 1) * S::GP; ++e) s[0][e] *= f;
+          }
+          part *= own == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(own - mn);
+        }
+        l += part;
+        seq_reduce<C>(acc, vt_lds, 0, dh, s[0]);
       }
     }
     if (more) {
@@ -238,8 +283,15 @@ seq_attn_fwd_kernel(SeqAttnArgs A) {
       if (more) seq_tile_move<C>(mv, vt_lds, vp, A.v_t, kt + C::BR, end, dbytes);
     }
   }
-  const uint32_t bad = seq_bad_rows<C>(acc, 0, red);
   l += __shfl_xor(l, 32);
+  if constexpr (C::DS > 1) {                           // the team's shares of the sum
+    if (h == 0) refs[w * 32 + lane] = l;
+    __syncthreads();
+    l = refs[(w - dh) * 32 + (lane & 31)];
+#pragma unroll
+    for (int j = 1; j < C::DS; ++j) l += refs[(w - dh + j) * 32 + (lane & 31)];
+  }
+  const uint32_t bad = seq_bad_rows<C>(acc, 0, red);
   if (bad) seq_attn_fwd_again<C>(A, sc, bad, me, row0, head, beg, end, dh);
   if (row >= A.tq || (bad >> (lane & 31) & 1)) return;
   if (A.splits > 1) {
@@ -260,7 +312,7 @@ seq_attn_fwd_kernel(SeqAttnArgs A) {
     return;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  const int64_t at = ((int64_t)row * A.hq + head) * dbytes;
+  const int64_t at = ((int64_t)row * A.hq + head) * A.d * C::OS;
   seq_store_own<C>(acc, inv, A.out + at, A.out_lo ? A.out_lo + at : nullptr, dh, A.d, A.aln);
   if (A.lse && dh == 0 && h == 0) A.lse[(int64_t)head * A.tq + row] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
@@ -330,11 +382,6 @@ hipError_t launch_seq_attn_join(hipStream_t s, int bf16, const SeqAttnArgs& A, c
   return hipGetLastError();
 }
 
-int seq_attn_splits(int bf16, const SeqAttnArgs& A) {
-  (void)bf16; (void)A;
-  return 1;
-}
-
 template <class C>
 static hipError_t fwd(hipStream_t s, const SeqAttnArgs& A) {
   constexpr int lds = SeqFwdLds<C>::kBytes;
@@ -346,21 +393,31 @@ static hipError_t fwd(hipStream_t s, const SeqAttnArgs& A) {
   const int tiles = (A.tq + C::RB - 1) / C::RB;
   fn<<<dim3((unsigned)(tiles * A.hq), (unsigned)A.splits), C::NT, lds, s>>>(A);
   e = hipGetLastError();
-  return e != hipSuccess || A.splits == 1 ? e : launch_seq_attn_join(s, C::ES == 2, A, nullptr, 0, 0);
+  return e != hipSuccess || A.splits == 1 ? e : launch_seq_attn_join(s, C::OS == 2, A, nullptr, 0, 0);
 }
 
+// Own rows a workgroup: 128 where a wave holds whole heads; 32 or 64 where teams of waves share them
 template <class T, bool VEC>
 static hipError_t pick(hipStream_t s, const SeqAttnArgs& A) {
   if (A.d <= 64) return fwd<SeqTile<T, 64, 1, 4, 64, VEC>>(s, A);
   if (A.d <= 128) return fwd<SeqTile<T, 128, 1, 4, sizeof(T) == 2 ? 64 : 32, VEC>>(s, A);
   return fwd<SeqTile<T, 256, sizeof(T) == 2 ? 2 : 4, 4, 32, VEC>>(s, A);
 }
+static hipError_t pick_planes(hipStream_t s, const SeqAttnArgs& A) {
+  if (A.d <= 64) return fwd<SeqTile<float, 64, 1, 4, 32, true, 3>>(s, A);
+  if (A.d <= 128) return fwd<SeqTile<float, 128, 2, 4, 32, true, 3>>(s, A);
+  return fwd<SeqTile<float, 256, 4, 8, 32, true, 3>>(s, A);
+}
+int seq_attn_fwd_tile(int bf16, bool planes, int d) {
+  if (planes) return d <= 64 ? 128 : 64;
+  return d <= 128 ? 128 : bf16 ? 64 : 32;
+}
 
-hipError_t launch_seq_attn_forward(hipStream_t s, int bf16, const SeqAttnArgs& A) {
-  if (A.tq == 0) return hipSuccess;
+hipError_t launch_seq_attn_fwd(hipStream_t s, int bf16, bool planes, const SeqAttnArgs& A) {
   const bool vec = A.aln >= 4;
+  if (planes) return pick_planes(s, A);
   if (bf16) return vec ? pick<__bf16, true>(s, A) : pick<__bf16, false>(s, A);
-  return vec ? pick<float, true>(s, A) : pick<float, false>(s, A);
+  return pick<float, true>(s, A);                       // 4-byte elements are 4-byte aligned
 }
 
 }  // namespace sttran

@@ -21,7 +21,7 @@ __global__ void __launch_bounds__(256) seq_attn_delta_kernel(SeqAttnArgs A) {
   const int c = threadIdx.x % LPR;
   if (item >= (int64_t)A.tq * A.hq) return;
   const int row = (int)(item / A.hq), head = (int)(item % A.hq), dbytes = A.d * (int)sizeof(T);
-  const seq_u32x4 g = seq_row_chunk(A.dout + row * A.do_t + head * A.do_h, c, dbytes, A.aln);
+  const seq_u32x4 g = seq_row_chunk(A.raw[3].p + row * A.raw[3].t + head * A.raw[3].h, c, dbytes, A.aln);
   const seq_u32x4 o = seq_row_chunk(A.out + item * dbytes, c, dbytes, A.aln);
   seq_u32x4 r = {0, 0, 0, 0};
   if (A.out_lo) r = seq_row_chunk(A.out_lo + item * dbytes, c, dbytes, A.aln);
@@ -89,20 +89,20 @@ __device__ __forceinline__ void seq_attn_dq_again(const SeqAttnArgs& A, const Se
     const int row = row0 + n;
     if (!(rows >> n & 1) || row >= A.tq || n % C::DS != dh) continue;
     const int lo = __shfl(me.lo, n), hi = __shfl(me.hi, n), base = __shfl(me.base, n);
-    const SeqSpread q = seq_spread<T>(A.q + head * A.q_h + (int64_t)row * A.q_t, A.d);
-    const SeqSpread g = seq_spread<T>(A.dout + head * A.do_h + (int64_t)row * A.do_t, A.d);
+    const SeqSpread q = seq_spread<T>(A.raw[0].p + head * A.raw[0].h + (int64_t)row * A.raw[0].t, A.d);
+    const SeqSpread g = seq_spread<T>(A.raw[3].p + head * A.raw[3].h + (int64_t)row * A.raw[3].t, A.d);
     const float lse = A.lse[(int64_t)head * A.tq + row], delta = A.delta[(int64_t)head * A.tq + row];
     float o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
     for (int key = lo; key < hi; ++key) {
-      const SeqSpread k = seq_spread<T>(A.k + kvh * A.k_h + (int64_t)key * A.k_t, A.d);
-      const SeqSpread v = seq_spread<T>(A.v + kvh * A.v_h + (int64_t)key * A.v_t, A.d);
+      const SeqSpread k = seq_spread<T>(A.raw[1].p + kvh * A.raw[1].h + (int64_t)key * A.raw[1].t, A.d);
+      const SeqSpread v = seq_spread<T>(A.raw[2].p + kvh * A.raw[2].h + (int64_t)key * A.raw[2].t, A.d);
       float s = seq_spread_dot(q, k), dp = seq_spread_dot(g, v);
       seq_pair_any<T>(A, sc, s, dp, true, lse, delta, base - key);
 #pragma unroll
       for (int u = 0; u < 4; ++u) o[u] = fmaf(dp, k.x[u], o[u]);
     }
-    seq_spread_store<T>(A.dq + ((int64_t)row * A.hq + head) * A.d * C::ES, nullptr, o, A.scale, A.d);
+    seq_spread_store<T>(A.dq + ((int64_t)row * A.hq + head) * A.d * C::OS, nullptr, o, A.scale, A.d);
   }
 }
 
@@ -128,7 +128,7 @@ seq_attn_dq_kernel(SeqAttnArgs A) {
   const int head = id / tiles, tile = tiles - 1 - id % tiles;
   const int kvh = head / (A.hq / A.hk), dh = w % C::DS;
   const int row0 = tile * C::RB + 32 * (w / C::DS), row = row0 + (lane & 31);
-  const int dbytes = A.d * C::ES;
+  const int dbytes = C::row_bytes(A.d);
 
   SeqRow me{0, 0, 0};
   float lse = INFINITY, delta = 0.f;
@@ -159,7 +159,7 @@ seq_attn_dq_kernel(SeqAttnArgs A) {
     seq_tile_move<C>(mk, kt_lds, kp, A.k_t, beg, end, dbytes);
     seq_tile_move<C>(mv, vt_lds, vp, A.v_t, beg, end, dbytes);
   }
-  seq_u32x4 oq[C::NF], og[C::NF];
+  seq_u32x4 oq[C::PL * C::NF], og[C::PL * C::NF];
   seq_own_load<C>(oq, A.q + head * A.q_h, A.q_t, row0, A.tq, dh, dbytes);
   seq_own_load<C>(og, A.dout + head * A.do_h, A.do_t, row0, A.tq, dh, dbytes);
   const SeqScore sc(A, head);
@@ -205,8 +205,8 @@ seq_attn_dq_kernel(SeqAttnArgs A) {
       if constexpr (C::DS > 1) {
         static_assert(C::NSUB == 1, "one pair of blocks is exchanged");
         if (active) {
-          SeqShare<C, 2>::put(s, xch, w, 0);
-          SeqShare<C, 2>::put(dp, xch, w, 1);
+          SeqShare<C, 2>::put(s, xch, w - dh, dh, 0);
+          SeqShare<C, 2>::put(dp, xch, w - dh, dh, 1);
         }
         __syncthreads();                             // the values' tile is free
         if (!SeqDqLds<C>::kOver && more) seq_tile_move<C>(mv, vt_lds, vp, A.v_t, kt + C::BR, end, dbytes);
@@ -237,8 +237,8 @@ seq_attn_dq_kernel(SeqAttnArgs A) {
 #pragma unroll
             for (int i = 0; i < S::GP; ++i) {
               const int g = dh * S::GP + i;
-              const seq_f32x4 a = S::sum(xch, w - dh, 0, g);
-              seq_f32x4 b = S::sum(xch, w - dh, 1, g);
+              const seq_f32x4 a = S::sum(s, xch, w - dh, dh, 0, i);
+              seq_f32x4 b = S::sum(dp, xch, w - dh, dh, 1, i);
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const int key = kb + 8 * g + 4 * h + e;
@@ -246,7 +246,7 @@ seq_attn_dq_kernel(SeqAttnArgs A) {
                 seq_pair<T, cap.value, slope.value>(sc, x, y, full || (key >= me.lo && key < me.hi), lse, delta, me.base - key);
                 b[e] = y;
               }
-              *S::slot(xch, w, 1, g) = b;
+              S::leave(b, xch, w - dh, dh, 1, i);
             }
           });
         __syncthreads();
@@ -274,7 +274,7 @@ seq_attn_dq_kernel(SeqAttnArgs A) {
   const uint32_t bad = seq_bad_rows<C>(acc, 0, red);
   if (bad) seq_attn_dq_again<C>(A, sc, bad, me, row0, head, dh);
   if (row >= A.tq || (bad >> (lane & 31) & 1)) return;
-  seq_store_own<C>(acc, A.scale, A.dq + ((int64_t)row * A.hq + head) * dbytes, nullptr, dh, A.d, A.aln);
+  seq_store_own<C>(acc, A.scale, A.dq + ((int64_t)row * A.hq + head) * A.d * C::OS, nullptr, dh, A.d, A.aln);
 }
 
 // ---- dk, dv: own rows = keys, queries and dout stream ---------------------------------------------------------------------
@@ -289,8 +289,8 @@ __device__ __forceinline__ void seq_attn_dkv_again(const SeqAttnArgs& A, uint32_
   for (int n = 0; n < 32; ++n) {
     const int key = row0 + n;
     if (!(rows >> n & 1) || key >= A.tk || n % C::DS != dh) continue;
-    const SeqSpread k = seq_spread<T>(A.k + kvh * A.k_h + (int64_t)key * A.k_t, A.d);
-    const SeqSpread v = seq_spread<T>(A.v + kvh * A.v_h + (int64_t)key * A.v_t, A.d);
+    const SeqSpread k = seq_spread<T>(A.raw[1].p + kvh * A.raw[1].h + (int64_t)key * A.raw[1].t, A.d);
+    const SeqSpread v = seq_spread<T>(A.raw[2].p + kvh * A.raw[2].h + (int64_t)key * A.raw[2].t, A.d);
     float dk[4] = {0.f, 0.f, 0.f, 0.f}, dv[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
     for (int it = i0; it < i1; ++it) {
@@ -300,8 +300,8 @@ __device__ __forceinline__ void seq_attn_dkv_again(const SeqAttnArgs& A, uint32_
       for (int row = q0; row < q1; ++row) {
         const int4 r = A.rows[row];
         if (key < r.x || key >= r.y) continue;
-        const SeqSpread q = seq_spread<T>(A.q + head * A.q_h + (int64_t)row * A.q_t, A.d);
-        const SeqSpread o = seq_spread<T>(A.dout + head * A.do_h + (int64_t)row * A.do_t, A.d);
+        const SeqSpread q = seq_spread<T>(A.raw[0].p + head * A.raw[0].h + (int64_t)row * A.raw[0].t, A.d);
+        const SeqSpread o = seq_spread<T>(A.raw[3].p + head * A.raw[3].h + (int64_t)row * A.raw[3].t, A.d);
         float s = seq_spread_dot(q, k), dp = seq_spread_dot(o, v);
         seq_pair_any<T>(A, sc, s, dp, true, A.lse[(int64_t)head * A.tq + row], A.delta[(int64_t)head * A.tq + row], r.z - key);
 #pragma unroll
@@ -316,8 +316,8 @@ __device__ __forceinline__ void seq_attn_dkv_again(const SeqAttnArgs& A, uint32_
       seq_spread_store<float>((char*)(part + at), nullptr, dk, A.scale, A.d);
       seq_spread_store<float>((char*)(part + (int64_t)A.tk * A.hk * A.d + at), nullptr, dv, 1.f, A.d);
     } else {
-      seq_spread_store<T>(A.dk + at * C::ES, nullptr, dk, A.scale, A.d);
-      seq_spread_store<T>(A.dv + at * C::ES, nullptr, dv, 1.f, A.d);
+      seq_spread_store<T>(A.dk + at * C::OS, nullptr, dk, A.scale, A.d);
+      seq_spread_store<T>(A.dv + at * C::OS, nullptr, dv, 1.f, A.d);
     }
   }
 }
@@ -327,7 +327,7 @@ struct SeqDkvLds {                                       // tiles, statistics of
   // bfloat16 at 128 columns a wave: keys, values and both accumulators are 192 registers of the 256 that two waves a SIMD leave each,
   // too many next to a pair of blocks (spilled, the kernel took 2.4 ms where it now takes DKV_MS): the values' fragments and PK of the
   // keys' are read from LDS instead, as many as leave room for two workgroups a CU
-  static constexpr bool kPark = C::ES == 2 && C::DH == 128;
+  static constexpr bool kPark = C::OS == 2 && C::DH == 128;
   static constexpr int PK = 3, kParked = kPark ? (PK + C::NF) * 1024 : 0;          // bytes a wave
   static constexpr int kBufs = C::DS == 1 ? 2 : 1, kStat = 5 * C::BR * 4;
   static constexpr int kRows = 2 * kBufs * C::kTileBytes, kXch = kRows + kBufs * kStat;
@@ -347,7 +347,7 @@ seq_attn_dkv_kernel(SeqAttnArgs A) {
   const int id = seq_xcd_order(blockIdx.x, gridDim.x);
   const int kvh = id / tiles, tile = id % tiles, dh = w % C::DS;
   const int first = tile * C::RB, row0 = first + 32 * (w / C::DS), key = row0 + (lane & 31);
-  const int dbytes = A.d * C::ES;
+  const int dbytes = C::row_bytes(A.d);
 
   // query rows that may see a key of this tile: those of the sequences that the tile touches
   int qbeg = 0, qend = 0;
@@ -405,7 +405,7 @@ seq_attn_dkv_kernel(SeqAttnArgs A) {
     load_stat(i0);
     store_stat(st);
   }
-  seq_u32x4 ok[C::NF], ov[C::NF];
+  seq_u32x4 ok[C::PL * C::NF], ov[C::PL * C::NF];
   seq_own_load<C>(ok, A.k + kvh * A.k_h, A.k_t, row0, A.tk, dh, dbytes);
   seq_own_load<C>(ov, A.v + kvh * A.v_h, A.v_t, row0, A.tk, dh, dbytes);
   char* parked = smem + L::kOwn + w * L::kParked;       // read by this wave alone
@@ -522,8 +522,8 @@ seq_attn_dkv_kernel(SeqAttnArgs A) {
         static_assert(C::NSUB == 1, "one pair of blocks is exchanged");
         using S = SeqShare<C, 2>;
         if (active) {
-          S::put(s, xch, w, 0);
-          S::put(dp, xch, w, 1);
+          S::put(s, xch, w - dh, dh, 0);
+          S::put(dp, xch, w - dh, dh, 1);
         }
         __syncthreads();
         if (active)
@@ -531,11 +531,11 @@ seq_attn_dkv_kernel(SeqAttnArgs A) {
 #pragma unroll
             for (int i = 0; i < S::GP; ++i) {
               const int g = dh * S::GP + i;
-              seq_f32x4 a = S::sum(xch, w - dh, 0, g), b = S::sum(xch, w - dh, 1, g);
+              seq_f32x4 a = S::sum(s, xch, w - dh, dh, 0, i), b = S::sum(dp, xch, w - dh, dh, 1, i);
               quad(cap, slope, u, g, a, b);
               if (!full) hide(u, g, a, b);
-              *S::slot(xch, w, 0, g) = a;
-              *S::slot(xch, w, 1, g) = b;
+              S::leave(a, xch, w - dh, dh, 0, i);
+              S::leave(b, xch, w - dh, dh, 1, i);
             }
           });
         __syncthreads();                             // also: the statistics' last reader has passed
@@ -578,7 +578,7 @@ seq_attn_dkv_kernel(SeqAttnArgs A) {
     seq_store_part<C>(dv, 1.f, part + (int64_t)A.tk * A.hk * A.d + to, dh, A.d, 4);
     return;
   }
-  const int64_t at = ((int64_t)key * A.hk + kvh) * dbytes;
+  const int64_t at = ((int64_t)key * A.hk + kvh) * A.d * C::OS;
   seq_store_own<C>(dk, A.scale, A.dk + at, nullptr, dh, A.d, A.aln);
   seq_store_own<C>(dv, 1.f, A.dv + at, nullptr, dh, A.d, A.aln);
 }
@@ -600,21 +600,6 @@ __global__ void __launch_bounds__(256) seq_attn_dkv_join_kernel(SeqAttnArgs A, i
 #pragma unroll
   for (int u = 0; u < 4; ++u)
     if (u < left) out[u] = (T)x[u];
-}
-
-// into how many shares a key tile's work is cut: none with 1024 workgroups or more (4 a CU: as the order masks, their work differs by
-// up to the whole length), else as many as bring it there, 8 at most, within 512 MB of partial sums
-int seq_attn_dkv_splits(int bf16, const SeqAttnArgs& A) {
-  const int rb = A.d <= (bf16 ? 128 : 64) ? 128 : A.d > 128 && bf16 ? 32 : 64;       // own rows of a workgroup
-
-  const int64_t wgs = ((int64_t)A.tk + rb - 1) / rb * A.hk, bytes = (int64_t)A.tk * A.hk * A.d * 8;
-  if (wgs == 0 || wgs >= 1024) return 1;
-  const int64_t work = (int64_t)(A.hq / A.hk) * ((A.tq / (A.nseq > 0 ? A.nseq : 1) + 31) / 32);       // query tiles a key tile sees, about
-  int64_t n = (1024 + wgs - 1) / wgs;
-  n = std::min<int64_t>(n, 8);
-  n = std::min<int64_t>(n, work / 8);                        // a share is 8 tiles at least
-  n = std::min<int64_t>(n, (int64_t(512) << 20) / std::max<int64_t>(bytes, 1));
-  return (int)std::max<int64_t>(n, 1);
 }
 
 template <class C>
@@ -656,26 +641,46 @@ static hipError_t delta(hipStream_t s, const SeqAttnArgs& A) {
 }
 
 template <class T, bool VEC>
-static hipError_t pick(hipStream_t s, const SeqAttnArgs& A) {
-  hipError_t e = hipSuccess;
-  if (A.tq > 0) {
-    e = delta<T>(s, A);
-    if (e != hipSuccess) return e;
-    if (A.d <= 64) e = dq<SeqTile<T, 64, 1, 4, 64, VEC>>(s, A);
-    else if (A.d <= 128) e = dq<SeqTile<T, 128, sizeof(T) == 2 ? 1 : 2, 4, sizeof(T) == 2 ? 64 : 32, VEC>>(s, A);
-    else e = dq<SeqTile<T, 256, sizeof(T) == 2 ? 2 : 4, 4, 32, VEC>>(s, A);
-    if (e != hipSuccess) return e;
-  }
-  if (A.tk == 0) return e;
+static hipError_t pick_dq(hipStream_t s, const SeqAttnArgs& A) {
+  if (A.d <= 64) return dq<SeqTile<T, 64, 1, 4, 64, VEC>>(s, A);
+  if (A.d <= 128) return dq<SeqTile<T, 128, sizeof(T) == 2 ? 1 : 2, 4, sizeof(T) == 2 ? 64 : 32, VEC>>(s, A);
+  return dq<SeqTile<T, 256, sizeof(T) == 2 ? 2 : 4, 4, 32, VEC>>(s, A);
+}
+template <class T, bool VEC>
+static hipError_t pick_dkv(hipStream_t s, const SeqAttnArgs& A) {
   if (A.d <= 64) return dkv<SeqTile<T, 64, 1, 4, 64, VEC>>(s, A);
   if (A.d <= 128) return dkv<SeqTile<T, 128, sizeof(T) == 2 ? 1 : 2, 4, 32, VEC>>(s, A);
   return dkv<SeqTile<T, 256, 4, sizeof(T) == 2 ? 4 : 8, 32, VEC>>(s, A);
 }
+static hipError_t pick_dq_planes(hipStream_t s, const SeqAttnArgs& A) {
+  if (A.d <= 64) return dq<SeqTile<float, 64, 1, 4, 32, true, 3>>(s, A);
+  if (A.d <= 128) return dq<SeqTile<float, 128, 2, 4, 32, true, 3>>(s, A);
+  return dq<SeqTile<float, 256, 4, 8, 32, true, 3>>(s, A);
+}
+static hipError_t pick_dkv_planes(hipStream_t s, const SeqAttnArgs& A) {
+  if (A.d <= 64) return dkv<SeqTile<float, 64, 1, 4, 32, true, 3>>(s, A);
+  if (A.d <= 128) return dkv<SeqTile<float, 128, 2, 4, 32, true, 3>>(s, A);
+  return dkv<SeqTile<float, 256, 4, 8, 32, true, 3>>(s, A);
+}
+int seq_attn_dkv_tile(int bf16, bool planes, int d) {
+  if (planes) return d <= 64 ? 128 : 64;
+  return d <= (bf16 ? 128 : 64) ? 128 : d > 128 && bf16 ? 32 : 64;
+}
 
-hipError_t launch_seq_attn_backward(hipStream_t s, int bf16, const SeqAttnArgs& A) {
+hipError_t launch_seq_attn_bwd(hipStream_t s, int bf16, bool planes, const SeqAttnArgs& A) {
   const bool vec = A.aln >= 4;
-  if (bf16) return vec ? pick<__bf16, true>(s, A) : pick<__bf16, false>(s, A);
-  return vec ? pick<float, true>(s, A) : pick<float, false>(s, A);
+  if (A.tq > 0) {
+    hipError_t e = bf16 ? delta<__bf16>(s, A) : delta<float>(s, A);
+    if (e != hipSuccess) return e;
+    if (planes) e = pick_dq_planes(s, A);
+    else if (bf16) e = vec ? pick_dq<__bf16, true>(s, A) : pick_dq<__bf16, false>(s, A);
+    else e = pick_dq<float, true>(s, A);                // 4-byte elements are 4-byte aligned
+    if (e != hipSuccess) return e;
+  }
+  if (A.tk == 0) return hipSuccess;
+  if (planes) return pick_dkv_planes(s, A);
+  if (bf16) return vec ? pick_dkv<__bf16, true>(s, A) : pick_dkv<__bf16, false>(s, A);
+  return pick_dkv<float, true>(s, A);
 }
 
 }  // namespace sttran

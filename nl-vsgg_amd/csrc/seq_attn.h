@@ -8,7 +8,10 @@
 // The accumulator layout of the score block (lane = own row, 16 registers = stream rows) IS the B layout of the second product
 // once the contraction index is permuted, so probabilities go from the exponential into the next matrix instruction without
 // leaving their lane; row statistics of an own row live in one lane (plus its partner 32 lanes further).
-// bfloat16: v_mfma_f32_32x32x16_bf16, transposed reads by ds_read_b64_tr_b16; fp32: v_mfma_f32_32x32x2_f32 (exact products).
+// bfloat16: v_mfma_f32_32x32x16_bf16, transposed reads by ds_read_b64_tr_b16; fp32: v_mfma_f32_32x32x2_f32 (exact products), or
+// (PL = 3, large calls) three bfloat16 planes: x = hi + mid + lo, 8 bits of mantissa each, so the sum is x exactly, and of the nine
+// products of two such numbers the six that are not below 2^-24 of the largest, each exact in the fp32 accumulator.  That is
+// 6 / 16 of the exact instruction's time, and leaves the vector units free meanwhile, which fp32 matrix instructions do not.
 // Head dims are padded to DP = 64 / 128 / 256 with zeros.  Where 32 own rows and their accumulators would not fit half of a SIMD's
 // registers (so that two waves share it), a team of DS = 2 or 4 waves shares 32 own rows, each contracting (scores) and accumulating
 // (reductions) its part of d; the partial scores meet in LDS.
@@ -19,22 +22,24 @@
 
 namespace sttran {
 
-template <class T, int DP_, int DS_, int NW_, int BR_, bool VEC_>
+template <class T, int DP_, int DS_, int NW_, int BR_, bool VEC_, int PL_ = 1>
 struct SeqTile {
-  using E = T;
+  using E = T;                                       // what the caller's tensors hold
   static constexpr bool VEC = VEC_;
   static constexpr int DP = DP_, DS = DS_, NW = NW_, BR = BR_;
-  static constexpr int ES = sizeof(T);
+  static constexpr int PL = PL_;                     // 3: fp32 as three bfloat16 planes
+  static constexpr int OS = sizeof(T), ES = PL == 3 ? 2 : OS;      // bytes of an element of the tensors / of a tile
   static constexpr int NT = NW * 64;                 // threads
   static constexpr int DH = DP / DS;                 // columns of one wave
   static constexpr int RS = DP * ES;                 // bytes of a tile row
   static constexpr int NC = RS / 16;                 // 16-byte chunks of a tile row
-  static constexpr int NF = DH * ES / 32;            // fragments (16 bytes a lane) of one own row's half
+  static constexpr int NF = DH * ES / 32;            // fragments (16 bytes a lane) of one own row's part, a plane
   static constexpr int NB = DH / 32;                 // 32-column blocks of one wave's accumulator
   static constexpr int NSUB = BR / 32;
   static constexpr int RB = 32 * NW / DS;            // own rows of a workgroup
-  static constexpr int NL = BR * NC / NT;            // chunks a thread moves per tile
-  static constexpr int kTileBytes = BR * RS;
+  static constexpr int NL = BR * NC / NT;            // chunks a thread moves per tile and plane
+  static constexpr int kPlaneBytes = BR * RS, kTileBytes = PL * kPlaneBytes;
+  static __host__ __device__ int row_bytes(int d) { return PL == 3 ? (d + 7) / 8 * 16 : d * OS; }      // of a plane's row in memory
   static constexpr int kStep = NT / NC;              // tile rows between a thread's chunks
   static_assert(BR * NC % NT == 0 && NT % NC == 0, "whole chunks");
   static_assert(2 * kStep % (ES == 4 ? 8 : 16) == 0, "two source offsets: the layout's XOR repeats every 8 (fp32) or 16 rows");
@@ -89,11 +94,14 @@ __device__ __forceinline__ void seq_tile_move(const SeqMover& mv, char* tile, co
 #ifdef __HIP_DEVICE_COMPILE__                              // the host pass refuses 16-byte copies into LDS
   const int rows = min(hi - row0, C::BR);
   if constexpr (C::VEC) {
-    const auto rs = seq_rsrc(base + (int64_t)row0 * stride, stride, rows, dbytes);
 #pragma unroll
-    for (int i = 0; i < C::NL; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(tile + (i * C::NT + mv.wave * 64) * 16), 16,
-                                               mv.off[i & 1], i * C::kStep * (uint32_t)stride, 0, 0);
+    for (int pl = 0; pl < C::PL; ++pl) {                 // a row of planes is [plane][d, padded to 8] in memory
+      const auto rs = seq_rsrc(base + (int64_t)row0 * stride + pl * dbytes, stride, rows, dbytes);
+#pragma unroll
+      for (int i = 0; i < C::NL; ++i)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(tile + pl * C::kPlaneBytes + (i * C::NT + mv.wave * 64) * 16),
+                                                 16, mv.off[i & 1], i * C::kStep * (uint32_t)stride, 0, 0);
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < C::NL; ++i) {
@@ -121,21 +129,25 @@ __device__ __forceinline__ void seq_tile_done(const SeqMover& mv, char* tile, in
   }
 }
 
-// own rows row0 .. row0 + 31 of this wave as B fragments
+// own rows row0 .. row0 + 31 of this wave as B fragments, plane behind plane
 template <class C>
-__device__ __forceinline__ void seq_own_load(seq_u32x4 (&f)[C::NF], const char* base, int64_t stride, int row0, int rows, int dh, int dbytes) {
+__device__ __forceinline__ void seq_own_load(seq_u32x4 (&f)[C::PL * C::NF], const char* base, int64_t stride, int row0, int rows, int dh, int dbytes) {
   const int h = (threadIdx.x >> 5) & 1, n = threadIdx.x & 31, c0 = dh * (C::DH * C::ES / 16) + h;
   const int left = min(rows - row0, 32);
   const char* p = base + (int64_t)row0 * stride;
   if constexpr (C::VEC) {
-    const auto rs = seq_rsrc(p, stride, left, dbytes);
 #pragma unroll
-    for (int i = 0; i < C::NF; ++i) {
-      const int at = 16 * (c0 + 2 * i);
-      f[i] = __builtin_bit_cast(seq_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, at < dbytes ? n * (uint32_t)stride + at : kSeqOob, 0, 0));
+    for (int pl = 0; pl < C::PL; ++pl) {
+      const auto rs = seq_rsrc(p + pl * dbytes, stride, left, dbytes);
+#pragma unroll
+      for (int i = 0; i < C::NF; ++i) {
+        const int at = 16 * (c0 + 2 * i);
+        f[pl * C::NF + i] =
+            __builtin_bit_cast(seq_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, at < dbytes ? n * (uint32_t)stride + at : kSeqOob, 0, 0));
+      }
     }
 #pragma unroll
-    for (int i = 0; i < C::NF; ++i) f[i] &= seq_chunk_mask(c0 + 2 * i, dbytes);
+    for (int i = 0; i < C::PL * C::NF; ++i) f[i] &= seq_chunk_mask(c0 + 2 * (i % C::NF), dbytes);
   } else {
 #pragma unroll
     for (int i = 0; i < C::NF; ++i) {
@@ -156,16 +168,40 @@ __device__ __forceinline__ void seq_wave_range(int& lo, int& hi) {
   hi = __builtin_amdgcn_readfirstlane(hi);
 }
 
+__device__ __forceinline__ seq_f32x16 seq_mma(seq_f32x16 acc, seq_u32x4 a, seq_u32x4 b) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(seq_bf16x8, a), __builtin_bit_cast(seq_bf16x8, b), acc, 0, 0, 0);
+}
+// (a0 + a1 + a2)(b0 + b1 + b2) without the three smallest terms, small ones first
+__device__ __forceinline__ seq_f32x16 seq_six(seq_f32x16 acc, seq_u32x4 a0, seq_u32x4 a1, seq_u32x4 a2, seq_u32x4 b0, seq_u32x4 b1, seq_u32x4 b2) {
+  acc = seq_mma(acc, a2, b0);
+  acc = seq_mma(acc, a0, b2);
+  acc = seq_mma(acc, a1, b1);
+  acc = seq_mma(acc, a1, b0);
+  acc = seq_mma(acc, a0, b1);
+  return seq_mma(acc, a0, b0);
+}
+// x = hi + mid + lo, each a bfloat16 (what the rounding of one leaves is the next one's number)
+__device__ __forceinline__ void seq_split3(float x, __bf16& hi, __bf16& mid, __bf16& lo) {
+  hi = (__bf16)x;
+  const float r = x - (float)hi;
+  mid = (__bf16)r;
+  lo = (__bf16)(r - (float)mid);
+}
+
 // acc[stream row][own row] += tile . own
 template <class C>
-__device__ __forceinline__ void seq_scores(seq_f32x16& acc, const char* tile, int sub, int dh, const seq_u32x4 (&own)[C::NF]) {
+__device__ __forceinline__ void seq_scores(seq_f32x16& acc, const char* tile, int sub, int dh, const seq_u32x4 (&own)[C::PL * C::NF]) {
   const int lane = threadIdx.x & 63, row = 32 * sub + (lane & 31), h = lane >> 5;
   const char* p = tile + row * C::RS;
   const int x = (h ^ seq_swz<C>(row)) << 4;
 #pragma unroll
   for (int f = 0; f < C::NF; ++f) {
     const seq_u32x4 a = *reinterpret_cast<const seq_u32x4*>(p + ((dh * C::DH * C::ES + 32 * f) ^ x));
-    if constexpr (C::ES == 2) {
+    if constexpr (C::PL == 3) {
+      const seq_u32x4 a1 = *reinterpret_cast<const seq_u32x4*>(p + C::kPlaneBytes + ((dh * C::DH * C::ES + 32 * f) ^ x));
+      const seq_u32x4 a2 = *reinterpret_cast<const seq_u32x4*>(p + 2 * C::kPlaneBytes + ((dh * C::DH * C::ES + 32 * f) ^ x));
+      acc = seq_six(acc, a, a1, a2, own[f], own[C::NF + f], own[2 * C::NF + f]);
+    } else if constexpr (C::ES == 2) {
       acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(seq_bf16x8, a), __builtin_bit_cast(seq_bf16x8, own[f]), acc, 0, 0, 0);
     } else {
 #pragma unroll
@@ -177,7 +213,7 @@ __device__ __forceinline__ void seq_scores(seq_f32x16& acc, const char* tile, in
 
 // the same with the first P of the own rows' fragments parked in LDS (`parked`: this wave's, fragment by fragment, 16 bytes a lane)
 template <class C, int P>
-__device__ __forceinline__ void seq_scores_parked(seq_f32x16& acc, const char* tile, int sub, int dh, const char* parked, const seq_u32x4 (&own)[C::NF]) {
+__device__ __forceinline__ void seq_scores_parked(seq_f32x16& acc, const char* tile, int sub, int dh, const char* parked, const seq_u32x4 (&own)[C::PL * C::NF]) {
   const int lane = threadIdx.x & 63, row = 32 * sub + (lane & 31), h = lane >> 5;
   const char* p = tile + row * C::RS;
   const int x = (h ^ seq_swz<C>(row)) << 4;
@@ -198,20 +234,37 @@ __device__ __forceinline__ void seq_reduce(seq_f32x16 (&acc)[C::NB], const char*
     const int g = lane >> 4, i = lane & 15, h = g >> 1;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      seq_bf16x8 b;
+      seq_bf16x8 b[C::PL];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) b[j] = (__bf16)w[8 * t + j];
+      for (int j = 0; j < 8; ++j) {
+        if constexpr (C::PL == 3) {
+          __bf16 x, y, z;
+          seq_split3(w[8 * t + j], x, y, z);
+          b[0][j] = x; b[1][j] = y; b[2][j] = z;
+        } else {
+          b[0][j] = (__bf16)w[8 * t + j];
+        }
+      }
       const int row0 = 32 * sub + 16 * t + 4 * h + (i >> 2), row1 = row0 + 8;
       const int col = 2 * (dh * C::DH + 16 * (g & 1)) + 8 * (i & 3);                // byte within the row, block 0
       const int x0 = seq_swz<C>(row0) << 4, x1 = seq_swz<C>(row1) << 4;
 #pragma unroll
       for (int nb = 0; nb < C::NB; ++nb) {
-        typedef __attribute__((address_space(3))) seq_s16x4 lds_s16x4;
-        const seq_s16x4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + row0 * C::RS + ((col + 64 * nb) ^ x0)));
-        const seq_s16x4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + row1 * C::RS + ((col + 64 * nb) ^ x1)));
-        typedef short s16x8 __attribute__((ext_vector_type(8)));
-        const s16x8 a = {a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]};
-        acc[nb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(seq_bf16x8, a), b, acc[nb], 0, 0, 0);
+        seq_u32x4 a[C::PL];
+#pragma unroll
+        for (int pl = 0; pl < C::PL; ++pl) {
+          typedef __attribute__((address_space(3))) seq_s16x4 lds_s16x4;
+          const char* p = tile + pl * C::kPlaneBytes;
+          const seq_s16x4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + row0 * C::RS + ((col + 64 * nb) ^ x0)));
+          const seq_s16x4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + row1 * C::RS + ((col + 64 * nb) ^ x1)));
+          typedef short s16x8 __attribute__((ext_vector_type(8)));
+          a[pl] = __builtin_bit_cast(seq_u32x4, s16x8{a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]});
+        }
+        if constexpr (C::PL == 3)
+          acc[nb] = seq_six(acc[nb], a[0], a[1], a[2], __builtin_bit_cast(seq_u32x4, b[0]), __builtin_bit_cast(seq_u32x4, b[1]),
+                            __builtin_bit_cast(seq_u32x4, b[2]));
+        else
+          acc[nb] = seq_mma(acc[nb], a[0], __builtin_bit_cast(seq_u32x4, b[0]));
       }
     }
   } else {
@@ -300,26 +353,39 @@ __device__ __forceinline__ void seq_set_quad(seq_f32x16& s, int g, seq_f32x4 x) 
 __device__ __forceinline__ seq_f32x4* seq_slot(char* at, int slot) {
   return reinterpret_cast<seq_f32x4*>(at + slot * 1024) + (threadIdx.x & 63);
 }
-// B blocks a wave.  Member j of a team finishes quads j * GP .. (j + 1) * GP - 1: everyone puts its blocks; after a barrier the
-// finisher sums its quads over the members, in their order, and leaves what it made of them in its OWN slot of that quad, which
-// nobody else reads before the next barrier; after that, take() has the whole blocks.
+// B blocks a wave.  Member j of a team finishes quads j * GP .. (j + 1) * GP - 1: everyone puts the quads that are not its own;
+// after a barrier the finisher adds up its quads and leaves what it made of a quad in a slot of it that nobody but itself has read;
+// after another barrier take() has the whole blocks.
 template <class C, int B>
 struct SeqShare {
-  static constexpr int GP = 4 / C::DS, kWave = B * 4096;
-  static __device__ __forceinline__ seq_f32x4* slot(char* xch, int wave, int block, int g) { return seq_slot(xch, (wave * B + block) * 4 + g); }
-  static __device__ __forceinline__ void put(const seq_f32x16& s, char* xch, int wave, int block) {
-#pragma unroll
-    for (int g = 0; g < 4; ++g) *slot(xch, wave, block, g) = seq_quad(s, g);
+  static constexpr int GP = 4 / C::DS, kSlots = 4 - GP, kWave = B * kSlots * 1024;
+  static __device__ __forceinline__ seq_f32x4* slot(char* xch, int first, int j, int block, int g) {     // of quad g in member j's area
+    return seq_slot(xch, ((first + j) * B + block) * kSlots + (g < j * GP ? g : g - GP));
   }
-  static __device__ __forceinline__ seq_f32x4 sum(char* xch, int first, int block, int g) {
-    seq_f32x4 r = *slot(xch, first, block, g);
+  static __device__ __forceinline__ void put(const seq_f32x16& s, char* xch, int first, int j, int block) {
 #pragma unroll
-    for (int m = 1; m < C::DS; ++m) r += *slot(xch, first + m, block, g);
+    for (int g = 0; g < 4; ++g)
+      if (g / GP != j) *slot(xch, first, j, block, g) = seq_quad(s, g);
+  }
+  // own quad i (number j * GP + i) over all members, one after the other from the next one on
+  static __device__ __forceinline__ seq_f32x4 sum(const seq_f32x16& s, char* xch, int first, int j, int block, int i) {
+    seq_f32x4 r = seq_quad(s, i);
+#pragma unroll
+    for (int o = 1; o < C::DS; ++o) {
+      const seq_f32x4 q = seq_quad(s, o * GP + i);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) r[u] = j == o ? q[u] : r[u];
+    }
+#pragma unroll
+    for (int o = 1; o < C::DS; ++o) r += *slot(xch, first, (j + o) % C::DS, block, j * GP + i);
     return r;
+  }
+  static __device__ __forceinline__ void leave(seq_f32x4 x, char* xch, int first, int j, int block, int i) {
+    *slot(xch, first, (j + 1) % C::DS, block, j * GP + i) = x;
   }
   static __device__ __forceinline__ void take(seq_f32x16& s, char* xch, int first, int block) {
 #pragma unroll
-    for (int g = 0; g < 4; ++g) seq_set_quad(s, g, *slot(xch, first + g / GP, block, g));
+    for (int g = 0; g < 4; ++g) seq_set_quad(s, g, *slot(xch, first, (g / GP + 1) % C::DS, block, g));
   }
 };
 
@@ -334,7 +400,7 @@ __device__ __forceinline__ void seq_store_own(const seq_f32x16 (&acc)[C::NB], fl
     for (int q = 0; q < 4; ++q) {
       const int col = dh * C::DH + 32 * nb + 8 * q + 4 * h;
       if (col >= d) continue;
-      if constexpr (C::ES == 4) {
+      if constexpr (C::OS == 4) {
         seq_u32x4 r;
 #pragma unroll
         for (int u = 0; u < 4; ++u) r[u] = __float_as_uint(acc[nb][4 * q + u] * mul);

@@ -120,6 +120,7 @@ __device__ __forceinline__ float seq_group_sum(float x) {
 struct SeqAttnArgs {
   const char *q, *k, *v, *dout;
   int64_t q_t, q_h, k_t, k_h, v_t, v_h, do_t, do_h;
+  struct In { const char* p; int64_t t, h; } raw[4];      // q, k, v, dout as the caller gave them (the above may be planes of them)
   char *out, *out_lo, *dq, *dk, *dv;      // contiguous [rows, heads, d]; out_lo: what rounding took from out (bfloat16, training)
   float* lse;                             // [q heads][q rows], base 2: max + log2(sum); +inf for a row that sees nothing
   float* delta;                           // [q heads][q rows]: sum of dout * out

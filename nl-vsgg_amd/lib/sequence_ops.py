@@ -144,8 +144,9 @@ class _PackedAttention(torch.autograd.Function):
         a.dout, a.dout_row_stride, a.dout_head_stride = dout.data_ptr(), dout.stride(0) if dout.shape[0] > 1 else 0, dout.stride(1)
         a.dq, a.dk, a.dv = (g.data_ptr() for g in grads)
         need = lib.sttran_attention_workspace_bytes(C.byref(a), 1)
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), need
+        if need:
+            ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), need
         _launch(lib.sttran_attention_backward, (C.byref(a),), q.device)
         return (*grads, None, None, None, None, None, None, None)
 
