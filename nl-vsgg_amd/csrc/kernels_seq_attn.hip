@@ -49,28 +49,28 @@ __device__ __forceinline__ void seq_attn_fwd_again(const SeqAttnArgs& A, const S
 // only when the maximum grows by more than 8 (a factor of 256): p stays below 2^8 and the final division by l undoes any
 // common factor exactly as the textbook form does.
 // N scores of one row, x[i] of key k0 + 8 (i / 4) + i % 4, become what z is linear in -- z = c1 * x + c0 -- so that one fma stands
-// before the exponential; hidden ones become -inf (c1 > 0); returns the largest z.
-//   plain: the products (scale > 0);  cap (bfloat16): -1 / (1 + e^(2 products)), z = cap - 2 cap / (1 + ..);  else: z itself
-template <class C, int N>
+// before the exponential; hidden ones become -inf (c1 > 0); returns the largest z.  SLOPE: distances, or a scale that is not positive.
+//   neither: the products;  CAP alone (bfloat16): -1 / (1 + e^(2 products)), z = cap - 2 cap / (1 + ..);  else: z itself
+template <class C, bool CAP, bool SLOPE, int N>
 __device__ __forceinline__ float seq_bend(const SeqAttnArgs& A, const SeqScore& sc, float (&x)[N], int k0, int base, bool full, int lo, int hi,
                                           float& c1, float& c0) {
   using T = typename C::E;
-  if (A.cap <= 0.f && !A.slope && sc.mul > 0.f) {
+  if constexpr (!CAP && !SLOPE) {
     c1 = sc.mul; c0 = 0.f;
-  } else if (C::OS == 2 && A.cap > 0.f && !A.slope) {
+  } else if constexpr (C::OS == 2 && CAP && !SLOPE) {
     c1 = 2.f * sc.capl; c0 = sc.capl;
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = -__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x[i] * (sc.mul * (2.f * kSeqLog2e))));
   } else {
     c1 = 1.f; c0 = 0.f;
-    if (A.cap > 0.f) {
+    if constexpr (CAP) {
 #pragma unroll
       for (int i = 0; i < N; ++i) x[i] = sc.capl * seq_tanh<T>(x[i] * sc.mul);
     } else {
 #pragma unroll
       for (int i = 0; i < N; ++i) x[i] *= sc.mul;
     }
-    if (A.slope) {
+    if constexpr (SLOPE) {
       const float at = (float)(base - k0);
 #pragma unroll
       for (int i = 0; i < N; ++i) x[i] = fmaf(-sc.slope, fabsf(at - (float)(8 * (i >> 2) + (i & 3))), x[i]);
@@ -97,7 +97,7 @@ struct SeqFwdLds {                                       // DS == 1: two tiles o
   static constexpr int kXch = 2 * kBufs * C::kTileBytes, kRed = kXch, kRefs = kXch + (C::DS > 1 ? C::NW * SeqShare<C, 1>::kWave : 0);
   static constexpr int kBytes = C::DS > 1 ? kRefs + C::NW * 128 : kXch + C::NW * 8;
 };
-template <class C>
+template <class C, bool CAP, bool SLOPE>
 __global__ void __launch_bounds__(C::NT) __attribute__((amdgpu_waves_per_eu(2, 2)))
 seq_attn_fwd_kernel(SeqAttnArgs A) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -180,7 +180,7 @@ seq_attn_fwd_kernel(SeqAttnArgs A) {
         float x[16 * C::NSUB];
 #pragma unroll
         for (int i = 0; i < 16 * C::NSUB; ++i) x[i] = s[i >> 4][i & 15];
-        float mt = seq_bend<C>(A, sc, x, kt + 4 * h, me.base, full, rlo, rhi, c1, c0);
+        float mt = seq_bend<C, CAP, SLOPE>(A, sc, x, kt + 4 * h, me.base, full, rlo, rhi, c1, c0);
         mt = fmaxf(mt, __shfl_xor(mt, 32));
         if (__any(mt > m + 8.f || (m == -INFINITY && mt > -INFINITY))) {
           const float mn = fmaxf(m, mt);
@@ -222,7 +222,7 @@ seq_attn_fwd_kernel(SeqAttnArgs A) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) x[4 * i + e] = q[e];
         }
-        float mt = seq_bend<C>(A, sc, x, kt + 8 * dh * S::GP + 4 * h, me.base, full, rlo, rhi, c1, c0);
+        float mt = seq_bend<C, CAP, SLOPE>(A, sc, x, kt + 8 * dh * S::GP + 4 * h, me.base, full, rlo, rhi, c1, c0);
         mt = fmaxf(mt, __shfl_xor(mt, 32));
         const float ref = mt > m + 30.f ? mt : m;
         c0 -= ref == -INFINITY ? 0.f : ref;
@@ -382,12 +382,12 @@ hipError_t launch_seq_attn_join(hipStream_t s, int bf16, const SeqAttnArgs& A, c
   return hipGetLastError();
 }
 
-template <class C>
-static hipError_t fwd(hipStream_t s, const SeqAttnArgs& A) {
+template <class C, bool CAP, bool SLOPE>
+static hipError_t fwd_as(hipStream_t s, const SeqAttnArgs& A) {
   constexpr int lds = SeqFwdLds<C>::kBytes;
   static_assert(lds <= 160 * 1024, "LDS of a CU");
   static DeviceMarks marks;
-  auto fn = seq_attn_fwd_kernel<C>;
+  auto fn = seq_attn_fwd_kernel<C, CAP, SLOPE>;
   hipError_t e = marks.raise_lds(reinterpret_cast<const void*>(fn), lds);
   if (e != hipSuccess) return e;
   const int tiles = (A.tq + C::RB - 1) / C::RB;
@@ -396,10 +396,20 @@ static hipError_t fwd(hipStream_t s, const SeqAttnArgs& A) {
   return e != hipSuccess || A.splits == 1 ? e : launch_seq_attn_join(s, C::OS == 2, A, nullptr, 0, 0);
 }
 
-// Own rows a workgroup: 128 where a wave holds whole heads; 32 or 64 where teams of waves share them
+// A kernel for each of no cap and cap, no distances and distances: with the others' bodies beside its own in one kernel the registers
+// spill and drain the loads in flight (three sequences of 4000 .. 8000 rows, 128 columns: forward 335 -> 307 us)
+template <class C>
+static hipError_t fwd(hipStream_t s, const SeqAttnArgs& A) {
+  const bool slope = A.slope || A.scale <= 0.f;          // without distances their factor is zero
+  if (A.cap > 0.f) return slope ? fwd_as<C, true, true>(s, A) : fwd_as<C, true, false>(s, A);
+  return slope ? fwd_as<C, false, true>(s, A) : fwd_as<C, false, false>(s, A);
+}
+
+// Own rows a workgroup: 128 or (heads of 64 columns, whose calls have small tiles to spare: 84 -> 74 us on 96 sequences of 37 .. 500
+// rows, 263 -> 254 us on three of 4000 .. 8000) 64 where a wave holds whole heads; 32 or 64 where teams of waves share them
 template <class T, bool VEC>
 static hipError_t pick(hipStream_t s, const SeqAttnArgs& A) {
-  if (A.d <= 64) return fwd<SeqTile<T, 64, 1, 4, 64, VEC>>(s, A);
+  if (A.d <= 64) return fwd<SeqTile<T, 64, 1, 2, 64, VEC>>(s, A);
   if (A.d <= 128) return fwd<SeqTile<T, 128, 1, 4, sizeof(T) == 2 ? 64 : 32, VEC>>(s, A);
   return fwd<SeqTile<T, 256, sizeof(T) == 2 ? 2 : 4, 4, 32, VEC>>(s, A);
 }
@@ -410,7 +420,7 @@ static hipError_t pick_planes(hipStream_t s, const SeqAttnArgs& A) {
 }
 int seq_attn_fwd_tile(int bf16, bool planes, int d) {
   if (planes) return d <= 64 ? 128 : 64;
-  return d <= 128 ? 128 : bf16 ? 64 : 32;
+  return d <= 64 ? 64 : d <= 128 ? 128 : bf16 ? 64 : 32;
 }
 
 hipError_t launch_seq_attn_fwd(hipStream_t s, int bf16, bool planes, const SeqAttnArgs& A) {
