@@ -310,10 +310,10 @@ __device__ __forceinline__ void seq_attn_dkv_again(const SeqAttnArgs& A, uint32_
 template <class C>
 struct SeqDkvLds {                                       // tiles, statistics of the tile's rows, partial and whole score blocks
   // bfloat16 at 128 columns a wave: keys, values and both accumulators are 192 registers of the 256 that two waves a SIMD leave each,
-  // too many next to a pair of blocks (spilled, the kernel took 2.4 ms where it now takes DKV_MS): the values' fragments and PK of the
-  // keys' are read from LDS instead, as many as leave room for two workgroups a CU
+  // too many next to a pair of blocks (spilled, the kernel took 2.4 ms on three sequences of 4000 .. 8000 rows, 8 heads, where it now
+  // takes 0.85): the values' fragments are read from LDS instead
   static constexpr bool kPark = C::OS == 2 && C::DH == 128;
-  static constexpr int PK = 3, kParked = kPark ? (PK + C::NF) * 1024 : 0;          // bytes a wave
+  static constexpr int kParked = kPark ? C::NF * 1024 : 0;          // bytes a wave
   static constexpr int kBufs = C::DS == 1 ? 2 : 1, kStat = 5 * C::BR * 4;
   static constexpr int kRows = 2 * kBufs * C::kTileBytes, kXch = kRows + kBufs * kStat;
   static constexpr int kRed = kXch + (C::DS > 1 ? C::NW * SeqShare<C, 2>::kWave : 0);
@@ -396,10 +396,7 @@ seq_attn_dkv_kernel(SeqAttnArgs A) {
   char* parked = smem + L::kOwn + w * L::kParked;       // read by this wave alone
   if constexpr (L::kPark) {
 #pragma unroll
-    for (int f = 0; f < C::NF; ++f) {
-      if (f < L::PK) *reinterpret_cast<seq_u32x4*>(parked + f * 1024 + lane * 16) = ok[f];
-      *reinterpret_cast<seq_u32x4*>(parked + (L::PK + f) * 1024 + lane * 16) = ov[f];
-    }
+    for (int f = 0; f < C::NF; ++f) *reinterpret_cast<seq_u32x4*>(parked + f * 1024 + lane * 16) = ov[f];
   }
   seq_f32x16 dk[C::NB], dv[C::NB];
 #pragma unroll
@@ -463,8 +460,7 @@ seq_attn_dkv_kernel(SeqAttnArgs A) {
       if (active) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[e] = 0.f;
-        if constexpr (L::kPark) seq_scores_parked<C, L::PK>(s, qt_lds, u, dh, parked, ok);
-        else seq_scores<C>(s, qt_lds, u, dh, ok);
+        seq_scores<C>(s, qt_lds, u, dh, ok);
       }
       if constexpr (C::DS > 1) {                     // dout's tile was still on its way while q's was used
         if (it > i0) {
@@ -475,7 +471,7 @@ seq_attn_dkv_kernel(SeqAttnArgs A) {
       if (active) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) dp[e] = 0.f;
-        if constexpr (L::kPark) seq_scores_parked<C, C::NF>(dp, gt_lds, u, dh, parked + L::PK * 1024, ov);
+        if constexpr (L::kPark) seq_scores_parked<C>(dp, gt_lds, u, dh, parked);
         else seq_scores<C>(dp, gt_lds, u, dh, ov);
       }
       if constexpr (C::DS == 1) {

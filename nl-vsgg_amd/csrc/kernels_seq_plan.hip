@@ -49,16 +49,22 @@ __global__ void __launch_bounds__(256) seq_split_kernel(SeqSplitArgs A) {
 static int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 
 // Planes take the matrix products from fp32 instructions to bfloat16 ones (6 of them for one, of a sixteenth of the time each) and cost a
-// pass over the tensors: worth it from sequences of some hundred keys on, and where a launch is long against three more.
+// pass over the tensors, three times the LDS of a tile and up to three more launches.  Measured on 16384 rows, 8 heads, a training step:
+//   64 columns: 128 keys 323 us on fp32 instructions, 308 on planes; 256 keys 514, 347; 2048 keys 2317, 1091
+//   128: 128 keys 467, 594; 256 keys 729, 736; 512 keys 1181, 943; 2048 keys 3298, 2137
+//   200: 512 keys 2151, 2148 (forward alone 474, 602); 1024 keys 3565, 3041 (790, 818); 2048 keys 5957, 4608 (1369, 1228)
+// and on calls too small to fill the card (one sequence): 2 heads of 64 columns, 256 rows 158, 106 (26, 24); 2 of 128, 512 rows 178, 137
+// (53, 35); 2 of 200, 1024 rows 275, 263 (42, 54).
 static bool use_planes(int bf16, const SeqAttnArgs& A) {
   if (bf16 || A.nseq <= 0) return false;
-  const double keys = (double)A.tk / A.nseq, flops = 4.0 * A.tq * keys * A.d * A.hq;
-  return keys >= 512 && flops >= 8e9;
+  if ((int64_t)std::max(A.hq, A.hk) * 48 * ((A.d + 7) / 8) > (1 << 24)) return false;      // a tile's rows are addressed in 32 bits
+  return A.tk / A.nseq >= (A.d <= 64 ? 256 : A.d <= 128 ? 512 : 1024);
 }
 
 // Shares of the keys: where there are too few (row tile, head) pairs for the 256 CUs, up to two workgroups a CU, 256 keys a share at
 // least.  The keys that a tile sees are known on the device alone; their number is taken from the tensors' sizes, and a share of
-// a shorter range is shorter.
+// a shorter range is shorter.  (8 heads, 128 columns, one share and these: 64 rows over 8192 keys 163 -> 25 us in bfloat16, 1053 -> 54 in
+// fp32; 1024 rows over 8192 keys 165 -> 78, 519 -> 262; 2 x 16 rows over 512 keys 35 -> 26, 145 -> 82.)
 static int fwd_splits(int bf16, bool planes, const SeqAttnArgs& A) {
   const int tile = seq_attn_fwd_tile(bf16, planes, A.d);
   const int64_t wgs = ((int64_t)A.tq + tile - 1) / tile * A.hq;
@@ -67,7 +73,8 @@ static int fwd_splits(int bf16, bool planes, const SeqAttnArgs& A) {
   return (int)std::max<int64_t>(1, std::min<int64_t>(n, 64));
 }
 // Shares of a key tile's work: none with 1024 workgroups or more (4 a CU: as the order masks, their work differs by up to the whole
-// length), else as many as bring it there, 8 at most, within 512 MB of partial sums
+// length), else as many as bring it there, 8 at most, within 512 MB of partial sums.  (A training step with one share and these: one
+// sequence of 4096 rows, 8 heads, 444 -> 379 us; three of 6000, 8 heads over 4, 1546 -> 1455; 96 of 250, 16 over 2: 337, 336.)
 static int dkv_splits(int bf16, bool planes, const SeqAttnArgs& A) {
   const int rb = seq_attn_dkv_tile(bf16, planes, A.d);
   const int64_t wgs = ((int64_t)A.tk + rb - 1) / rb * A.hk, bytes = (int64_t)A.tk * A.hk * A.d * 8;

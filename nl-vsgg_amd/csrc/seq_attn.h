@@ -211,16 +211,16 @@ __device__ __forceinline__ void seq_scores(seq_f32x16& acc, const char* tile, in
   }
 }
 
-// the same with the first P of the own rows' fragments parked in LDS (`parked`: this wave's, fragment by fragment, 16 bytes a lane)
-template <class C, int P>
-__device__ __forceinline__ void seq_scores_parked(seq_f32x16& acc, const char* tile, int sub, int dh, const char* parked, const seq_u32x4 (&own)[C::PL * C::NF]) {
+// the same with the own rows' fragments parked in LDS (`parked`: this wave's, fragment by fragment, 16 bytes a lane)
+template <class C>
+__device__ __forceinline__ void seq_scores_parked(seq_f32x16& acc, const char* tile, int sub, int dh, const char* parked) {
   const int lane = threadIdx.x & 63, row = 32 * sub + (lane & 31), h = lane >> 5;
   const char* p = tile + row * C::RS;
   const int x = (h ^ seq_swz<C>(row)) << 4;
 #pragma unroll
   for (int f = 0; f < C::NF; ++f) {
     const seq_u32x4 a = *reinterpret_cast<const seq_u32x4*>(p + ((dh * C::DH * C::ES + 32 * f) ^ x));
-    const seq_u32x4 b = f < P ? *reinterpret_cast<const seq_u32x4*>(parked + f * 1024 + lane * 16) : own[f];
+    const seq_u32x4 b = *reinterpret_cast<const seq_u32x4*>(parked + f * 1024 + lane * 16);
     acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(seq_bf16x8, a), __builtin_bit_cast(seq_bf16x8, b), acc, 0, 0, 0);
   }
 }

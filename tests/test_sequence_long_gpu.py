@@ -1,0 +1,267 @@
+"""Attention over long packed sequences: float32 tensors on bfloat16 planes, shares of the keys joined, in 64 bits' sight.
+
+Tolerances.  Beside those of short sequences (4e-6 of the 2-norm in float32, 2^-8 in bfloat16): a sum over n keys takes n roundings of
+its running value, about sqrt(n) * 2^-24 of its terms, so what was derived for 256 of them grows by sqrt(n / 256).  Three planes hold a
+number to 2^-26 of itself, and the three products of planes that are left out are below 2^-27 of the whole each: less than one rounding
+of the sum.  dq and dk further carry what dp - delta loses (4e-6 of the terms' 2-norms, weighted as ds is) and in bfloat16 the rounding
+of the probabilities in delta: at most 2^-8 sum_j p_j |dp_j|, and 2^-16 sum |dout out|."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DT = {"f32": torch.float32, "bf16": torch.bfloat16}
+
+
+@pytest.fixture(scope="module")
+def ops():
+    if not torch.cuda.is_available():
+        pytest.skip("needs an MI355X")
+    from nl_vsgg_amd.lib import sequence_ops
+    return sequence_ops
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def _offsets(lens):
+    off = [0]
+    for n in lens:
+        off.append(off[-1] + n)
+    return off
+
+
+def _normal(seed, *shape, dtype=torch.float32):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn(shape, generator=g, dtype=torch.float32).to(dtype).cuda()
+
+
+def _ref(q, k, v, do, off_q, off_k, causal=False, prefix_len=None, distance_slope=None, score_cap=0.0, scale=None):
+    """The definition in float64, finite inputs; (result, allowed error in its 2-norm) of out, dq, dk, dv."""
+    f32 = 4e-6 * max(1.0, math.sqrt(max(b - a for a, b in zip(off_k, off_k[1:])) / 256))
+    half = 2.0 ** -8 if q.dtype == torch.bfloat16 else 0.0
+    q, k, v, do = (x.detach().double().cpu() for x in (q, k, v, do))
+    grp, scale = q.shape[1] // k.shape[1], q.shape[2] ** -0.5 if scale is None else scale
+    out, dq, dk, dv, xq, xk = (torch.zeros_like(x) for x in (q, q, k, v, q, k))
+    for s in range(len(off_q) - 1):
+        a, b, c, d = off_q[s], off_q[s + 1], off_k[s], off_k[s + 1]
+        place, key = torch.arange(b - a)[:, None] + (d - c) - (b - a), torch.arange(d - c)[None]
+        see = torch.ones(b - a, d - c, dtype=torch.bool)
+        if causal:
+            see = (key <= place) | (key < (0 if prefix_len is None else prefix_len[s]))
+        for h in range(q.shape[1]):
+            Q, K, V, G = q[a:b, h], k[c:d, h // grp], v[c:d, h // grp], do[a:b, h]
+            z, bend = scale * Q @ K.T, 1.0
+            if score_cap:
+                t = torch.tanh(z / score_cap)
+                z, bend = score_cap * t, 1 - t * t
+            if distance_slope is not None:
+                z = z - distance_slope[h] * (place - key).abs()
+            z = z.masked_fill(~see, -math.inf)
+            p = torch.nan_to_num(torch.softmax(z, 1), nan=0.0)
+            O = p @ V
+            out[a:b, h] = O
+            dp, delta = G @ V.T, (G * O).sum(1, keepdim=True)
+            ds = p * (dp - delta) * bend
+            off = f32 * (((G * G) @ (V * V).T).sqrt() + (G * O).norm(dim=1, keepdim=True))
+            off = p * bend * (off + half * (p * dp.abs()).sum(1, keepdim=True) + half * half * (G * O).abs().sum(1, keepdim=True))
+            dq[a:b, h], xq[a:b, h] = scale * ds @ K, scale * off @ K.abs()
+            dk[c:d, h // grp] += scale * ds.T @ Q
+            xk[c:d, h // grp] += scale * off.T @ Q.abs()
+            dv[c:d, h // grp] += p.T @ G
+    rel = half or f32
+    return [(x, rel * x.norm() + e) for x, e in ((out, 0.0), (dq, xq.norm()), (dk, xk.norm()), (dv, 0.0))]
+
+
+def _run(ops, q, k, v, do, off_q, off_k, prefix_len=None, distance_slope=None, **kw):
+    leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+    out = ops.packed_attention(*leaves, _i32(off_q), _i32(off_k), prefix_len=None if prefix_len is None else _i32(prefix_len),
+                               distance_slope=None if distance_slope is None else torch.tensor(distance_slope, device="cuda"), **kw)
+    return [out.detach(), *torch.autograd.grad(out, leaves, do)]
+
+
+def _inputs(lq, lk, hq, hk, d, dtype, seed=0, tail=(0, 0)):
+    off_q, off_k = _offsets(lq), _offsets(lk)
+    tq, tk = off_q[-1] + tail[0], off_k[-1] + tail[1]
+    return [_normal(seed + i, n, h, d, dtype=dtype) for i, (n, h) in enumerate(((tq, hq), (tk, hk), (tk, hk), (tq, hq)))] + [off_q, off_k]
+
+
+def _check(ops, lq, lk, hq, hk, d, dtype, seed=0, tail=(0, 0), **kw):
+    x = _inputs(lq, lk, hq, hk, d, dtype, seed, tail)
+    got = _run(ops, *x, **kw)
+    for n, g, (r, tol) in zip(("out", "dq", "dk", "dv"), got, _ref(*x, **kw)):
+        assert bool(torch.isfinite(g).all()), n
+        off = (g.double().cpu() - r).norm()
+        assert off <= tol, f"{n}: off by {off / r.norm():.2e} of its norm, {tol / r.norm():.2e} allowed"
+    plain = ops.packed_attention(x[0], x[1], x[2], _i32(x[4]), _i32(x[5]), **{
+        n: (_i32(v) if n == "prefix_len" else torch.tensor(v, device="cuda") if n == "distance_slope" else v) for n, v in kw.items()})
+    assert torch.equal(plain, got[0]), "the training forward answers like the other"
+    return x, got
+
+
+def _on_planes(ops, q, k, v, off):
+    """whether a call takes the planes: its workspace holds 6 bytes an element of q, k and v"""
+    from nl_vsgg_amd import _native
+    a = ops._attention_struct(q, k, v, _i32(off), _i32(off), None, None, False, 0.0, 1.0)
+    return _native.load().sttran_attention_workspace_bytes(ctypes.byref(a), 0) >= 6 * (q.numel() + k.numel() + v.numel())
+
+
+MASKS = {
+    "all": {},
+    "causal": dict(causal=True),
+    "prefix": dict(causal=True, prefix_len=[700, 90]),
+    "distance": dict(distance_slope=[0.3, 0.01]),
+    "cap": dict(score_cap=1.5),
+    "everything": dict(causal=True, prefix_len=[9, 2000], distance_slope=[0.05, 0.002], score_cap=2.0, scale=0.3),
+    "falling": dict(causal=True, scale=-0.1),
+}
+
+
+@pytest.mark.parametrize("mask", MASKS)
+@pytest.mark.parametrize("d", [64, 128, 242])
+def test_planes_masks(ops, mask, d):
+    lens = [1100, 999]
+    x, _ = _check(ops, lens, lens, 2, 1, d, torch.float32, tail=(5, 5), **MASKS[mask])
+    assert _on_planes(ops, *x[:3], x[4])
+
+
+@pytest.mark.parametrize("d", [40, 57, 63, 65, 99, 127, 129, 143, 200, 255, 256])
+def test_planes_head_dims(ops, d):
+    lens = [1033, 1, 2100]
+    x, _ = _check(ops, lens, lens, 2, 2, d, torch.float32, seed=3, causal=True)
+    assert _on_planes(ops, *x[:3], x[4])
+
+
+@pytest.mark.parametrize("d", [64, 100, 242])
+def test_planes_few_queries_over_many_keys(ops, d):
+    """rows that see nothing, sequences of no rows, keys shared out: lengths of queries and keys that differ"""
+    x, got = _check(ops, [90, 0, 40, 700], [30, 50, 5000, 3000], 4, 2, d, torch.float32, seed=5, tail=(9, 17), causal=True)
+    out, dq, dk, dv = got
+    assert not out[:60].any() and not dq[:60].any() and not out[830:].any() and not dk[30:80].any() and not dv[8080:].any()
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("d", [64, 128, 242])
+@pytest.mark.parametrize("mask", ["all", "causal", "everything"])
+def test_shares_of_the_keys(ops, dtype, d, mask):
+    """few rows over many keys: each share's sums are joined, in the forward pass and in dk and dv; one of 2 rows over 3"""
+    _check(ops, [17, 2], [2500, 3], 2, 1, d, DT[dtype], seed=7, **MASKS[mask])
+
+
+@pytest.mark.parametrize("dtype", DT)
+def test_shares_of_a_key_tile(ops, dtype):
+    """many query heads on few key heads: dk and dv summed by several workgroups; again and again the same bits"""
+    x, got = _check(ops, [800], [800], 16, 1, 64, DT[dtype], seed=9, causal=True)
+    for _ in range(3):
+        for a, b in zip(got, _run(ops, *x, causal=True)):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("d,lens", [(64, [700, 900]), (128, [700, 900]), (242, [1100, 1300])])
+def test_masked_infinities_stay_out(ops, dtype, d, lens):
+    """NaN and infinities in later tokens and behind the last sequence: rows that do not see them answer as without them"""
+    x = _inputs(lens, lens, 2, 1, d, DT[dtype], 11, (9, 9))
+    q, k, v, do, off, _ = x
+    at, rel = off[1] + 333, 2.0 ** -6 if dtype == "bf16" else 1e-5
+    base = _run(ops, *x, causal=True)
+    for bad in (math.nan, math.inf, -math.inf):
+        q2, k2, v2, do2 = (t.clone() for t in (q, k, v, do))
+        k2[at], v2[at] = bad, bad
+        for t in (q2, k2, v2, do2):
+            t[off[-1]:] = bad
+        got = _run(ops, q2, k2, v2, do2, off, off, causal=True)
+        for g, b in zip(got[:2], base[:2]):
+            assert bool(torch.isfinite(g[:at]).all())
+            torch.testing.assert_close(g[:at].float(), b[:at].float(), rtol=rel, atol=rel * b.float().abs().max().item())
+            assert not g[off[-1]:].any()
+        for g, b in zip(got[2:], base[2:]):
+            torch.testing.assert_close(g[:off[1]].float(), b[:off[1]].float(), rtol=rel, atol=rel * b.float().abs().max().item())
+            assert not g[off[-1]:].any()
+        if math.isnan(bad):
+            assert bool(torch.isnan(got[0][at:off[-1]]).all()) and bool(torch.isnan(got[1][at:off[-1]]).all())
+
+
+@pytest.mark.parametrize("d,n", [(64, 900), (242, 1200)])
+def test_planes_hold_the_largest_numbers(ops, d, n):
+    """values whose upper 8 bits round to infinity: a first token that is seen alone passes its value, the others weigh it"""
+    big = torch.finfo(torch.float32).max
+    q, k, v, do, off, _ = _inputs([n], [n], 2, 2, d, torch.float32, 13)
+    v[0] = big
+    assert _on_planes(ops, q, k, v, off)
+    out = ops.packed_attention(q, k, v, _i32(off), causal=True).double().cpu()
+    assert bool(torch.isfinite(out).all()) and bool((out[0] >= big * (1 - 2.0 ** -21)).all())
+    z = torch.einsum("qhd,hd->qh", q.double().cpu(), k[0].double().cpu()) * d ** -0.5
+    s = torch.einsum("qhd,khd->hqk", q.double().cpu(), k.double().cpu()) * d ** -0.5
+    s = s.masked_fill(~torch.ones(n, n, dtype=torch.bool).tril(), -math.inf)
+    p = torch.exp(z - torch.logsumexp(s, 2).T)                  # of the first token, whose value outweighs all others
+    torch.testing.assert_close(out, (p[..., None] * big).expand_as(out), rtol=1e-5, atol=0)
+
+
+def test_planes_strides(ops):
+    n, d = 1000, 64
+    off = [0, 400, n]
+    qkv, do = _normal(15, n, 8, d), _normal(16, n, 4, d)
+    q, k, v = qkv[:, :4], qkv[:, 4:6], qkv[:, 6:]
+    assert _on_planes(ops, q, k, v, off)
+    want = _run(ops, q.contiguous(), k.contiguous(), v.contiguous(), do, off, off, causal=True)
+    for form in (lambda x: x, lambda x: x.transpose(0, 1).contiguous().transpose(0, 1), lambda x: x.transpose(1, 2).contiguous().transpose(1, 2)):
+        for g, w in zip(_run(ops, form(q), form(k), form(v), form(do), off, off, causal=True), want):
+            assert torch.equal(g, w)
+    odd = [torch.empty(x.shape[0], x.shape[1], d + 3, device="cuda")[..., 1:d + 1].copy_(x) for x in (q, k, v, do)]      # rows at any 4 bytes
+    for g, w in zip(_run(ops, *odd, off, off, causal=True), want):
+        assert torch.equal(g, w)
+
+
+@pytest.mark.parametrize("dtype", DT)
+def test_graphs_with_their_own_workspaces(ops, dtype):
+    """planes and shares of the keys in two captured graphs, replayed side by side with eager calls between"""
+    lens, d = ([600, 500], 64)
+    dt = DT[dtype]
+    offs, offd = _i32(_offsets(lens)), _i32([0, 5, 9])
+
+    def step(q, k, v, do, few):
+        leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+        out = ops.packed_attention(*leaves, offs, causal=True)
+        return [out.detach(), *torch.autograd.grad(out, leaves, do), ops.packed_attention(few, k, v, offd, offs)]
+
+    def fresh(seed):
+        return [_normal(seed + i, n, h, d, dtype=dt) for i, (n, h) in enumerate(((1100, 4), (1100, 2), (1100, 2), (1100, 4), (9, 4)))]
+    side, graphs = torch.cuda.Stream(), []
+    for j in range(2):
+        static = fresh(j)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(*static)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            res = step(*static)
+        graphs.append((g, static, res))
+    for seed in (100, 200, 300):
+        sets = [fresh(seed + 10 * j) for j in range(2)]
+        for (g, static, _), x in zip(graphs, sets):
+            for s, y in zip(static, x):
+                s.copy_(y)
+            g.replay()
+        want = [step(*x) for x in sets]
+        torch.cuda.synchronize()
+        for (_, _, res), w in zip(graphs, want):
+            for a, b in zip(res, w):
+                assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DT)
+def test_one_token_steps_over_a_long_cache(ops, dtype):
+    """the step over a cache and the packed form of the same call: 1 row over all the keys"""
+    dt, lens, hq, hk, d = DT[dtype], [3000, 1, 700], 16, 1, 96
+    cap = 3100
+    q, kc, vc = _normal(1, 3, hq, d, dtype=dt), _normal(2, 3, cap, hk, d, dtype=dt), _normal(3, 3, cap, hk, d, dtype=dt)
+    k, v = (torch.cat([c[i, :n] for i, n in enumerate(lens)]) for c in (kc, vc))
+    (out, tol), *_ = _ref(q, k, v, q, [0, 1, 2, 3], _offsets(lens))
+    for got in (ops.attention_step(q, kc, vc, _i32(lens)), ops.packed_attention(q, k, v, _i32([0, 1, 2, 3]), _i32(_offsets(lens)))):
+        assert (got.double().cpu() - out).norm() <= tol
