@@ -320,19 +320,20 @@ int sttran_roi_align(const float* fmaps, int32_t T, int32_t C, int32_t H, int32_
  * the rounding of out took away).
  * sttran_attention_backward: dq [q_rows, num_q_heads, head_dim], dk, dv [kv_rows, num_kv_heads, head_dim], contiguous, from dout
  * and the forward's inputs, out, out_residual and lse.  Every row is written (zeros where nothing reaches it); the result does
- * not depend on the order of workgroups.  Needs sttran_attention_workspace_bytes(args, 1) bytes of device memory. */
+ * not depend on the order of workgroups.
+ * Each needs sttran_attention_workspace_bytes(args, is it the backward) bytes of device memory, 16-byte aligned (0: none). */
 typedef struct SttranAttention {
   uint32_t struct_size;            /* = sizeof(SttranAttention) */
   int32_t dtype;                   /* STTRAN_DTYPE_F32 / STTRAN_DTYPE_BF16 */
   int32_t num_seq, num_q_heads, num_kv_heads, head_dim;     /* head_dim 1 .. 256 */
-  int64_t q_rows, kv_rows;         /* < 2^31 - 1024 */
+  int64_t q_rows, kv_rows;         /* < 2^31 - 1024, and times their heads < 2^29 */
   const void *q, *k, *v;
   int64_t q_row_stride, q_head_stride, k_row_stride, k_head_stride, v_row_stride, v_head_stride;
   const int32_t *seq_off, *key_off;        /* [num_seq + 1] */
   const int32_t* prefix_len;               /* [num_seq] or NULL: none */
   const float* distance_slope;             /* [num_q_heads] or NULL: none */
   int32_t causal;
-  float score_cap;                         /* 0: none */
+  float score_cap;                         /* 0: none; scale / score_cap must be a number */
   float scale;
   int32_t reserved;
   void *out, *out_residual;                /* contiguous [q_rows, num_q_heads, head_dim]; out_residual may be NULL */

@@ -10,11 +10,16 @@ using namespace sttran;
 namespace {
 
 constexpr int64_t kMaxRows = (int64_t(1) << 31) - 1024, kMaxRowBytes = int64_t(1) << 24, kMaxCacheRowBytes = int64_t(1) << 22;
+constexpr int64_t kMaxHeadRows = int64_t(1) << 29;       // a launch has 8 threads a head's row at most, and fewer than 2^32 of them
 
 bool dtype_ok(int32_t t) { return t == STTRAN_DTYPE_F32 || t == STTRAN_DTYPE_BF16; }
 int elt(int32_t t) { return t == STTRAN_DTYPE_BF16 ? 2 : 4; }
 bool heads_ok(int32_t hq, int32_t hk, int32_t d) { return hq > 0 && hk > 0 && hq <= 4096 && hq % hk == 0 && d > 0 && d <= 256; }
 bool number(float x) { return std::isfinite(x); }
+// the kernels work in base 2 and with scale / cap: those have to be numbers too
+bool score_ok(float scale, float cap) {
+  return number(scale * 1.5f) && number(cap * 3.f) && cap >= 0.f && (cap == 0.f || number(scale / cap * 3.f));
+}
 
 // what divides every address and stride that a call touches, up to 16; 0: something is not even aligned to its element
 struct Alignment {
@@ -41,14 +46,13 @@ bool attention_args(const SttranAttention* a, SeqAttnArgs& A, Alignment& al) {
   if (!a || a->struct_size != sizeof(SttranAttention) || !dtype_ok(a->dtype) || !heads_ok(a->num_q_heads, a->num_kv_heads, a->head_dim))
     return false;
   if (a->num_seq < 0 || a->q_rows < 0 || a->kv_rows < 0 || a->q_rows > kMaxRows || a->kv_rows > kMaxRows) return false;
-  if (!number(a->score_cap) || a->score_cap < 0.f || !number(a->scale)) return false;
+  if (!score_ok(a->scale, a->score_cap)) return false;
   const int es = elt(a->dtype);
   if (!row_stride_ok(a->q_row_stride, es) || !row_stride_ok(a->k_row_stride, es) || !row_stride_ok(a->v_row_stride, es) ||
       !head_stride_ok(a->q_head_stride) || !head_stride_ok(a->k_head_stride) || !head_stride_ok(a->v_head_stride))
     return false;
   if ((a->q_rows > 0 && !a->q) || (a->kv_rows > 0 && (!a->k || !a->v)) || (a->num_seq > 0 && (!a->seq_off || !a->key_off))) return false;
-  // a launch's workgroups: 32 rows at least a workgroup
-  if ((a->q_rows + 31) / 32 * a->num_q_heads >= (int64_t(1) << 31) || (a->kv_rows + 31) / 32 * a->num_kv_heads >= (int64_t(1) << 31)) return false;
+  if (a->q_rows * a->num_q_heads >= kMaxHeadRows || a->kv_rows * a->num_kv_heads >= kMaxHeadRows) return false;
   A.q = (const char*)a->q; A.k = (const char*)a->k; A.v = (const char*)a->v;
   A.q_t = a->q_row_stride * es; A.q_h = a->q_head_stride * es;
   A.k_t = a->k_row_stride * es; A.k_h = a->k_head_stride * es;
@@ -68,7 +72,7 @@ bool step_args(const SttranAttentionStep* a, SeqStepArgs& A) {
   if (!a || a->struct_size != sizeof(SttranAttentionStep) || !dtype_ok(a->dtype) || !heads_ok(a->num_q_heads, a->num_kv_heads, a->head_dim))
     return false;
   if (a->num_seq < 0 || a->num_seq > 65535 || a->capacity < 0 || a->capacity > kMaxRows) return false;
-  if (!number(a->score_cap) || a->score_cap < 0.f || !number(a->scale)) return false;
+  if (!score_ok(a->scale, a->score_cap)) return false;
   const int es = elt(a->dtype);
   if (!row_stride_ok(a->k_row_stride, es, kMaxCacheRowBytes) || !row_stride_ok(a->v_row_stride, es, kMaxCacheRowBytes) || !head_stride_ok(a->q_seq_stride) ||
       !head_stride_ok(a->q_head_stride) || !head_stride_ok(a->k_seq_stride) || !head_stride_ok(a->k_head_stride) ||

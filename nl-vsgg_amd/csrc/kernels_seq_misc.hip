@@ -130,6 +130,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(BWD ? 
 #pragma unroll
         for (int j = 0; j < EPL; ++j) z[j] = y[j ^ 1];
       }
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) z[j] = e0 + j < A.rot ? z[j] : 0.f;             // what passes has no partner, infinities neither
       seq_u32x4 out = {0, 0, 0, 0};
 #pragma unroll
       for (int j = 0; j < EPL; ++j) y[j] = fmaf(z[j], si[j], y[j] * co[j]);

@@ -57,7 +57,6 @@ static int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 // (53, 35); 2 of 200, 1024 rows 275, 263 (42, 54).
 static bool use_planes(int bf16, const SeqAttnArgs& A) {
   if (bf16 || A.nseq <= 0) return false;
-  if ((int64_t)std::max(A.hq, A.hk) * 48 * ((A.d + 7) / 8) > (1 << 24)) return false;      // a tile's rows are addressed in 32 bits
   return A.tk / A.nseq >= (A.d <= 64 ? 256 : A.d <= 128 ? 512 : 1024);
 }
 

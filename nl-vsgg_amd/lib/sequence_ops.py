@@ -8,7 +8,8 @@ bias, capped scores) and for clips that grow token by token.
     out = attention_step(q1, k_cache, v_cache, lengths)              # one new token a sequence
 
 float32 or bfloat16 throughout a call (statistics and sums in float32); tensors on one MI355X, no CPU path.  Work is enqueued
-on the current stream of the tensors' device and may be captured into a graph; nothing is read back.  Bad arguments raise
+on the current stream of the tensors' device and may be captured into a graph; nothing is read back.  (As with every torch
+operator: to capture a backward pass, let the results of eager calls on the same leaves go first.)  Bad arguments raise
 ValueError before anything is launched.  The last dimension of q / k / v must be contiguous (others are copied), other
 strides are free."""
 from __future__ import annotations
@@ -23,7 +24,7 @@ from .. import _native as nat
 
 _DTYPES = {torch.float32: nat.DTYPE_F32, torch.bfloat16: nat.DTYPE_BF16}
 _ATT_SIZE, _STEP_SIZE, _ROT_SIZE = (C.sizeof(t) for t in (nat.SttranAttention, nat.SttranAttentionStep, nat.SttranRotary))
-_MAX_ROW_BYTES, _MAX_CACHE_ROW_BYTES = 1 << 24, 1 << 22
+_MAX_ROW_BYTES, _MAX_CACHE_ROW_BYTES, _MAX_HEAD_ROWS = 1 << 24, 1 << 22, 1 << 29
 
 
 def _launch(fn, args, dev):
@@ -90,6 +91,8 @@ def _score(name, scale, cap, d):
     cap = 0.0 if cap is None else float(cap)
     if not math.isfinite(scale) or not math.isfinite(cap) or cap < 0:
         raise ValueError(f"{name}: scale must be finite and score_cap finite and >= 0 (0: none)")
+    if not max(abs(scale), cap, abs(scale) / cap if cap else 0.0) < 1e38 or (cap and cap < 1e-37):
+        raise ValueError(f"{name}: scale, score_cap and their quotient must fit float32")
     return scale, cap
 
 
@@ -192,6 +195,8 @@ def packed_attention(q, k, v, seq_off, key_off=None, *, causal=False, prefix_len
         if distance_slope.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"{name}: distance_slope is a constant, it gets no gradient")
         distance_slope = _small(name, "distance_slope", distance_slope, torch.float32, (hq,), dev)
+    if max(q.shape[0] * hq, k.shape[0] * k.shape[1]) >= _MAX_HEAD_ROWS:
+        raise ValueError(f"{name}: rows times heads must be below 2^29 a call")
     scale, cap = _score(name, scale, score_cap, q.shape[2])
     q, k, v = _rows(q), _rows(k), _rows(v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):

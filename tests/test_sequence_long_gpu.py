@@ -265,3 +265,35 @@ def test_one_token_steps_over_a_long_cache(ops, dtype):
     (out, tol), *_ = _ref(q, k, v, q, [0, 1, 2, 3], _offsets(lens))
     for got in (ops.attention_step(q, kc, vc, _i32(lens)), ops.packed_attention(q, k, v, _i32([0, 1, 2, 3]), _i32(_offsets(lens)))):
         assert (got.double().cpu() - out).norm() <= tol
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("d,lens", [(64, [20, 50]), (64, [700, 650]), (242, [60, 9]), (128, [600, 800])])
+def test_rows_before_the_first_sequence(ops, dtype, d, lens):
+    """sequences that begin at row 7 answer as they do from row 0, the rows around them are zeros with zero gradients"""
+    n = sum(lens)
+    q, k, v, do = _inputs([n], [n], 2, 2, d, DT[dtype], 17, (19, 19))[:4]
+    off = [7, 7 + lens[0], 7 + n]
+    got = _run(ops, q, k, v, do, off, off, causal=True)
+    want = _run(ops, q[7:7 + n], k[7:7 + n], v[7:7 + n], do[7:7 + n], _offsets(lens), _offsets(lens), causal=True)
+    rel = 2.0 ** -6 if dtype == "bf16" else 1e-5                # tiles begin at other rows: sums in another order
+    for g, w in zip(got, want):
+        assert not g[:7].any() and not g[7 + n:].any()
+        torch.testing.assert_close(g[7:7 + n].float(), w.float(), rtol=rel, atol=rel * w.float().abs().max().item())
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_columns_that_pass_keep_infinities(ops, dtype, interleaved):
+    """a column behind the turned ones passes as it is, next to an infinite one too, forward and backward"""
+    n, d, rot = 6, 64, 48
+    q, k = _normal(1, n, 2, d, dtype=DT[dtype]), _normal(2, n, 1, d, dtype=DT[dtype])
+    q[1, 0, 50], q[2, 1, 63], k[3, 0, 49] = math.inf, -math.inf, math.nan
+    freq, pos = ops.rotary_frequencies(rot, device="cuda"), torch.arange(n, device="cuda")
+    leaves = [x.clone().requires_grad_() for x in (q, k)]
+    out = ops.rotary_qk(*leaves, pos, freq, interleaved=interleaved)
+    back = torch.autograd.grad(out, leaves, [q, k])
+    for x, y, g in zip((q, k), out, back):
+        assert torch.equal(y[..., rot:].nan_to_num(7.0, 8.0, 9.0), x[..., rot:].nan_to_num(7.0, 8.0, 9.0))
+        assert torch.equal(g[..., rot:].nan_to_num(7.0, 8.0, 9.0), x[..., rot:].nan_to_num(7.0, 8.0, 9.0))
+        assert bool(torch.isfinite(y[..., :rot]).all()) and bool(torch.isfinite(g[..., :rot]).all())

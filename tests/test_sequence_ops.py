@@ -102,6 +102,16 @@ def test_dropout_refusals(native, args):
     assert native.load().sttran_dropout_add(*args, None, 0, 0, None, None) == 1
 
 
+@pytest.mark.parametrize("over", [dict(q_rows=1 << 27), dict(kv_rows=1 << 28), dict(scale=3e38), dict(score_cap=2e38), dict(score_cap=1e-39),
+                                  dict(scale=1e20, score_cap=1e-20)])
+def test_attention_refuses_what_it_cannot_count(native, over):
+    """more threads than a launch has, scores whose base-2 factors are infinite"""
+    lib = native.load()
+    a = _attention(native, **over)
+    assert lib.sttran_attention_forward(C.byref(a), None) == 1 and lib.sttran_attention_backward(C.byref(a), None) == 1
+    assert lib.sttran_attention_workspace_bytes(C.byref(a), 0) == 0
+
+
 def test_struct_layouts_match_the_c_header(native, tmp_path):
     import shutil
     import subprocess
