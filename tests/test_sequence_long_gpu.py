@@ -297,3 +297,52 @@ def test_rotary_columns_that_pass_keep_infinities(ops, dtype, interleaved):
         assert torch.equal(y[..., rot:].nan_to_num(7.0, 8.0, 9.0), x[..., rot:].nan_to_num(7.0, 8.0, 9.0))
         assert torch.equal(g[..., rot:].nan_to_num(7.0, 8.0, 9.0), x[..., rot:].nan_to_num(7.0, 8.0, 9.0))
         assert bool(torch.isfinite(y[..., :rot]).all()) and bool(torch.isfinite(g[..., :rot]).all())
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("d,lens", [(64, [50, 90]), (128, [70, 60]), (242, [50, 90]), (64, [700, 650]), (128, [600, 800]), (242, [1100, 1300])])
+def test_gradients_that_are_not_finite_reach_what_they_saw(ops, dtype, d, lens):
+    """an infinite or NaN gradient row reaches the keys its row saw and its own query, nothing else"""
+    x = _inputs(lens, lens, 4, 2, d, DT[dtype], 19)
+    q, k, v, do, off, _ = x
+    at, rel = off[1] + 21, 2.0 ** -6 if dtype == "bf16" else 1e-5
+    base = _run(ops, *x, causal=True)
+    for bad in (math.inf, math.nan):
+        do2 = do.clone()
+        do2[at, 1] = bad                              # query head 1 reads key head 0
+        out, dq, dk, dv = _run(ops, q, k, v, do2, off, off, causal=True)
+        assert torch.equal(out, base[0])
+        rows = [i for i in range(off[-1]) if i != at]
+        for g, b, keep in ((dq, base[1], rows), (dk, base[2], [*range(off[1]), *range(at + 1, off[-1])]), (dv, base[3], [*range(off[1]), *range(at + 1, off[-1])])):
+            torch.testing.assert_close(g[keep].float(), b[keep].float(), rtol=rel, atol=rel * b.float().abs().max().item())
+        assert torch.equal(dk[:, 1], base[2][:, 1]) and torch.equal(dv[:, 1], base[3][:, 1])
+        assert not torch.isfinite(dq[at, 1]).any() and not torch.isfinite(dv[off[1]:at + 1, 0]).any()
+        assert bool(torch.isfinite(dq[at, [0, 2, 3]]).all())
+
+
+@pytest.mark.parametrize("dtype", DT)
+def test_two_threads_on_two_streams(ops, dtype):
+    """calls from two host threads at once, each on its own stream, answer as calls in turn"""
+    import threading
+    sets = [_inputs([300, 333], [300, 333], 4, 2, 64, DT[dtype], 30 + 10 * i) for i in range(2)]
+    want = [_run(ops, *x, causal=True) for x in sets]
+    torch.cuda.synchronize()
+    got, failed = [None, None], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(10):
+                    got[i] = _run(ops, *sets[i], causal=True)
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:                        # shown by the assertion below
+            failed.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    for a, b in zip(got, want):
+        for x, y in zip(a, b):
+            assert torch.equal(x, y)
