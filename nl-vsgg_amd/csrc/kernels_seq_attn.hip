@@ -107,7 +107,7 @@ seq_attn_fwd_kernel(SeqAttnArgs A) {
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int tiles = (A.tq + C::RB - 1) / C::RB;
   const int id = seq_xcd_order(blockIdx.x, gridDim.x);
-  const int head = id / tiles, tile = tiles - 1 - id % tiles;      // rows that see most keys first where the order masks
+  const int head = id / tiles, tile = tiles - 1 - seq_spread_tile(A, id % tiles, tiles, A.hq);      // rows that see most keys first where the order masks
   const int kvh = head / (A.hq / A.hk), dh = w % C::DS;
   const int row0 = tile * C::RB + 32 * (w / C::DS), row = row0 + (lane & 31);
   const int dbytes = C::row_bytes(A.d);
