@@ -97,7 +97,7 @@ struct SeqFwdLds {                                       // DS == 1: two tiles o
   static constexpr int kXch = 2 * kBufs * C::kTileBytes, kRed = kXch, kRefs = kXch + (C::DS > 1 ? C::NW * SeqShare<C, 1>::kWave : 0);
   static constexpr int kBytes = C::DS > 1 ? kRefs + C::NW * 128 : kXch + C::NW * 8;
 };
-template <class C, bool CAP, bool SLOPE>
+template <class C, bool CAP, bool SLOPE, bool TWO>
 __global__ void __launch_bounds__(C::NT) __attribute__((amdgpu_waves_per_eu(2, 2)))
 seq_attn_fwd_kernel(SeqAttnArgs A) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -199,7 +199,7 @@ seq_attn_fwd_kernel(SeqAttnArgs A) {
             s[u][e] = __builtin_amdgcn_exp2f(fmaf(x[16 * u + e], c1, c0));
             l += s[u][e];
           }
-          seq_reduce<C>(acc, vt_lds, u, dh, s[u]);
+          seq_reduce<C, TWO>(acc, vt_lds, u, dh, s[u]);
         }
       }
     } else {
@@ -268,7 +268,7 @@ seq_attn_fwd_kernel(SeqAttnArgs A) {
           part *= own == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(own - mn);
         }
         l += part;
-        seq_reduce<C>(acc, vt_lds, 0, dh, s[0]);
+        seq_reduce<C, TWO>(acc, vt_lds, 0, dh, s[0]);
       }
     }
     if (more) {
@@ -382,12 +382,12 @@ hipError_t launch_seq_attn_join(hipStream_t s, int bf16, const SeqAttnArgs& A, c
   return hipGetLastError();
 }
 
-template <class C, bool CAP, bool SLOPE>
+template <class C, bool CAP, bool SLOPE, bool TWO>
 static hipError_t fwd_as(hipStream_t s, const SeqAttnArgs& A) {
   constexpr int lds = SeqFwdLds<C>::kBytes;
   static_assert(lds <= 160 * 1024, "LDS of a CU");
   static DeviceMarks marks;
-  auto fn = seq_attn_fwd_kernel<C, CAP, SLOPE>;
+  auto fn = seq_attn_fwd_kernel<C, CAP, SLOPE, TWO>;
   hipError_t e = marks.raise_lds(reinterpret_cast<const void*>(fn), lds);
   if (e != hipSuccess) return e;
   const int tiles = (A.tq + C::RB - 1) / C::RB;
@@ -398,20 +398,20 @@ static hipError_t fwd_as(hipStream_t s, const SeqAttnArgs& A) {
 
 // A kernel for each of no cap and cap, no distances and distances: with the others' bodies beside its own in one kernel the registers
 // spill and drain the loads in flight (three sequences of 4000 .. 8000 rows, 128 columns: forward 335 -> 307 us)
-template <class C>
+template <class C, bool TWO = false>
 static hipError_t fwd(hipStream_t s, const SeqAttnArgs& A) {
   const bool slope = A.slope || A.scale <= 0.f;          // without distances their factor is zero
-  if (A.cap > 0.f) return slope ? fwd_as<C, true, true>(s, A) : fwd_as<C, true, false>(s, A);
-  return slope ? fwd_as<C, false, true>(s, A) : fwd_as<C, false, false>(s, A);
+  if (A.cap > 0.f) return slope ? fwd_as<C, true, true, TWO>(s, A) : fwd_as<C, true, false, TWO>(s, A);
+  return slope ? fwd_as<C, false, true, TWO>(s, A) : fwd_as<C, false, false, TWO>(s, A);
 }
 
 // Own rows a workgroup: 128 or (heads of 64 columns, whose calls have small tiles to spare: 84 -> 74 us on 96 sequences of 37 .. 500
 // rows, 263 -> 254 us on three of 4000 .. 8000) 64 where a wave holds whole heads; 32 or 64 where teams of waves share them
-template <class T, bool VEC>
+template <class T, bool VEC, bool TWO>
 static hipError_t pick(hipStream_t s, const SeqAttnArgs& A) {
-  if (A.d <= 64) return fwd<SeqTile<T, 64, 1, 2, 64, VEC>>(s, A);
-  if (A.d <= 128) return fwd<SeqTile<T, 128, 1, 4, sizeof(T) == 2 ? 64 : 32, VEC>>(s, A);
-  return fwd<SeqTile<T, 256, sizeof(T) == 2 ? 2 : 4, 4, 32, VEC>>(s, A);
+  if (A.d <= 64) return fwd<SeqTile<T, 64, 1, 2, 64, VEC>, TWO>(s, A);
+  if (A.d <= 128) return fwd<SeqTile<T, 128, 1, 4, sizeof(T) == 2 ? 64 : 32, VEC>, TWO>(s, A);
+  return fwd<SeqTile<T, 256, sizeof(T) == 2 ? 2 : 4, 4, 32, VEC>, TWO>(s, A);
 }
 static hipError_t pick_planes(hipStream_t s, const SeqAttnArgs& A) {
   if (A.d <= 64) return fwd<SeqTile<float, 64, 1, 4, 32, true, 3>>(s, A);
@@ -423,11 +423,15 @@ int seq_attn_fwd_tile(int bf16, bool planes, int d) {
   return d <= 64 ? 64 : d <= 128 ? 128 : bf16 ? 64 : 32;
 }
 
+// bfloat16 in sequences of fewer than 64 rows on average: probabilities enter the product with 16 bits (TWO; with 8 the result is 1.2 .. 1.4
+// times as far off as its own rounding, with few rows up to 1.48, and dq, dk up to 1.73 through delta).  It costs a third of the products,
+// which such calls hardly wait for (1000 x 32 rows, 8 heads of 64 columns, 43 -> 44 us; 500 x 60, 16 over 4 of 128, 136 -> 145; but three of
+// 4000 .. 8000 rows 305 -> 396).  Rows at odd 2 bytes take 16 bits always.
 hipError_t launch_seq_attn_fwd(hipStream_t s, int bf16, bool planes, const SeqAttnArgs& A) {
   const bool vec = A.aln >= 4;
   if (planes) return pick_planes(s, A);
-  if (bf16) return vec ? pick<__bf16, true>(s, A) : pick<__bf16, false>(s, A);
-  return pick<float, true>(s, A);                       // 4-byte elements are 4-byte aligned
+  if (bf16) return !vec ? pick<__bf16, false, true>(s, A) : seq_fewer_rows(A, 64) ? pick<__bf16, true, true>(s, A) : pick<__bf16, true, false>(s, A);
+  return pick<float, true, false>(s, A);                // 4-byte elements are 4-byte aligned
 }
 
 }  // namespace sttran

@@ -103,7 +103,7 @@ struct SeqDqLds {                                        // as SeqFwdLds, with t
   static constexpr int kXch = kOver ? C::kTileBytes : 2 * kBufs * C::kTileBytes;
   static constexpr int kRed = 2 * kBufs * C::kTileBytes + (kOver ? 0 : kNeed), kBytes = kRed + C::NW * 8;
 };
-template <class C, bool CAP, bool SLOPE>
+template <class C, bool CAP, bool SLOPE, bool TWO>
 __global__ void __launch_bounds__(C::NT) __attribute__((amdgpu_waves_per_eu(2, 2)))
 seq_attn_dq_kernel(SeqAttnArgs A) {
   using T = typename C::E;
@@ -242,7 +242,7 @@ seq_attn_dq_kernel(SeqAttnArgs A) {
         }
         if (!active) continue;
       }
-      seq_reduce<C>(acc, kt_lds, u, dh, dp);
+      seq_reduce<C, TWO>(acc, kt_lds, u, dh, dp);
     }
     if (more) {
       if constexpr (C::DS == 1) seq_tile_done<C>(mk, kn, dbytes);
@@ -319,7 +319,7 @@ struct SeqDkvLds {                                       // tiles, statistics of
   static constexpr int kRed = kXch + (C::DS > 1 ? C::NW * SeqShare<C, 2>::kWave : 0);
   static constexpr int kOwn = (kRed + C::NW * 8 + 15) / 16 * 16, kBytes = kOwn + C::NW * kParked;
 };
-template <class C, bool CAP, bool SLOPE>
+template <class C, bool CAP, bool SLOPE, bool TWO>
 __global__ void __launch_bounds__(C::NT) __attribute__((amdgpu_waves_per_eu(2, 2)))
 seq_attn_dkv_kernel(SeqAttnArgs A) {
   using T = typename C::E;
@@ -505,8 +505,8 @@ seq_attn_dkv_kernel(SeqAttnArgs A) {
             __builtin_amdgcn_sched_barrier(0);
           }
         }
-        seq_reduce<C>(dv, gt_lds, u, dh, s);
-        seq_reduce<C>(dk, qt_lds, u, dh, dp);
+        seq_reduce<C, TWO>(dv, gt_lds, u, dh, s);
+        seq_reduce<C, TWO>(dk, qt_lds, u, dh, dp);
       } else {
         // each wave of the team sums and finishes its share of the block's quads, then all take the whole
         static_assert(C::NSUB == 1, "one pair of blocks is exchanged");
@@ -531,13 +531,13 @@ seq_attn_dkv_kernel(SeqAttnArgs A) {
         if (more) store_stat(st);
         if (active) {
           S::take(dp, xch, w - dh, 1);
-          seq_reduce<C>(dk, qt_lds, u, dh, dp);
+          seq_reduce<C, TWO>(dk, qt_lds, u, dh, dp);
         }
         __syncthreads();                             // q's tile is free
         if (more) seq_tile_move<C>(mq, qt_lds, A.q + head * A.q_h, A.q_t, row, qend, dbytes);
         if (active) {
           S::take(s, xch, w - dh, 0);
-          seq_reduce<C>(dv, gt_lds, u, dh, s);
+          seq_reduce<C, TWO>(dv, gt_lds, u, dh, s);
         }
       }
     }
@@ -591,23 +591,23 @@ __global__ void __launch_bounds__(256) seq_attn_dkv_join_kernel(SeqAttnArgs A, i
     if (u < left) out[u] = (T)x[u];
 }
 
-template <class C, bool CAP, bool SLOPE>
+template <class C, bool CAP, bool SLOPE, bool TWO>
 static hipError_t dq_as(hipStream_t s, const SeqAttnArgs& A) {
   constexpr int lds = SeqDqLds<C>::kBytes;
   static_assert(lds <= 160 * 1024, "LDS of a CU");
   static DeviceMarks marks;
-  auto fn = seq_attn_dq_kernel<C, CAP, SLOPE>;
+  auto fn = seq_attn_dq_kernel<C, CAP, SLOPE, TWO>;
   hipError_t e = marks.raise_lds(reinterpret_cast<const void*>(fn), lds);
   if (e != hipSuccess) return e;
   fn<<<(unsigned)((A.tq + C::RB - 1) / C::RB * A.hq), C::NT, lds, s>>>(A);
   return hipGetLastError();
 }
-template <class C, bool CAP, bool SLOPE>
+template <class C, bool CAP, bool SLOPE, bool TWO>
 static hipError_t dkv_as(hipStream_t s, const SeqAttnArgs& A) {
   constexpr int lds = SeqDkvLds<C>::kBytes;
   static_assert(lds <= 160 * 1024, "LDS of a CU");
   static DeviceMarks marks;
-  auto fn = seq_attn_dkv_kernel<C, CAP, SLOPE>;
+  auto fn = seq_attn_dkv_kernel<C, CAP, SLOPE, TWO>;
   hipError_t e = marks.raise_lds(reinterpret_cast<const void*>(fn), lds);
   if (e != hipSuccess) return e;
   fn<<<dim3((unsigned)((A.tk + C::RB - 1) / C::RB * A.hk), (unsigned)A.splits), C::NT, lds, s>>>(A);
@@ -618,15 +618,15 @@ static hipError_t dkv_as(hipStream_t s, const SeqAttnArgs& A) {
   return hipGetLastError();
 }
 // kernels by cap and distances as in the forward pass (same sequences: dq 440 -> 413 us, dk and dv 1180 -> 850 us)
-template <class C>
+template <class C, bool TWO = false>
 static hipError_t dq(hipStream_t s, const SeqAttnArgs& A) {
-  if (A.cap > 0.f) return A.slope ? dq_as<C, true, true>(s, A) : dq_as<C, true, false>(s, A);
-  return A.slope ? dq_as<C, false, true>(s, A) : dq_as<C, false, false>(s, A);
+  if (A.cap > 0.f) return A.slope ? dq_as<C, true, true, TWO>(s, A) : dq_as<C, true, false, TWO>(s, A);
+  return A.slope ? dq_as<C, false, true, TWO>(s, A) : dq_as<C, false, false, TWO>(s, A);
 }
-template <class C>
+template <class C, bool TWO = false>
 static hipError_t dkv(hipStream_t s, const SeqAttnArgs& A) {
-  if (A.cap > 0.f) return A.slope ? dkv_as<C, true, true>(s, A) : dkv_as<C, true, false>(s, A);
-  return A.slope ? dkv_as<C, false, true>(s, A) : dkv_as<C, false, false>(s, A);
+  if (A.cap > 0.f) return A.slope ? dkv_as<C, true, true, TWO>(s, A) : dkv_as<C, true, false, TWO>(s, A);
+  return A.slope ? dkv_as<C, false, true, TWO>(s, A) : dkv_as<C, false, false, TWO>(s, A);
 }
 template <class T>
 static hipError_t delta(hipStream_t s, const SeqAttnArgs& A) {
@@ -640,19 +640,19 @@ static hipError_t delta(hipStream_t s, const SeqAttnArgs& A) {
   return hipGetLastError();
 }
 
-template <class T, bool VEC>
+template <class T, bool VEC, bool TWO>
 static hipError_t pick_dq(hipStream_t s, const SeqAttnArgs& A) {
-  if (A.d <= 64) return dq<SeqTile<T, 64, 1, 2, 64, VEC>>(s, A);
-  if (A.d <= 128) return dq<SeqTile<T, 128, sizeof(T) == 2 ? 1 : 2, 4, sizeof(T) == 2 ? 64 : 32, VEC>>(s, A);
-  return dq<SeqTile<T, 256, sizeof(T) == 2 ? 2 : 4, 4, 32, VEC>>(s, A);
+  if (A.d <= 64) return dq<SeqTile<T, 64, 1, 2, 64, VEC>, TWO>(s, A);
+  if (A.d <= 128) return dq<SeqTile<T, 128, sizeof(T) == 2 ? 1 : 2, 4, sizeof(T) == 2 ? 64 : 32, VEC>, TWO>(s, A);
+  return dq<SeqTile<T, 256, sizeof(T) == 2 ? 2 : 4, 4, 32, VEC>, sizeof(T) == 2>(s, A);
 }
 // Waves a workgroup with 64 columns: two in bfloat16 (a training step of 96 sequences of 37 .. 500 rows 313 -> 301 us; 64 x 256 rows,
 // 8 heads over 2, 174 -> 164; 1 x 16384 1942 -> 1967), four in fp32 (128 x 128 rows 311 us, with two 372)
-template <class T, bool VEC>
+template <class T, bool VEC, bool TWO>
 static hipError_t pick_dkv(hipStream_t s, const SeqAttnArgs& A) {
-  if (A.d <= 64) return dkv<SeqTile<T, 64, 1, sizeof(T) == 2 ? 2 : 4, 64, VEC>>(s, A);
-  if (A.d <= 128) return dkv<SeqTile<T, 128, sizeof(T) == 2 ? 1 : 2, 4, 32, VEC>>(s, A);
-  return dkv<SeqTile<T, 256, 4, sizeof(T) == 2 ? 4 : 8, 32, VEC>>(s, A);
+  if (A.d <= 64) return dkv<SeqTile<T, 64, 1, sizeof(T) == 2 ? 2 : 4, 64, VEC>, TWO>(s, A);
+  if (A.d <= 128) return dkv<SeqTile<T, 128, sizeof(T) == 2 ? 1 : 2, 4, 32, VEC>, TWO>(s, A);
+  return dkv<SeqTile<T, 256, 4, sizeof(T) == 2 ? 4 : 8, 32, VEC>, sizeof(T) == 2>(s, A);
 }
 static hipError_t pick_dq_planes(hipStream_t s, const SeqAttnArgs& A) {
   if (A.d <= 64) return dq<SeqTile<float, 64, 1, 4, 32, true, 3>>(s, A);
@@ -670,20 +670,25 @@ int seq_attn_dkv_tile(int bf16, bool planes, int d) {
   return d > 128 ? (bf16 ? 32 : 64) : bf16 ? 128 : 64;
 }
 
+// bfloat16 in sequences of fewer than 512 rows on average, or of more than 128 columns: p and ds enter the products with 16 bits (TWO).
+// With 8, dq and dk carry that rounding, the forward pass's (in delta) and the result's own: 1.44 .. 1.49 times the error of the last
+// alone, but up to 1.97 where few terms sum (1 .. 60 rows) and 1.54 with 242 columns; with 16 bits 1.02 .. 1.13.  The price, a training
+// step: 96 sequences of 37 .. 500 rows 285 -> 312 us; 8 x 2048 rows of 242 columns 1972 -> 2048; three of 4000 .. 8000 rows of 128 columns,
+// 1663 -> 1855, keep 8.  Rows at odd 2 bytes take 16 bits always.
 hipError_t launch_seq_attn_bwd(hipStream_t s, int bf16, bool planes, const SeqAttnArgs& A) {
-  const bool vec = A.aln >= 4;
+  const bool vec = A.aln >= 4, two = A.d > 128 || seq_fewer_rows(A, 512);
   if (A.tq > 0) {
     hipError_t e = bf16 ? delta<__bf16>(s, A) : delta<float>(s, A);
     if (e != hipSuccess) return e;
     if (planes) e = pick_dq_planes(s, A);
-    else if (bf16) e = vec ? pick_dq<__bf16, true>(s, A) : pick_dq<__bf16, false>(s, A);
-    else e = pick_dq<float, true>(s, A);                // 4-byte elements are 4-byte aligned
+    else if (bf16) e = !vec ? pick_dq<__bf16, false, true>(s, A) : two ? pick_dq<__bf16, true, true>(s, A) : pick_dq<__bf16, true, false>(s, A);
+    else e = pick_dq<float, true, false>(s, A);                // 4-byte elements are 4-byte aligned
     if (e != hipSuccess) return e;
   }
   if (A.tk == 0) return hipSuccess;
   if (planes) return pick_dkv_planes(s, A);
-  if (bf16) return vec ? pick_dkv<__bf16, true>(s, A) : pick_dkv<__bf16, false>(s, A);
-  return pick_dkv<float, true>(s, A);
+  if (bf16) return !vec ? pick_dkv<__bf16, false, true>(s, A) : two ? pick_dkv<__bf16, true, true>(s, A) : pick_dkv<__bf16, true, false>(s, A);
+  return pick_dkv<float, true, false>(s, A);
 }
 
 }  // namespace sttran

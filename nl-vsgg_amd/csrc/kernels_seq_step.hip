@@ -13,7 +13,7 @@ namespace sttran {
 // Scores of U rows times GT heads are NS = 8 or 16 sums over the LPK lanes of a row.  They are not summed into every lane: at each
 // step of the reduction a lane hands half of its sums to the lane across and keeps the other half, so lane i ends with score i
 // mod NS alone, and bends, biases and exponentiates that one.  A broadcast within the row of 16 lanes gives each probability back.
-// (All lanes on all scores: 283 us where this takes STEP_US on 48 caches of 700 .. 8192 rows, 32 heads over 8, 128 columns.)
+// (All lanes on all scores: 283 us where this takes 172 on 48 caches of 700 .. 8192 rows, 32 heads over 8, 128 columns.)
 template <int LPK, int GT>
 struct SeqStepShape {
   static constexpr int NS = LPK >= 16 && GT > 1 ? 16 : 8, U = NS / GT, KPW = 64 / LPK, NW = 4, STEP = NW * KPW * U;

@@ -226,15 +226,16 @@ __device__ __forceinline__ void seq_scores_parked(seq_f32x16& acc, const char* t
 }
 
 // acc[d][own row] += tile^T . w, w = a score block's registers.  bfloat16: w is rounded to 8 bits of mantissa here, the one
-// rounding of probabilities (or of their derivatives) on the way into the matrix instruction; sums stay in fp32
-template <class C>
+// rounding of probabilities (or of their derivatives) on the way into the matrix instruction -- TWO: what that takes away follows in
+// an instruction of its own, 16 bits in all; sums stay in fp32
+template <class C, bool TWO = false>
 __device__ __forceinline__ void seq_reduce(seq_f32x16 (&acc)[C::NB], const char* tile, int sub, int dh, const seq_f32x16& w) {
   const int lane = threadIdx.x & 63;
   if constexpr (C::ES == 2) {
     const int g = lane >> 4, i = lane & 15, h = g >> 1;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      seq_bf16x8 b[C::PL];
+      seq_bf16x8 b[TWO ? 2 : C::PL];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         if constexpr (C::PL == 3) {
@@ -243,6 +244,7 @@ __device__ __forceinline__ void seq_reduce(seq_f32x16 (&acc)[C::NB], const char*
           b[0][j] = x; b[1][j] = y; b[2][j] = z;
         } else {
           b[0][j] = (__bf16)w[8 * t + j];
+          if constexpr (TWO) b[1][j] = (__bf16)(w[8 * t + j] - (float)b[0][j]);
         }
       }
       const int row0 = 32 * sub + 16 * t + 4 * h + (i >> 2), row1 = row0 + 8;
@@ -265,6 +267,7 @@ __device__ __forceinline__ void seq_reduce(seq_f32x16 (&acc)[C::NB], const char*
                             __builtin_bit_cast(seq_u32x4, b[2]));
         else
           acc[nb] = seq_mma(acc[nb], a[0], __builtin_bit_cast(seq_u32x4, b[0]));
+        if constexpr (TWO) acc[nb] = seq_mma(acc[nb], a[0], __builtin_bit_cast(seq_u32x4, b[1]));
       }
     }
   } else {
@@ -485,6 +488,9 @@ __device__ __forceinline__ float seq_z(const SeqAttnArgs& A, const SeqScore& sc,
   }
   return A.slope ? fmaf(-sc.slope, fabsf((float)(base - key)), s) : s;
 }
+
+// whether sequences have fewer than n rows on average, of queries or of keys
+inline bool seq_fewer_rows(const SeqAttnArgs& A, int64_t n) { return (A.tq < A.tk ? A.tq : A.tk) < n * A.nseq; }
 
 // workgroups of one head's neighbouring tiles on one XCD (they share its L2): blocks are dealt to the 8 XCDs in turn
 __device__ __forceinline__ int seq_xcd_order(int b, int n) {

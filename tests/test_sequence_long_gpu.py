@@ -346,3 +346,16 @@ def test_two_threads_on_two_streams(ops, dtype):
     for a, b in zip(got, want):
         for x, y in zip(a, b):
             assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("d", [64, 96, 128, 131, 242])
+def test_short_bfloat16_sequences_round_once(ops, d):
+    """below 64 rows probabilities and their derivatives enter the products with 16 bits: each is off by 2^-17 of itself, as delta is, a
+    hundredth of the result's own rounding (2^-8 / sqrt(6) of it in its 2-norm); terms that cancel to a tenth bring that to a tenth, and
+    what is off in quadrature to it adds under 1%.  A quarter more than the rounding of the exact result is allowed, rounding each product
+    to 8 bits would take 1.4 times."""
+    lens = [20, 41, 9, 63, 33]
+    x = _inputs(lens, lens, 4, 2, d, torch.bfloat16, 23)
+    for n, g, (r, _) in zip(("out", "dq", "dk", "dv"), _run(ops, *x), _ref(*x)):
+        own = (r.to(torch.bfloat16).double() - r).norm()
+        assert (g.double().cpu() - r).norm() <= 1.25 * own, n
