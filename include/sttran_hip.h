@@ -326,7 +326,7 @@ typedef struct SttranAttention {
   uint32_t struct_size;            /* = sizeof(SttranAttention) */
   int32_t dtype;                   /* STTRAN_DTYPE_F32 / STTRAN_DTYPE_BF16 */
   int32_t num_seq, num_q_heads, num_kv_heads, head_dim;     /* head_dim 1 .. 256 */
-  int64_t q_rows, kv_rows;         /* < 2^31 - 1024, and times their heads < 2^29 */
+  int64_t q_rows, kv_rows;         /* < 2^31 - 1024, and times their heads < 2^29 - 1024 */
   const void *q, *k, *v;
   int64_t q_row_stride, q_head_stride, k_row_stride, k_head_stride, v_row_stride, v_head_stride;
   const int32_t *seq_off, *key_off;        /* [num_seq + 1] */
@@ -350,7 +350,7 @@ int sttran_attention_backward(const SttranAttention* args, void* stream);
 
 /* One new token a sequence: q [num_seq, num_q_heads, head_dim] over the first lengths[s] rows (clamped to capacity) of the caches
  * k / v [num_seq, capacity, num_kv_heads, head_dim]; the token's place is lengths[s] - 1.  Same z as above; length 0 gives zeros.
- * Rows from lengths[s] on are not read.  num_seq <= 65535; a row stride is at most 2^22 bytes.  Workspace: sttran_attention_step_workspace_bytes(args). */
+ * Rows from lengths[s] on are not read.  num_seq <= 65535, capacity <= 2^30; a row stride is at most 2^22 bytes.  Workspace: sttran_attention_step_workspace_bytes(args). */
 typedef struct SttranAttentionStep {
   uint32_t struct_size;            /* = sizeof(SttranAttentionStep) */
   int32_t dtype;

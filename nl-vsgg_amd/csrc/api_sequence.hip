@@ -10,7 +10,8 @@ using namespace sttran;
 namespace {
 
 constexpr int64_t kMaxRows = (int64_t(1) << 31) - 1024, kMaxRowBytes = int64_t(1) << 24, kMaxCacheRowBytes = int64_t(1) << 22;
-constexpr int64_t kMaxHeadRows = int64_t(1) << 29;       // a launch has 8 threads a head's row at most, and fewer than 2^32 of them
+constexpr int64_t kMaxHeadRows = (int64_t(1) << 29) - 1024;  // a launch has 8 threads a head's row at most, and fewer than 2^32 of them
+constexpr int64_t kMaxCapacity = int64_t(1) << 30;            // rows and a chunk of them are counted in 32 bits
 
 bool dtype_ok(int32_t t) { return t == STTRAN_DTYPE_F32 || t == STTRAN_DTYPE_BF16; }
 int elt(int32_t t) { return t == STTRAN_DTYPE_BF16 ? 2 : 4; }
@@ -71,7 +72,7 @@ bool attention_args(const SttranAttention* a, SeqAttnArgs& A, Alignment& al) {
 bool step_args(const SttranAttentionStep* a, SeqStepArgs& A) {
   if (!a || a->struct_size != sizeof(SttranAttentionStep) || !dtype_ok(a->dtype) || !heads_ok(a->num_q_heads, a->num_kv_heads, a->head_dim))
     return false;
-  if (a->num_seq < 0 || a->num_seq > 65535 || a->capacity < 0 || a->capacity > kMaxRows) return false;
+  if (a->num_seq < 0 || a->num_seq > 65535 || a->capacity < 0 || a->capacity > kMaxCapacity) return false;
   if (!score_ok(a->scale, a->score_cap)) return false;
   const int es = elt(a->dtype);
   if (!row_stride_ok(a->k_row_stride, es, kMaxCacheRowBytes) || !row_stride_ok(a->v_row_stride, es, kMaxCacheRowBytes) || !head_stride_ok(a->q_seq_stride) ||

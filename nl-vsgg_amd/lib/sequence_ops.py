@@ -24,7 +24,7 @@ from .. import _native as nat
 
 _DTYPES = {torch.float32: nat.DTYPE_F32, torch.bfloat16: nat.DTYPE_BF16}
 _ATT_SIZE, _STEP_SIZE, _ROT_SIZE = (C.sizeof(t) for t in (nat.SttranAttention, nat.SttranAttentionStep, nat.SttranRotary))
-_MAX_ROW_BYTES, _MAX_CACHE_ROW_BYTES, _MAX_HEAD_ROWS = 1 << 24, 1 << 22, 1 << 29
+_MAX_ROW_BYTES, _MAX_CACHE_ROW_BYTES, _MAX_HEAD_ROWS = 1 << 24, 1 << 22, (1 << 29) - 1024
 
 
 def _launch(fn, args, dev):
@@ -196,7 +196,7 @@ def packed_attention(q, k, v, seq_off, key_off=None, *, causal=False, prefix_len
             raise ValueError(f"{name}: distance_slope is a constant, it gets no gradient")
         distance_slope = _small(name, "distance_slope", distance_slope, torch.float32, (hq,), dev)
     if max(q.shape[0] * hq, k.shape[0] * k.shape[1]) >= _MAX_HEAD_ROWS:
-        raise ValueError(f"{name}: rows times heads must be below 2^29 a call")
+        raise ValueError(f"{name}: rows times heads must be below 2^29 - 1024 a call")
     scale, cap = _score(name, scale, score_cap, q.shape[2])
     q, k, v = _rows(q), _rows(k), _rows(v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
@@ -219,6 +219,8 @@ def attention_step(q, k_cache, v_cache, lengths, *, distance_slope=None, score_c
     n, dev, d = q.shape[0], q.device, q.shape[2]
     if n > 65535:
         raise ValueError(f"{name}: at most 65535 sequences a call")
+    if k_cache.shape[1] > 1 << 30:
+        raise ValueError(f"{name}: at most 2^30 rows a cache")
     if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
         raise ValueError(f"{name} has no gradient: call it under torch.no_grad()")
     lengths = _small(name, "lengths", lengths, torch.int32, (n,), dev)

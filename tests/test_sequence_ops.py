@@ -112,6 +112,14 @@ def test_attention_refuses_what_it_cannot_count(native, over):
     assert lib.sttran_attention_workspace_bytes(C.byref(a), 0) == 0
 
 
+def test_attention_step_refuses_rows_it_cannot_count(native):
+    lib = native.load()
+    a = native.SttranAttentionStep(struct_size=C.sizeof(native.SttranAttentionStep), dtype=3, num_seq=1, num_q_heads=1, num_kv_heads=1, head_dim=2,
+                                   capacity=(1 << 30) + 1, q=4096, k=4096, v=4096, q_seq_stride=2, q_head_stride=2, k_row_stride=2, v_row_stride=2,
+                                   lengths=4096, scale=1.0, out=4096, workspace=4096, workspace_bytes=1 << 40)
+    assert lib.sttran_attention_step(C.byref(a), None) == 1 and lib.sttran_attention_step_workspace_bytes(C.byref(a)) == 0
+
+
 def test_struct_layouts_match_the_c_header(native, tmp_path):
     import shutil
     import subprocess
