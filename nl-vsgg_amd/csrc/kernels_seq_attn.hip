@@ -120,7 +120,7 @@ seq_attn_fwd_kernel(SeqAttnArgs A) {
   const int row0 = tile * C::RB + 32 * (w / C::DS), row = row0 + (lane & 31);
   const int dbytes = C::row_bytes(A.d);
 
-  const SeqRow me = seq_row(A, row);
+  const SeqRow me = seq_row_of_wave(A, row0, row);
   int lo = me.hi > me.lo ? me.lo : INT_MAX, hi = me.hi;
   seq_wave_range(lo, hi);
   const int wlo = lo, whi = hi;                                     // what this wave's rows see

@@ -33,7 +33,7 @@ __global__ void __launch_bounds__(256) seq_attn_delta_kernel(SeqAttnArgs A) {
   if (c) return;
   A.delta[(int64_t)head * A.tq + row] = s;
   if (head == 0) {
-    const SeqRow i = seq_row(A, row);
+    const SeqRow i = seq_row(A, row, seq_find(A.off_q, A.nseq, row));
     A.rows[row] = make_int4(i.lo, i.hi, i.base, 0);
   }
 }
@@ -343,7 +343,7 @@ seq_attn_dkv_kernel(SeqAttnArgs A) {
   // query rows that may see a key of this tile: those of the sequences that the tile touches
   int qbeg = 0, qend = 0;
   {
-    const int s0 = seq_find(A.off_k, A.nseq, first), s1 = min(seq_find(A.off_k, A.nseq, min(first + C::RB, A.tk) - 1), A.nseq - 1);
+    const int s0 = seq_find_wave(A.off_k, A.nseq, first), s1 = min(seq_find_wave(A.off_k, A.nseq, min(first + C::RB, A.tk) - 1), A.nseq - 1);
     if (s0 < A.nseq) {
       qbeg = A.off_q[s0];
       qend = min(max(A.off_q[s1 + 1], 0), A.tq);

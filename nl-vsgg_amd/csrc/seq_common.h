@@ -144,11 +144,22 @@ __device__ __forceinline__ int seq_find(const int* off, int n, int t) {      // 
   }
   return a;
 }
-__device__ __forceinline__ SeqRow seq_row(const SeqAttnArgs& A, int t) {
+// the same for a t that the wave shares, 64 offsets at a time: two dependent loads for 4096 sequences instead of twelve
+__device__ __forceinline__ int seq_find_wave(const int* off, int n, int t) {
+  const int lane = threadIdx.x & 63;
+  int a = 0, b = n;
+  while (a < b) {                                         // the answer is one of a .. b
+    const int step = (b - a + 63) >> 6, at = a + (lane + 1) * step - 1;
+    const uint64_t yes = __ballot(at >= b || off[at + 1] > t);
+    a += (yes ? __builtin_ctzll(yes) : 64) * step;
+    b = min(a + step - 1, b);
+    a = min(a, b);
+  }
+  return a;
+}
+__device__ __forceinline__ SeqRow seq_row(const SeqAttnArgs& A, int t, int s) {         // s: seq_find of t
   SeqRow r{0, 0, 0};
-  if (t >= A.tq) return r;
-  const int s = seq_find(A.off_q, A.nseq, t);
-  if (s >= A.nseq) return r;
+  if (t >= A.tq || s >= A.nseq) return r;
   const int q0 = A.off_q[s], q1 = A.off_q[s + 1];
   if (t < q0) return r;
   const int k0 = min(max(A.off_k[s], 0), A.tk), k1 = min(max(A.off_k[s + 1], k0), A.tk);
@@ -158,6 +169,17 @@ __device__ __forceinline__ SeqRow seq_row(const SeqAttnArgs& A, int t) {
   r.lo = k0; r.hi = k0 + len; r.base = k0 + pos;
   if (len <= 0) r.lo = r.hi = 0;
   return r;
+}
+// row t of the 32 from row0 on that a wave holds
+__device__ __forceinline__ SeqRow seq_row_of_wave(const SeqAttnArgs& A, int row0, int t) {
+  const int s0 = seq_find_wave(A.off_q, A.nseq, row0), at = s0 + 1 + (threadIdx.x & 63);
+  const int o = at <= A.nseq ? A.off_q[at] : 0x7fffffff;
+  const int ends = __popcll(__ballot(o <= row0 + 31));    // sequences that end within these rows
+  int s = s0;
+  if (ends == 64) s = seq_find(A.off_q, A.nseq, t);
+  else
+    for (int j = 0; j < ends; ++j) s += __builtin_amdgcn_readlane(o, j) <= t;
+  return seq_row(A, t, s);
 }
 
 }  // namespace sttran

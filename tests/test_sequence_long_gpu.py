@@ -359,3 +359,29 @@ def test_short_bfloat16_sequences_round_once(ops, d):
     for n, g, (r, _) in zip(("out", "dq", "dk", "dv"), _run(ops, *x), _ref(*x)):
         own = (r.to(torch.bfloat16).double() - r).norm()
         assert (g.double().cpu() - r).norm() <= 1.25 * own, n
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("n,most", [(64, 3), (65, 3), (700, 1), (4097, 2), (300, 40)])
+def test_many_short_sequences(ops, dtype, n, most):
+    """hundreds of sequences of 0 .. `most` rows: more than 64 of them may end within a wave's 32 rows, empty ones among them"""
+    g = torch.Generator().manual_seed(n)
+    lens = torch.randint(0, most + 1, (n,), generator=g).tolist()
+    lens[n // 2:n // 2 + 80] = [0] * len(lens[n // 2:n // 2 + 80])
+    off = _offsets(lens)
+    q, k, v, do = (_normal(40 + i, off[-1] + 3, 2, 64, dtype=DT[dtype]) for i in range(4))
+    out, dq, dk, dv = _run(ops, q, k, v, do, off, off, causal=True)
+    # the same rows by their definition: one softmax over all rows, other sequences' masked
+    seq = torch.repeat_interleave(torch.arange(n), torch.tensor(lens))
+    see = (seq[:, None] == seq[None]).tril()
+    Q, K, V, G = (x[:off[-1]].double().cpu().transpose(0, 1) for x in (q, k, v, do))
+    p = torch.softmax((Q @ K.transpose(1, 2) / 8).masked_fill(~see, -math.inf), -1)
+    dp = G @ V.transpose(1, 2)
+    ds = p * (dp - (G * (p @ V)).sum(-1, keepdim=True)) / 8
+    rel = 2.0 ** -8 if dtype == "bf16" else 4e-6
+    for name, got, want, terms in (("out", out, p @ V, 0.0), ("dv", dv, p.transpose(1, 2) @ G, 0.0),
+                                   ("dq", dq, ds @ K, (p * dp.abs()).norm()), ("dk", dk, ds.transpose(1, 2) @ Q, (p * dp.abs()).norm())):
+        # dq, dk: dp - delta cancels, to zero for a first row, so its terms' rounding counts: 2^-16 of them in bfloat16 (delta's two parts)
+        more = (2.0 ** -16 if dtype == "bf16" else 4e-6) * terms * 8
+        assert (got[:off[-1]].double().cpu().transpose(0, 1) - want).norm() <= rel * want.norm() + more, name
+        assert not got[off[-1]:].any()
