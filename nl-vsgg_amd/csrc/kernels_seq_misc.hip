@@ -13,8 +13,10 @@ namespace sttran {
 // has no exact fraction in 32), then in fp32.  LPR lanes hold one row, 16 bytes each; the halves' partners come through LDS.
 // What bounds it is the bytes in flight, so registers are kept low for more waves: 8 a SIMD forward (110 us at 7), 5 backward (166 us
 // at 4); the rows' next pass fetched ahead cost registers and was slower (135 / 266 us), and so were larger grids.
-// Measured (32768 tokens, 16 + 4 heads of 128 columns, 96 turned, bfloat16, norm): 93 us forward (3.6 TB/s), 150 us backward (3.4 TB/s) and
-// 6 us for the weights' gradients.
+// Non-temporal stores: 249 -> 236 us for both passes by themselves, but the attention that reads the result next loses it (64 x 512 rows,
+// the two together 301 -> 304 us): plain ones.
+// Measured (32768 tokens, 16 + 4 heads of 128 columns, 96 turned, bfloat16, norm): 90 us forward (3.7 TB/s), 147 us backward (3.4 TB/s) and
+// 7 us for the weights' gradients.
 template <class T, int LPR, bool BWD>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(BWD ? 5 : 8, 8))) seq_rotary_kernel(SeqRotaryArgs A, int TT) {
   constexpr int EPL = SeqElt<T>::kPer16, ROWS = 256 / LPR, ROW = LPR * EPL;
@@ -236,6 +238,7 @@ hipError_t launch_seq_rotary_backward(hipStream_t s, int bf16, const SeqRotaryAr
 // (Salmon, Moraes, Dror, Shaw: Parallel random numbers: as easy as 1, 2, 3, SC 2011): block i / 4 has the 128-bit counter
 // (i / 4, offset) under the 64-bit key and gives the words of four elements, so the mask is a function of (key, offset, i) and
 // is never stored.  Bound by memory: x and res in, y out; 10 rounds are 20 wide multiplies for four elements.
+// Measured (22528 x 4096, bfloat16, residual): 104 us forward, 5.3 TB/s, 68 us backward, 5.4: a large copy's rate.
 __device__ __forceinline__ void seq_philox(uint64_t block, uint64_t offset, uint64_t key, uint32_t (&out)[4]) {
   uint32_t x0 = (uint32_t)block, x1 = (uint32_t)(block >> 32), x2 = (uint32_t)offset, x3 = (uint32_t)(offset >> 32);
   uint32_t k0 = (uint32_t)key, k1 = (uint32_t)(key >> 32);
