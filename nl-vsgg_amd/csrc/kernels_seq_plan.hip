@@ -72,8 +72,9 @@ static int fwd_splits(int bf16, bool planes, const SeqAttnArgs& A) {
   return (int)std::max<int64_t>(1, std::min<int64_t>(n, 64));
 }
 // Shares of a key tile's work: none with 1024 workgroups or more (4 a CU: as the order masks, their work differs by up to the whole
-// length), else as many as bring it there, 8 at most, within 512 MB of partial sums.  (A training step with one share and these: one
-// sequence of 4096 rows, 8 heads, 444 -> 379 us; 6 of 4000, 8 heads over 2, 930 -> 807; three of 6000, 8 over 4, 1498 -> 1410.)  A
+// length), else as many as bring it to 1536 (3 x 8000 rows, 8 heads over 2 of 64, 1412 us; to 1024 1502, to 2048 1417), 8 at most, within
+// 512 MB of partial sums.  (A training step with one share and these: one
+// sequence of 4096 rows, 8 heads, 444 -> 379 us; 6 of 4000, 8 heads over 2, 930 -> 756; three of 6000, 8 over 4, 1498 -> 1340.)  A
 // share is 32 tiles at least where every CU has a workgroup anyway: less does not pay for the join (40 of 600 rows, 8 over 4, 364 us in
 // one share, 420 in two), 8 where not.
 static int dkv_splits(int bf16, bool planes, const SeqAttnArgs& A) {
@@ -81,7 +82,7 @@ static int dkv_splits(int bf16, bool planes, const SeqAttnArgs& A) {
   const int64_t wgs = ((int64_t)A.tk + rb - 1) / rb * A.hk, bytes = (int64_t)A.tk * A.hk * A.d * 8;
   if (wgs == 0 || wgs >= 1024) return 1;
   const int64_t work = (int64_t)(A.hq / A.hk) * ((A.tq / (A.nseq > 0 ? A.nseq : 1) + 31) / 32);       // query tiles a key tile sees, about
-  int64_t n = std::min<int64_t>((1024 + wgs - 1) / wgs, 8);
+  int64_t n = std::min<int64_t>((1536 + wgs - 1) / wgs, 8);
   n = std::min<int64_t>(n, work / (wgs >= 256 ? 32 : 8));
   n = std::min<int64_t>(n, (int64_t(512) << 20) / std::max<int64_t>(bytes, 1));
   return (int)std::max<int64_t>(n, 1);
