@@ -323,7 +323,7 @@ struct SeqDkvLds {                                       // tiles, statistics of
 };
 // Four products.  Two accumulators and both stationary operands do not fit the registers, so LDS carries the values' fragments beside the
 // streamed tiles: 40 KB a wave and 32 query rows, 2560 cycles of a CU's LDS for 2048 of its matrix pipes -- the bound.  Measured on the
-// same sequences: 770 us, 690 TFLOP/s, and 28 us to join the shares; 138 us (64 columns, short, 16 bits); 2245 us (fp32 on planes, 242
+// same sequences: 760 us, 700 TFLOP/s, and 41 us to join the shares; 138 us (64 columns, short, 16 bits); 2245 us (fp32 on planes, 242
 // columns).
 template <class C, bool CAP, bool SLOPE, bool TWO>
 __global__ void __launch_bounds__(C::NT) __attribute__((amdgpu_waves_per_eu(2, 2)))
