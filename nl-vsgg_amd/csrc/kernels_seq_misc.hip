@@ -260,9 +260,10 @@ __global__ void __launch_bounds__(256) seq_dropout_kernel(SeqDropoutArgs A) {
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < chunks; i += (int64_t)gridDim.x * 256) {
     const int64_t left = (A.n - i * EPL) * (int64_t)sizeof(T);
     const int valid = left < 16 ? (int)left : 16;
-    const seq_u32x4 x = seq_load16(A.x + i * 16, valid, A.aln);
+    const int aln = valid & 3 ? 2 : A.aln;              // an odd number of 2-byte elements ends within a dword that is not all its own
+    const seq_u32x4 x = seq_load16(A.x + i * 16, valid, aln);
     seq_u32x4 r = {0, 0, 0, 0}, y = {0, 0, 0, 0};
-    if (A.res) r = seq_load16(A.res + i * 16, valid, A.aln);
+    if (A.res) r = seq_load16(A.res + i * 16, valid, aln);
 #pragma unroll
     for (int b = 0; b < EPL / 4; ++b) {
       uint32_t word[4];
@@ -273,7 +274,7 @@ __global__ void __launch_bounds__(256) seq_dropout_kernel(SeqDropoutArgs A) {
         SeqElt<T>::put(y, 4 * b + j, A.res ? SeqElt<T>::get(r, 4 * b + j) + v : v);
       }
     }
-    seq_store16(A.y + i * 16, y, valid, A.aln);
+    seq_store16(A.y + i * 16, y, valid, aln);
   }
   if (A.used && blockIdx.x == 0 && threadIdx.x == 0) { A.used[0] = key; A.used[1] = offset; }
 }

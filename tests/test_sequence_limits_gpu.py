@@ -1,0 +1,48 @@
+"""The sequence operators at the limits of their arguments: what lies beside a buffer, the largest and smallest numbers, the largest calls."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DT = {"f32": torch.float32, "bf16": torch.bfloat16}
+
+
+@pytest.fixture(scope="module")
+def ops():
+    if not torch.cuda.is_available():
+        pytest.skip("needs an MI355X")
+    from nl_vsgg_amd.lib import sequence_ops
+    return sequence_ops
+
+
+@pytest.fixture(scope="module")
+def native(ops):
+    from nl_vsgg_amd import _native
+    return _native
+
+
+def _normal(seed, *shape, dtype=torch.float32):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn(shape, generator=g, dtype=torch.float32).to(dtype).cuda()
+
+
+# ---- dropout -----------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("n", [1, 2, 3, 5, 7, 8, 9, 15, 17, 2047, 2049])
+def test_dropout_leaves_what_lies_behind_its_elements(ops, native, dtype, n):
+    """the C entry on a part of a larger buffer, at an address of 16 bytes' alignment: only its n elements are written"""
+    dt, stream = DT[dtype], torch.cuda.current_stream().cuda_stream
+    x, r = _normal(1, n + 24, dtype=dt), _normal(2, n + 24, dtype=dt)
+    y = torch.full_like(x, 7.0)
+    for at in (8, 0):
+        y.fill_(7.0)
+        rc = native.load().sttran_dropout_add(x[at:].data_ptr(), r[at:].data_ptr(), y[at:].data_ptr(), n, native.DTYPE_BF16 if dtype == "bf16" else native.DTYPE_F32,
+                                              0.25, None, 5, 6, None, stream)
+        assert rc == 0
+        assert bool((y[:at] == 7).all()) and bool((y[at + n:] == 7).all())
+        assert torch.equal(y[at:at + n], ops.dropout_add(x[at:at + n].clone(), r[at:at + n].clone(), p=0.25, seed=5, offset=6))
