@@ -7,6 +7,8 @@
 // fp32) over its rows, and the groups are merged once at the end: no communication inside the loop but the dot products.
 // Measured: 48 caches of 700 .. 8192 rows, 32 heads over 8 of 128 columns, capped, distances, bfloat16: 172 us, 5.2 TB/s, and 7 us to join;
 // one of 2201 rows, 8 heads of 242, fp32: 9 and 5 us.
+#include <algorithm>
+
 #include "kernels_seq.h"
 #include "seq_attn.h"
 
@@ -235,8 +237,8 @@ int seq_step_chunk(int n, int hq, int hk, int capacity) {
   const int grp = hq / hk, gt = grp <= 1 ? 1 : grp <= 2 ? 2 : grp <= 4 ? 4 : 8;
   const int64_t per = (int64_t)n * hk * ((grp + gt - 1) / gt);
   const int64_t want = (per * capacity + 4095) / 4096;
-  const int64_t chunk = (want + 63) / 64 * 64;
-  return (int)(chunk < 192 ? 192 : chunk);
+  const int64_t chunk = std::min<int64_t>((want + 63) / 64 * 64, capacity);       // one cache for thousands of sequences: `want` passes 32 bits
+  return (int)std::max<int64_t>(chunk, 192);
 }
 
 hipError_t launch_seq_step(hipStream_t s, int bf16, const SeqStepArgs& A) {
