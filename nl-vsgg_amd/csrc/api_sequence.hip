@@ -10,7 +10,7 @@ using namespace sttran;
 namespace {
 
 constexpr int64_t kMaxRows = (int64_t(1) << 31) - 1024, kMaxRowBytes = int64_t(1) << 24, kMaxCacheRowBytes = int64_t(1) << 22;
-constexpr int64_t kMaxHeadRows = (int64_t(1) << 29) - 1024;  // a launch has 8 threads a head's row at most, and fewer than 2^32 of them
+constexpr int64_t kMaxHeadRows = (int64_t(1) << 29) - 1024;  // a launch over tiles has 8 threads a head's row at most, and fewer than 2^32 of them
 constexpr int64_t kMaxCapacity = int64_t(1) << 30;            // rows and a chunk of them are counted in 32 bits
 
 bool dtype_ok(int32_t t) { return t == STTRAN_DTYPE_F32 || t == STTRAN_DTYPE_BF16; }

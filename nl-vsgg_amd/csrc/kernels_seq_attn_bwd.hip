@@ -14,27 +14,28 @@
 namespace sttran {
 
 // delta and the rows' key ranges: LPR lanes a (row, head), 16 bytes a lane.  The sums take out in full width: out + what its
-// rounding took (out_lo), because delta's error is common to a whole row of ds
+// rounding took (out_lo), because delta's error is common to a whole row of ds.  Each thread walks on by the grid: 64 lanes for each of
+// 2^26 wide rows would be more threads than a launch may have
 template <class T, int LPR>
 __global__ void __launch_bounds__(256) seq_attn_delta_kernel(SeqAttnArgs A) {
-  const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPR;
-  const int c = threadIdx.x % LPR;
-  if (item >= (int64_t)A.tq * A.hq) return;
-  const int row = (int)(item / A.hq), head = (int)(item % A.hq), dbytes = A.d * (int)sizeof(T);
-  const seq_u32x4 g = seq_row_chunk(A.raw[3].p + row * A.raw[3].t + head * A.raw[3].h, c, dbytes, A.aln);
-  const seq_u32x4 o = seq_row_chunk(A.out + item * dbytes, c, dbytes, A.aln);
-  seq_u32x4 r = {0, 0, 0, 0};
-  if (A.out_lo) r = seq_row_chunk(A.out_lo + item * dbytes, c, dbytes, A.aln);
-  float s = 0.f;
+  const int c = threadIdx.x % LPR, dbytes = A.d * (int)sizeof(T);
+  const int64_t items = (int64_t)A.tq * A.hq, step = (int64_t)gridDim.x * (256 / LPR);
+  for (int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPR; item < items; item += step) {
+    const int row = (int)(item / A.hq), head = (int)(item % A.hq);
+    const seq_u32x4 g = seq_row_chunk(A.raw[3].p + row * A.raw[3].t + head * A.raw[3].h, c, dbytes, A.aln);
+    const seq_u32x4 o = seq_row_chunk(A.out + item * dbytes, c, dbytes, A.aln);
+    seq_u32x4 r = {0, 0, 0, 0};
+    if (A.out_lo) r = seq_row_chunk(A.out_lo + item * dbytes, c, dbytes, A.aln);
+    float s = 0.f;
 #pragma unroll
-  for (int i = 0; i < SeqElt<T>::kPer16; ++i)
-    s = fmaf(SeqElt<T>::get(g, i), SeqElt<T>::get(o, i) + (sizeof(T) == 2 ? SeqElt<T>::get(r, i) : 0.f), s);
-  s = seq_group_sum<LPR>(s);
-  if (c) return;
-  A.delta[(int64_t)head * A.tq + row] = s;
-  if (head == 0) {
-    const SeqRow i = seq_row(A, row, seq_find(A.off_q, A.nseq, row));
-    A.rows[row] = make_int4(i.lo, i.hi, i.base, 0);
+    for (int i = 0; i < SeqElt<T>::kPer16; ++i)
+      s = fmaf(SeqElt<T>::get(g, i), SeqElt<T>::get(o, i) + (sizeof(T) == 2 ? SeqElt<T>::get(r, i) : 0.f), s);
+    s = seq_group_sum<LPR>(s);
+    if (c == 0) A.delta[(int64_t)head * A.tq + row] = s;
+    if (c == 0 && head == 0) {
+      const SeqRow i = seq_row(A, row, seq_find(A.off_q, A.nseq, row));
+      A.rows[row] = make_int4(i.lo, i.hi, i.base, 0);
+    }
   }
 }
 
@@ -638,7 +639,7 @@ template <class T>
 static hipError_t delta(hipStream_t s, const SeqAttnArgs& A) {
   const int chunks = (A.d * (int)sizeof(T) + 15) / 16;
   const int64_t items = (int64_t)A.tq * A.hq;
-  const auto grid = [&](int lpr) { return (unsigned)((items * lpr + 255) / 256); };
+  const auto grid = [&](int lpr) { return (unsigned)std::min<int64_t>((items * lpr + 255) / 256, 1 << 23); };       // 2^31 threads at most
   if (chunks <= 8) seq_attn_delta_kernel<T, 8><<<grid(8), 256, 0, s>>>(A);
   else if (chunks <= 16) seq_attn_delta_kernel<T, 16><<<grid(16), 256, 0, s>>>(A);
   else if (chunks <= 32) seq_attn_delta_kernel<T, 32><<<grid(32), 256, 0, s>>>(A);

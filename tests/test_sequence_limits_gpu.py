@@ -46,3 +46,33 @@ def test_dropout_leaves_what_lies_behind_its_elements(ops, native, dtype, n):
         assert rc == 0
         assert bool((y[:at] == 7).all()) and bool((y[at + n:] == 7).all())
         assert torch.equal(y[at:at + n], ops.dropout_add(x[at:at + n].clone(), r[at:at + n].clone(), p=0.25, seed=5, offset=6))
+
+
+# ---- attention ---------------------------------------------------------------------------------------------------------
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def _run(ops, q, k, v, do, off_q, off_k, **kw):
+    leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+    out = ops.packed_attention(*leaves, _i32(off_q), _i32(off_k), **kw)
+    return [out.detach(), *torch.autograd.grad(out, leaves, do)]
+
+
+@pytest.mark.parametrize("dtype,d,rows", [("f32", 129, (1 << 26) + 3), ("bf16", 66, (1 << 28) + 5)])
+def test_attention_gradients_of_the_most_rows(ops, dtype, d, rows):
+    """a row for each of more lanes than a launch has threads: queries and gradient broadcast over the rows, the last 50 see 40 keys and
+    answer as by themselves (their tiles begin elsewhere: sums in another order, 2^-6 of the largest in bfloat16, 1e-5 in float32)"""
+    n, nk, dt = 50, 40, DT[dtype]
+    if torch.cuda.mem_get_info()[0] < 150 << 30:
+        pytest.skip("needs 150 GB of device memory")
+    q, do, k, v = (_normal(i, m, 1, d, dtype=dt) for i, m in enumerate((1, 1, nk, nk)))
+    small = _run(ops, q.expand(n, 1, d), k, v, do.expand(n, 1, d), [0, n], [0, nk], causal=True)
+    got = _run(ops, q.expand(rows, 1, d), k, v, do.expand(rows, 1, d), [0, rows - n, rows], [0, 0, nk], causal=True)
+    rel = 2.0 ** -6 if dtype == "bf16" else 1e-5
+    for g, w in zip((got[0][-n:], got[1][-n:], got[2], got[3]), small):
+        torch.testing.assert_close(g.float(), w.float(), rtol=rel, atol=rel * w.float().abs().max().item())
+    for g in got[:2]:
+        assert not g[:rows - n].any()
