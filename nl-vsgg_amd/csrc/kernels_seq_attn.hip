@@ -23,7 +23,7 @@ __device__ __forceinline__ void seq_attn_fwd_again(const SeqAttnArgs& A, const S
     for (int key = lo; key < hi; ++key) {
       const SeqSpread k = seq_spread<T>(A.raw[1].p + kvh * A.raw[1].h + (int64_t)key * A.raw[1].t, A.d);
       const SeqSpread v = seq_spread<T>(A.raw[2].p + kvh * A.raw[2].h + (int64_t)key * A.raw[2].t, A.d);
-      const float z = seq_z<T>(A, sc, seq_spread_dot(q, k), base, key, unused);
+      const float z = seq_z(A, sc, seq_spread_dot(q, k), base, key, unused);
       const float mn = fmaxf(m, z), ms = mn == -INFINITY ? 0.f : mn, al = __builtin_amdgcn_exp2f(m - ms), p = __builtin_amdgcn_exp2f(z - ms);
       l = fmaf(l, al, p);
 #pragma unroll
@@ -50,22 +50,21 @@ __device__ __forceinline__ void seq_attn_fwd_again(const SeqAttnArgs& A, const S
 // common factor exactly as the textbook form does.
 // N scores of one row, x[i] of key k0 + 8 (i / 4) + i % 4, become what z is linear in -- z = c1 * x + c0 -- so that one fma stands
 // before the exponential; hidden ones become -inf (c1 > 0); returns the largest z.  SLOPE: distances, or a scale that is not positive.
-//   neither: the products;  CAP alone (bfloat16): -1 / (1 + e^(2 products)), z = cap - 2 cap / (1 + ..);  else: z itself
-template <class C, bool CAP, bool SLOPE, int N>
+//   neither: the products;  kSeqCapNear alone: -1 / (1 + e^(2 products)), z = cap - 2 cap / (1 + ..);  else: z itself
+template <class C, int CAP, bool SLOPE, int N>
 __device__ __forceinline__ float seq_bend(const SeqAttnArgs& A, const SeqScore& sc, float (&x)[N], int k0, int base, bool full, int lo, int hi,
                                           float& c1, float& c0) {
-  using T = typename C::E;
-  if constexpr (!CAP && !SLOPE) {
+  if constexpr (CAP == kSeqCapNone && !SLOPE) {
     c1 = sc.mul; c0 = 0.f;
-  } else if constexpr (C::OS == 2 && CAP && !SLOPE) {
+  } else if constexpr (CAP == kSeqCapNear && !SLOPE) {
     c1 = 2.f * sc.capl; c0 = sc.capl;
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = -__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x[i] * (sc.mul * (2.f * kSeqLog2e))));
   } else {
     c1 = 1.f; c0 = 0.f;
-    if constexpr (CAP) {
+    if constexpr (CAP != kSeqCapNone) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) x[i] = sc.capl * seq_tanh<T>(x[i] * sc.mul);
+      for (int i = 0; i < N; ++i) x[i] = sc.capl * seq_tanh<CAP == kSeqCapNear>(x[i] * sc.mul);
     } else {
 #pragma unroll
       for (int i = 0; i < N; ++i) x[i] *= sc.mul;
@@ -105,7 +104,7 @@ struct SeqFwdLds {                                       // DS == 1: two tiles o
 //   four of 1800 .. 2240 rows, 8 heads of 242, distances, fp32 on planes: 1240 us (six products for one);  1024 of 5 .. 35, 8 of 242, fp32
 //   instructions: 255 us, 2.5 TB/s
 // 32 own rows a wave: the stationary operand stays in registers, so every value read from LDS serves 32 rows.
-template <class C, bool CAP, bool SLOPE, bool TWO>
+template <class C, int CAP, bool SLOPE, bool TWO>
 __global__ void __launch_bounds__(C::NT) __attribute__((amdgpu_waves_per_eu(2, 2)))
 seq_attn_fwd_kernel(SeqAttnArgs A) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -390,7 +389,7 @@ hipError_t launch_seq_attn_join(hipStream_t s, int bf16, const SeqAttnArgs& A, c
   return hipGetLastError();
 }
 
-template <class C, bool CAP, bool SLOPE, bool TWO>
+template <class C, int CAP, bool SLOPE, bool TWO>
 static hipError_t fwd_as(hipStream_t s, const SeqAttnArgs& A) {
   constexpr int lds = SeqFwdLds<C>::kBytes;
   static_assert(lds <= 160 * 1024, "LDS of a CU");
@@ -405,12 +404,17 @@ static hipError_t fwd_as(hipStream_t s, const SeqAttnArgs& A) {
 }
 
 // A kernel for each of no cap and cap, no distances and distances: with the others' bodies beside its own in one kernel the registers
-// spill and drain the loads in flight (three sequences of 4000 .. 8000 rows, 128 columns: forward 335 -> 307 us)
+// spill and drain the loads in flight (three sequences of 4000 .. 8000 rows, 128 columns: forward 335 -> 307 us).  bfloat16 under a large
+// cap, which bends hardly a score, has one: with distances, whose factor may be zero, and probabilities of 16 bits
 template <class C, bool TWO = false>
 static hipError_t fwd(hipStream_t s, const SeqAttnArgs& A) {
   const bool slope = A.slope || A.scale <= 0.f;          // without distances their factor is zero
-  if (A.cap > 0.f) return slope ? fwd_as<C, true, true, TWO>(s, A) : fwd_as<C, true, false, TWO>(s, A);
-  return slope ? fwd_as<C, false, true, TWO>(s, A) : fwd_as<C, false, false, TWO>(s, A);
+  if constexpr (C::OS == 2) {
+    if (A.cap > kSeqNearCap) return fwd_as<C, kSeqCap, true, true>(s, A);
+  }
+  constexpr int cap = C::OS == 2 ? kSeqCapNear : kSeqCap;
+  if (A.cap > 0.f) return slope ? fwd_as<C, cap, true, TWO>(s, A) : fwd_as<C, cap, false, TWO>(s, A);
+  return slope ? fwd_as<C, kSeqCapNone, true, TWO>(s, A) : fwd_as<C, kSeqCapNone, false, TWO>(s, A);
 }
 
 // Own rows a workgroup: 128 or (heads of 64 columns, whose calls have small tiles to spare: 84 -> 74 us on 96 sequences of 37 .. 500

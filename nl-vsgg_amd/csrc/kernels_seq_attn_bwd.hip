@@ -40,11 +40,11 @@ __global__ void __launch_bounds__(256) seq_attn_delta_kernel(SeqAttnArgs A) {
 }
 
 // p and ds of one pair from its products (s = q.k, dp = dout.v); hidden pairs become exact zeros in both
-template <class T, bool CAP, bool SLOPE>
+template <int CAP, bool SLOPE>
 __device__ __forceinline__ void seq_pair(const SeqScore& sc, float& s, float& dp, bool seen, float lse, float delta, int away) {
   float z, bend = 1.f;
-  if constexpr (CAP) {
-    const float t = seq_tanh<T>(s * sc.mul);
+  if constexpr (CAP != kSeqCapNone) {
+    const float t = seq_tanh<CAP == kSeqCapNear>(s * sc.mul);
     bend = 1.f - t * t;
     z = fmaf(sc.capl, t, -lse);
   } else {
@@ -53,19 +53,18 @@ __device__ __forceinline__ void seq_pair(const SeqScore& sc, float& s, float& dp
   if constexpr (SLOPE) z = fmaf(-sc.slope, fabsf((float)away), z);
   const float p = __builtin_amdgcn_exp2f(z);
   dp = (dp - delta) * p;
-  if constexpr (CAP) dp *= bend;
+  if constexpr (CAP != kSeqCapNone) dp *= bend;
   s = seen ? p : 0.f;
   dp = seen ? dp : 0.f;
 }
-template <class T>
 __device__ __forceinline__ void seq_pair_any(const SeqAttnArgs& A, const SeqScore& sc, float& s, float& dp, bool seen, float lse, float delta,
                                              int away) {
   if (A.cap > 0.f) {
-    if (A.slope) seq_pair<T, true, true>(sc, s, dp, seen, lse, delta, away);
-    else seq_pair<T, true, false>(sc, s, dp, seen, lse, delta, away);
+    if (A.slope) seq_pair<kSeqCap, true>(sc, s, dp, seen, lse, delta, away);
+    else seq_pair<kSeqCap, false>(sc, s, dp, seen, lse, delta, away);
   } else {
-    if (A.slope) seq_pair<T, false, true>(sc, s, dp, seen, lse, delta, away);
-    else seq_pair<T, false, false>(sc, s, dp, seen, lse, delta, away);
+    if (A.slope) seq_pair<kSeqCapNone, true>(sc, s, dp, seen, lse, delta, away);
+    else seq_pair<kSeqCapNone, false>(sc, s, dp, seen, lse, delta, away);
   }
 }
 // ---- dq: own rows = queries, keys and values stream ---------------------------------------------------------------------
@@ -87,7 +86,7 @@ __device__ __forceinline__ void seq_attn_dq_again(const SeqAttnArgs& A, const Se
       const SeqSpread k = seq_spread<T>(A.raw[1].p + kvh * A.raw[1].h + (int64_t)key * A.raw[1].t, A.d);
       const SeqSpread v = seq_spread<T>(A.raw[2].p + kvh * A.raw[2].h + (int64_t)key * A.raw[2].t, A.d);
       float s = seq_spread_dot(q, k), dp = seq_spread_dot(g, v);
-      seq_pair_any<T>(A, sc, s, dp, true, lse, delta, base - key);
+      seq_pair_any(A, sc, s, dp, true, lse, delta, base - key);
 #pragma unroll
       for (int u = 0; u < 4; ++u) o[u] = fmaf(dp, k.x[u], o[u]);
     }
@@ -106,10 +105,9 @@ struct SeqDqLds {                                        // as SeqFwdLds, with t
 };
 // Three products, bound as the forward pass.  Measured on the same sequences as there: 412 us, 960 TFLOP/s (bfloat16, 128 columns);
 // 77 us (64 columns, short, ds with 16 bits); 1615 us (fp32 on planes, 242 columns).
-template <class C, bool CAP, bool SLOPE, bool TWO>
+template <class C, int CAP, bool SLOPE, bool TWO>
 __global__ void __launch_bounds__(C::NT) __attribute__((amdgpu_waves_per_eu(2, 2)))
 seq_attn_dq_kernel(SeqAttnArgs A) {
-  using T = typename C::E;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   char* xch = smem + SeqDqLds<C>::kXch;
   int* red = reinterpret_cast<int*>(smem + SeqDqLds<C>::kRed);
@@ -208,7 +206,7 @@ seq_attn_dq_kernel(SeqAttnArgs A) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           float x = s[e], y = dp[e];
-          seq_pair<T, CAP, SLOPE>(sc, x, y, true, lse, delta, me.base - kb - 4 * h - 8 * (e >> 2) - (e & 3));
+          seq_pair<CAP, SLOPE>(sc, x, y, true, lse, delta, me.base - kb - 4 * h - 8 * (e >> 2) - (e & 3));
           dp[e] = y;
         }
         if (!full) {
@@ -231,7 +229,7 @@ seq_attn_dq_kernel(SeqAttnArgs A) {
             for (int e = 0; e < 4; ++e) {
               const int key = kb + 8 * g + 4 * h + e;
               float x = a[e], y = b[e];
-              seq_pair<T, CAP, SLOPE>(sc, x, y, full || (key >= me.lo && key < me.hi), lse, delta, me.base - key);
+              seq_pair<CAP, SLOPE>(sc, x, y, full || (key >= me.lo && key < me.hi), lse, delta, me.base - key);
               b[e] = y;
             }
             S::leave(b, xch, w - dh, dh, 1, i);
@@ -291,7 +289,7 @@ __device__ __forceinline__ void seq_attn_dkv_again(const SeqAttnArgs& A, uint32_
         const SeqSpread q = seq_spread<T>(A.raw[0].p + head * A.raw[0].h + (int64_t)row * A.raw[0].t, A.d);
         const SeqSpread o = seq_spread<T>(A.raw[3].p + head * A.raw[3].h + (int64_t)row * A.raw[3].t, A.d);
         float s = seq_spread_dot(q, k), dp = seq_spread_dot(o, v);
-        seq_pair_any<T>(A, sc, s, dp, true, A.lse[(int64_t)head * A.tq + row], A.delta[(int64_t)head * A.tq + row], r.z - key);
+        seq_pair_any(A, sc, s, dp, true, A.lse[(int64_t)head * A.tq + row], A.delta[(int64_t)head * A.tq + row], r.z - key);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           dk[u] = fmaf(dp, q.x[u], dk[u]);
@@ -326,10 +324,9 @@ struct SeqDkvLds {                                       // tiles, statistics of
 // streamed tiles: 40 KB a wave and 32 query rows, 2560 cycles of a CU's LDS for 2048 of its matrix pipes -- the bound.  Measured on the
 // same sequences: 760 us, 700 TFLOP/s, and 41 us to join the shares; 138 us (64 columns, short, 16 bits); 2245 us (fp32 on planes, 242
 // columns).
-template <class C, bool CAP, bool SLOPE, bool TWO>
+template <class C, int CAP, bool SLOPE, bool TWO>
 __global__ void __launch_bounds__(C::NT) __attribute__((amdgpu_waves_per_eu(2, 2)))
 seq_attn_dkv_kernel(SeqAttnArgs A) {
-  using T = typename C::E;
   using L = SeqDkvLds<C>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   char* xch = smem + L::kXch;
@@ -455,7 +452,7 @@ seq_attn_dkv_kernel(SeqAttnArgs A) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float x = s4[i], y = p4[i];
-        seq_pair<T, CAP, SLOPE>(sc, x, y, true, l4[i], d4[i], ba[i] - key);
+        seq_pair<CAP, SLOPE>(sc, x, y, true, l4[i], d4[i], ba[i] - key);
         s4[i] = x; p4[i] = y;
       }
     };
@@ -598,7 +595,7 @@ __global__ void __launch_bounds__(256) seq_attn_dkv_join_kernel(SeqAttnArgs A, i
     if (u < left) out[u] = (T)x[u];
 }
 
-template <class C, bool CAP, bool SLOPE, bool TWO>
+template <class C, int CAP, bool SLOPE, bool TWO>
 static hipError_t dq_as(hipStream_t s, const SeqAttnArgs& A) {
   constexpr int lds = SeqDqLds<C>::kBytes;
   static_assert(lds <= 160 * 1024, "LDS of a CU");
@@ -609,7 +606,7 @@ static hipError_t dq_as(hipStream_t s, const SeqAttnArgs& A) {
   fn<<<(unsigned)((A.tq + C::RB - 1) / C::RB * A.hq), C::NT, lds, s>>>(A);
   return hipGetLastError();
 }
-template <class C, bool CAP, bool SLOPE, bool TWO>
+template <class C, int CAP, bool SLOPE, bool TWO>
 static hipError_t dkv_as(hipStream_t s, const SeqAttnArgs& A) {
   constexpr int lds = SeqDkvLds<C>::kBytes;
   static_assert(lds <= 160 * 1024, "LDS of a CU");
@@ -627,13 +624,21 @@ static hipError_t dkv_as(hipStream_t s, const SeqAttnArgs& A) {
 // kernels by cap and distances as in the forward pass (same sequences: dq 440 -> 413 us, dk and dv 1180 -> 850 us)
 template <class C, bool TWO = false>
 static hipError_t dq(hipStream_t s, const SeqAttnArgs& A) {
-  if (A.cap > 0.f) return A.slope ? dq_as<C, true, true, TWO>(s, A) : dq_as<C, true, false, TWO>(s, A);
-  return A.slope ? dq_as<C, false, true, TWO>(s, A) : dq_as<C, false, false, TWO>(s, A);
+  if constexpr (C::OS == 2) {
+    if (A.cap > kSeqNearCap) return dq_as<C, kSeqCap, true, true>(s, A);
+  }
+  constexpr int cap = C::OS == 2 ? kSeqCapNear : kSeqCap;
+  if (A.cap > 0.f) return A.slope ? dq_as<C, cap, true, TWO>(s, A) : dq_as<C, cap, false, TWO>(s, A);
+  return A.slope ? dq_as<C, kSeqCapNone, true, TWO>(s, A) : dq_as<C, kSeqCapNone, false, TWO>(s, A);
 }
 template <class C, bool TWO = false>
 static hipError_t dkv(hipStream_t s, const SeqAttnArgs& A) {
-  if (A.cap > 0.f) return A.slope ? dkv_as<C, true, true, TWO>(s, A) : dkv_as<C, true, false, TWO>(s, A);
-  return A.slope ? dkv_as<C, false, true, TWO>(s, A) : dkv_as<C, false, false, TWO>(s, A);
+  if constexpr (C::OS == 2) {
+    if (A.cap > kSeqNearCap) return dkv_as<C, kSeqCap, true, true>(s, A);
+  }
+  constexpr int cap = C::OS == 2 ? kSeqCapNear : kSeqCap;
+  if (A.cap > 0.f) return A.slope ? dkv_as<C, cap, true, TWO>(s, A) : dkv_as<C, cap, false, TWO>(s, A);
+  return A.slope ? dkv_as<C, kSeqCapNone, true, TWO>(s, A) : dkv_as<C, kSeqCapNone, false, TWO>(s, A);
 }
 template <class T>
 static hipError_t delta(hipStream_t s, const SeqAttnArgs& A) {

@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(256) seq_step_kernel(SeqStepArgs A) {
     if constexpr (LPK >= 64) s = seq_add32(s);
     const int key = k0 + (my_u * NW + w) * KPW + kg;
     s *= mul;
-    if (A.cap > 0.f) s = capl * seq_tanh<T>(s);
+    if (A.cap > 0.f) s = capl * seq_tanh<false>(s);
     s = key < end ? fmaf(-slope, (float)(len - 1 - key), s) : -INFINITY;
     const float mn = fmaxf(m, seq_same_head<LPK, GT>(s, [](float a, float b) { return fmaxf(a, b); }));
     const float ms = mn == -INFINITY ? 0.f : mn, al = __builtin_amdgcn_exp2f(m - ms), p = __builtin_amdgcn_exp2f(s - ms);

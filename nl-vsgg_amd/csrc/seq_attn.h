@@ -457,13 +457,18 @@ struct SeqScore {
   __device__ __forceinline__ SeqScore(const SeqAttnArgs& A, int head)
       : mul(A.cap > 0.f ? A.scale / A.cap : A.scale * kSeqLog2e), capl(A.cap * kSeqLog2e), slope(A.slope ? A.slope[head] * kSeqLog2e : 0.f) {}
 };
-// Without branches.  bfloat16: 1 - 2 / (1 + e^2x), absolute error about 1e-7, times a cap of some tens far below the rounding of the
-// scores' inputs.  fp32: that form from |x| = 0.55 on (where it is good to 3 * 2^-24 of itself), below it the Taylor series up to
-// x^15 (its next term is under 2^-24 of x there)
-template <class T>
+// How a kernel bends its scores: not at all, by tanh with an absolute error of some 2^-23 (kSeqCapNear), or with a relative one (kSeqCap).
+// bfloat16 takes the first of the two up to a cap of kSeqNearCap, where what it is off by, times the cap, is 2e-4 of a probability at
+// most (256 scores of unit variance: 5e-5 in the 2-norm), against 2^-8 = 4e-3 for the result's own rounding.  Beyond, it would take
+// the scores with it -- 4e-4 at a cap of 1e4, 5 % at 1e6, one value for all of them at 1e9 -- and float32 has no such room.
+constexpr int kSeqCapNone = 0, kSeqCapNear = 1, kSeqCap = 2;
+constexpr float kSeqNearCap = 1024.f;
+// Without branches.  NEAR: 1 - 2 / (1 + e^2x), absolute error about 1.2e-7.  Else that form from |x| = 0.55 on (where it is good to
+// 3 * 2^-24 of itself), below it the Taylor series up to x^15 (its next term is under 2^-24 of x there)
+template <bool NEAR>
 __device__ __forceinline__ float seq_tanh(float x) {
-  const float big = 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f((sizeof(T) == 4 ? fabsf(x) : x) * (2.f * kSeqLog2e)));
-  if constexpr (sizeof(T) == 2) return big;
+  const float big = 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f((NEAR ? x : fabsf(x)) * (2.f * kSeqLog2e)));
+  if constexpr (NEAR) return big;
   const float y = x * x;
   float p = -929569.f / 638512875.f;
   p = fmaf(p, y, 21844.f / 6081075.f);
@@ -476,11 +481,10 @@ __device__ __forceinline__ float seq_tanh(float x) {
   return fabsf(x) < 0.55f ? small : copysignf(big, x);
 }
 // one pair's z from its scaled-less product; slope_z = dz / d(scale * product) where a cap bends it
-template <class T>
 __device__ __forceinline__ float seq_z(const SeqAttnArgs& A, const SeqScore& sc, float s, int base, int key, float& slope_z) {
   slope_z = 1.f;
   if (A.cap > 0.f) {
-    const float t = seq_tanh<T>(s * sc.mul);
+    const float t = seq_tanh<false>(s * sc.mul);
     slope_z = 1.f - t * t;
     s = sc.capl * t;
   } else {

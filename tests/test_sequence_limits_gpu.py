@@ -1,8 +1,14 @@
-"""The sequence operators at the limits of their arguments: what lies beside a buffer, the largest and smallest numbers, the largest calls."""
-import ctypes
+"""The sequence operators at the limits of their arguments: what lies beside a buffer, the largest and smallest numbers, the largest calls.
+
+Tolerances of attention are those that test_sequence_long_gpu.py derives (half a step, 2^-8, of the 2-norm in bfloat16, 4e-6 of it in
+float32 and what dp - delta loses), against the definition in float64.  A cap adds to them: tanh is taken to 3 * 2^-24 of itself, with the
+roundings of its argument and of the product with the cap 5 * 2^-24 of a score, and a probability is off by that times the score, below 6
+here: 2e-6 of itself, within float32's 4e-6 as it is spread over the keys; in bfloat16, up to a cap of 1024, 1024 * 2^-22 = 2.5e-4 of
+itself at most, a sixteenth of 2^-8, where the roundings that are counted in 2^-8 add up to sqrt(2 / 3) of it."""
 import math
 
 import pytest
+import test_sequence_long_gpu as long_sequences
 import torch
 
 pytestmark = pytest.mark.gpu
@@ -76,3 +82,44 @@ def test_attention_gradients_of_the_most_rows(ops, dtype, d, rows):
         torch.testing.assert_close(g.float(), w.float(), rtol=rel, atol=rel * w.float().abs().max().item())
     for g in got[:2]:
         assert not g[:rows - n].any()
+
+
+CAPS = [30.0, 1024.0, 1025.0, 1e4, 1e6, 1e9, 1e37]
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("cap", CAPS)
+@pytest.mark.parametrize("d,lens", [(64, [33, 20]), (64, [600, 700]), (128, [40, 50]), (128, [600, 700]), (242, [50, 30]), (33, [90, 70])])
+def test_attention_under_large_caps(ops, dtype, cap, d, lens):
+    """the larger the cap, the nearer to no cap at all: results and gradients, short and long sequences, odd rows"""
+    long_sequences._check(ops, lens, lens, 2, 1, d, DT[dtype], seed=29, causal=True, score_cap=cap)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("cap", CAPS)
+def test_attention_under_large_caps_and_distances(ops, dtype, cap):
+    long_sequences._check(ops, [90, 60], [90, 75], 2, 2, 64, DT[dtype], seed=31, causal=True, score_cap=cap, distance_slope=[0.2, 0.03], scale=-0.2)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("cap", CAPS)
+@pytest.mark.parametrize("d", [64, 242])
+def test_step_under_large_caps(ops, dtype, cap, d):
+    dt, lens = DT[dtype], [700, 1, 64]
+    q, kc, vc = _normal(1, 3, 4, d, dtype=dt), _normal(2, 3, 700, 2, d, dtype=dt), _normal(3, 3, 700, 2, d, dtype=dt)
+    k, v = (torch.cat([c[i, :n] for i, n in enumerate(lens)]) for c in (kc, vc))
+    (out, tol), *_ = long_sequences._ref(q, k, v, q, [0, 1, 2, 3], [0, 700, 701, 765], score_cap=cap)
+    assert (ops.attention_step(q, kc, vc, _i32(lens), score_cap=cap).double().cpu() - out).norm() <= tol
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_large_caps_with_what_is_not_finite(ops, d):
+    """a NaN key under a large cap reaches the rows that see it and no others"""
+    n, at = 150, 100
+    q, k, v, do = (_normal(50 + i, n, 2, d, dtype=torch.bfloat16) for i in range(4))
+    base = _run(ops, q, k, v, do, [0, n], [0, n], causal=True, score_cap=1e6)
+    k[at] = math.nan
+    got = _run(ops, q, k, v, do, [0, n], [0, n], causal=True, score_cap=1e6)
+    for g, b in zip(got[:2], base[:2]):
+        assert torch.isnan(g[at:]).all()
+        torch.testing.assert_close(g[:at].float(), b[:at].float(), rtol=2.0 ** -6, atol=2.0 ** -6 * b.float().abs().max().item())
