@@ -237,7 +237,8 @@ int sttran_dropout_add(const void* x, const void* residual, void* y, int64_t n, 
   const double words = std::nearbyint(p * 4294967296.0);
   A.x = (const char*)x; A.res = (const char*)residual; A.y = (char*)y;
   A.rng = rng_state; A.key = key; A.offset = offset; A.used = used; A.n = n;
-  A.threshold = words >= 4294967295.0 ? 4294967295u : (uint32_t)words;
+  A.none = words >= 4294967296.0;                          // below 2^32 are all words
+  A.threshold = A.none ? 0u : (uint32_t)words;
   A.mul = (float)(1.0 / (1.0 - p));
   return code(launch_seq_dropout(str(stream), dtype == STTRAN_DTYPE_BF16, A));
 }

@@ -66,6 +66,7 @@ struct SeqDropoutArgs {
   int64_t* used;                   // optional, device: the state this launch drew from
   int64_t n;
   uint32_t threshold;              // words below it drop their element
+  bool none;                       // every element is dropped
   float mul;
   int aln;
 };

@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(256) seq_dropout_kernel(SeqDropoutArgs A) {
       seq_philox((uint64_t)i * (EPL / 4) + b, (uint64_t)offset, (uint64_t)key, word);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float v = word[j] >= A.threshold ? SeqElt<T>::get(x, 4 * b + j) * A.mul : 0.f;
+        const float v = word[j] >= A.threshold && !A.none ? SeqElt<T>::get(x, 4 * b + j) * A.mul : 0.f;
         SeqElt<T>::put(y, 4 * b + j, A.res ? SeqElt<T>::get(r, 4 * b + j) + v : v);
       }
     }

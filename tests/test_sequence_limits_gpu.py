@@ -9,6 +9,7 @@ import math
 
 import pytest
 import test_sequence_long_gpu as long_sequences
+import test_sequence_ops_gpu as short_sequences
 import torch
 
 pytestmark = pytest.mark.gpu
@@ -52,6 +53,19 @@ def test_dropout_leaves_what_lies_behind_its_elements(ops, native, dtype, n):
         assert rc == 0
         assert bool((y[:at] == 7).all()) and bool((y[at + n:] == 7).all())
         assert torch.equal(y[at:at + n], ops.dropout_add(x[at:at + n].clone(), r[at:at + n].clone(), p=0.25, seed=5, offset=6))
+
+
+@pytest.mark.parametrize("dtype", DT)
+def test_dropout_of_everything(ops, dtype):
+    """where p * 2^32 rounds to 2^32 no word is as large: nothing is kept, infinities neither.  Word 2 is 2^32 - 1 at this key and offset,
+    the largest there is (the first offset under key 0 that a search over the generator's definition finds)"""
+    key, offset, at = 0, 389732782, 2
+    assert short_sequences._philox(0, offset, key)[at] == 2 ** 32 - 1
+    x = torch.full((8,), math.inf, dtype=DT[dtype], device="cuda")
+    for p in (1 - 2.0 ** -34, 1 - 2.0 ** -53):
+        assert not ops.dropout_add(x, p=p, seed=key, offset=offset).any()
+    kept = ops.dropout_add(x, p=1 - 2.0 ** -32, seed=key, offset=offset)            # round(p * 2^32) = 2^32 - 1: that word alone is kept
+    assert kept[at] == math.inf and kept.isinf().sum() == 1
 
 
 # ---- attention ---------------------------------------------------------------------------------------------------------
