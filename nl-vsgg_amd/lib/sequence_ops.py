@@ -10,7 +10,8 @@ bias, capped scores) and for clips that grow token by token.
 float32 or bfloat16 throughout a call (statistics and sums in float32); tensors on one MI355X, no CPU path.  Work is enqueued
 on the current stream of the tensors' device and may be captured into a graph; nothing is read back.  (As with every torch
 operator: to capture a backward pass, let the results of eager calls on the same leaves go first.)  Bad arguments raise
-ValueError before anything is launched.  The last dimension of q / k / v must be contiguous (others are copied), other
+ValueError before anything is launched.  Derivatives are reverse-mode and of first order: tensors with a forward-mode tangent are
+refused, and so are calls under a tracer that would record the result's allocation without the kernel.  The last dimension of q / k / v must be contiguous (others are copied), other
 strides are free."""
 from __future__ import annotations
 
@@ -18,6 +19,7 @@ import ctypes as C
 import math
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .. import _native as nat
@@ -39,9 +41,18 @@ def _launch(fn, args, dev):
         raise nat.SttranError(rc, f"{fn.__name__} failed")
 
 
+def _no_tangents(name, *tensors):
+    """A kernel gives its result no tangent, which reads as a derivative of zero."""
+    if forward_ad._current_level >= 0 and any(x is not None and forward_ad.unpack_dual(x).tangent is not None for x in tensors):
+        raise ValueError(f"{name} has no forward-mode derivative, and one of its tensors has a tangent")
+
+
 def _checked(name, *tensors):
-    """The library, if `tensors` share a served dtype and device."""
+    """The library, if `tensors` share a served dtype and device and the call may run as it is."""
     t = tensors[0]
+    _no_tangents(name, *tensors)
+    if torch._C._is_tracing() or (torch._C._len_torch_dispatch_stack() and torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY)):
+        raise RuntimeError(f"{name} cannot be traced: its kernels are launched beside torch's operators")
     if not t.is_cuda:
         raise RuntimeError(f"{name} runs on an MI355X only (no CPU path)")
     if t.dtype not in _DTYPES:
@@ -63,6 +74,7 @@ def _rows(x, limit=True):
 
 def _small(name, what, x, dtype, shape, dev):
     """An index / parameter vector: exact dtype, shape and device, contiguous."""
+    _no_tangents(name, x)
     if x.dtype != dtype or tuple(x.shape) != shape or x.device != dev:
         raise ValueError(f"{name}: {what} must be {dtype} {list(shape)} on {dev}, got {x.dtype} {list(x.shape)} on {x.device}")
     return x.contiguous()
@@ -139,6 +151,7 @@ class _PackedAttention(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout):
         q, k, v, seq_off, key_off, prefix, slope, out, low, lse = ctx.saved_tensors
+        _no_tangents("packed_attention", dout)
         lib = nat.load()
         dout = _rows(dout)
         a = _attention_struct(q, k, v, seq_off, key_off, prefix, slope, *ctx.plain)
@@ -230,8 +243,10 @@ def attention_step(q, k_cache, v_cache, lengths, *, distance_slope=None, score_c
     q = _rows(q, limit=False)
     if out is None:
         out = _like(q)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
-        raise ValueError(f"{name}: out must be contiguous and like q")
+    else:
+        _no_tangents(name, out)
+        if out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
+            raise ValueError(f"{name}: out must be contiguous and like q")
     for what, x in (("k_cache", k_cache), ("v_cache", v_cache)):
         if d > 1 and x.stride(3) != 1 or x.shape[1] > 1 and x.stride(1) * x.element_size() > _MAX_CACHE_ROW_BYTES:
             raise ValueError(f"{name}: {what}'s head dim must be contiguous and its rows at most {_MAX_CACHE_ROW_BYTES} bytes apart (a cache is never copied)")
@@ -306,6 +321,7 @@ class _RotaryQK(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dyq, dyk):
         q, k, positions, freq, wq, wk = ctx.saved_tensors
+        _no_tangents("rotary_qk", dyq, dyk)
         lib, dev = nat.load(), q.device
         dyq, dyk = _rows(dyq, limit=False), _rows(dyk, limit=False)
         a = _rotary_struct(q, k, positions, freq, wq, wk, *ctx.plain)
@@ -382,6 +398,7 @@ class _DropoutAdd(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         used, = ctx.saved_tensors
+        _no_tangents("dropout_add", dy)
         p, key, offset, added = ctx.plain
         dx = _dropout(dy.contiguous(), None, p, used, key, offset, None) if ctx.needs_input_grad[0] else None
         return dx, dy if added and ctx.needs_input_grad[1] else None, None, None, None, None

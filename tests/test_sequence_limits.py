@@ -33,3 +33,43 @@ def test_step_shares_cover_the_cache(native, n, heads, capacity):
     need = native.load().sttran_attention_step_workspace_bytes(C.byref(_step(native, n, heads, capacity)))
     shares, rest = divmod(need, heads * n * (1 + 2) * 4)
     assert rest == 0 and 2 <= shares <= 4096 + 1 and -(-capacity // shares) >= 97           # 192 rows a share, or what is left of them
+
+
+def _calls(ops):
+    """each operator, its tensors by name (float32 unless counted or placed by them) and which of them are numbers"""
+    f = lambda *s: torch.randn(*s)  # noqa: E731
+    off, pos = torch.tensor([0, 4], dtype=torch.int32), torch.arange(4)
+    return [
+        (lambda **t: ops.packed_attention(t["q"], t["k"], t["v"], off), dict(q=f(4, 2, 8), k=f(4, 2, 8), v=f(4, 2, 8))),
+        (lambda **t: ops.attention_step(t["q"], t["k"], t["v"], off[:1]), dict(q=f(1, 2, 8), k=f(1, 5, 2, 8), v=f(1, 5, 2, 8))),
+        (lambda **t: ops.rotary_qk(t["q"], t["k"], pos, torch.ones(4)), dict(q=f(4, 2, 8), k=f(4, 2, 8))),
+        (lambda **t: ops.dropout_add(t["x"], t["residual"], p=0.1, seed=1), dict(x=f(6), residual=f(6))),
+    ]
+
+
+def test_forward_mode_is_refused():
+    """a tangent would be lost without a word: each operator refuses one in each of its tensors, by dual numbers and by torch.func.jvp"""
+    import torch.autograd.forward_ad as fw
+    from nl_vsgg_amd.lib import sequence_ops as ops
+    for call, tensors in _calls(ops):
+        for name, x in tensors.items():
+            with fw.dual_level():
+                with pytest.raises(ValueError, match="forward-mode"):
+                    call(**{**tensors, name: fw.make_dual(x, torch.ones_like(x))})
+            with pytest.raises(ValueError, match="forward-mode"):
+                torch.func.jvp(lambda y: call(**{**tensors, name: y}), (x,), (torch.ones_like(x),))
+        with fw.dual_level(), pytest.raises(RuntimeError, match="MI355X only"):
+            call(**tensors)                          # without a tangent: the next check's answer
+
+
+def test_tracers_are_refused():
+    """a trace would hold the result's allocation and not the kernel"""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from nl_vsgg_amd.lib import sequence_ops as ops
+    for call, tensors in _calls(ops):
+        names = list(tensors)
+        flat = lambda *a: call(**dict(zip(names, a)))  # noqa: E731
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(flat, tuple(tensors.values()), check_trace=False)
+        with pytest.raises(RuntimeError, match="traced"):
+            make_fx(flat)(*tensors.values())

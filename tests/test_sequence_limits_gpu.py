@@ -137,3 +137,24 @@ def test_large_caps_with_what_is_not_finite(ops, d):
     for g, b in zip(got[:2], base[:2]):
         assert torch.isnan(g[at:]).all()
         torch.testing.assert_close(g[:at].float(), b[:at].float(), rtol=2.0 ** -6, atol=2.0 ** -6 * b.float().abs().max().item())
+
+
+def test_tangents_are_refused_wherever_they_come_in(ops):
+    """constants, the buffer to write into, and the gradient that a backward pass is given"""
+    import torch.autograd.forward_ad as fw
+    q, k, freq, w, off = _normal(1, 6, 4, 16), _normal(2, 6, 2, 16), ops.rotary_frequencies(16, device="cuda"), torch.ones(16, device="cuda"), _i32([0, 6])
+    pos, slope, lens, cache = torch.arange(6, device="cuda"), torch.ones(4, device="cuda"), _i32([3] * 6), _normal(3, 6, 5, 2, 16)
+    with fw.dual_level():
+        dual = lambda x: fw.make_dual(x, torch.ones_like(x))  # noqa: E731
+        for call in (lambda: ops.packed_attention(q, k, k, off, distance_slope=dual(slope)), lambda: ops.attention_step(q, cache, cache, lens, distance_slope=dual(slope)),
+                     lambda: ops.attention_step(q, cache, cache, lens, out=dual(torch.empty_like(q))), lambda: ops.rotary_qk(q, k, pos, dual(freq)),
+                     lambda: ops.rotary_qk(q, k, pos, freq, dual(w), w), lambda: ops.rotary_qk(q, k, pos, freq, w, dual(w))):
+            with pytest.raises(ValueError, match="forward-mode"):
+                call()
+        ql = q.clone().requires_grad_()
+        for y in (ops.packed_attention(ql, k, k, off), ops.rotary_qk(ql, k, pos, freq)[0], ops.dropout_add(ql, p=0.5, seed=1)):
+            with pytest.raises(ValueError, match="forward-mode"):
+                torch.autograd.grad(y, ql, dual(torch.ones_like(y)))
+        ops.packed_attention(q, k, k, off), ops.attention_step(q, cache, cache, lens), ops.rotary_qk(q, k, pos, freq), ops.dropout_add(q, p=0.5, seed=1)
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda x: ops.packed_attention(x, k, k, off))(q[None])
