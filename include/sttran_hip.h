@@ -325,7 +325,7 @@ int sttran_roi_align(const float* fmaps, int32_t T, int32_t C, int32_t H, int32_
 typedef struct SttranAttention {
   uint32_t struct_size;            /* = sizeof(SttranAttention) */
   int32_t dtype;                   /* STTRAN_DTYPE_F32 / STTRAN_DTYPE_BF16 */
-  int32_t num_seq, num_q_heads, num_kv_heads, head_dim;     /* head_dim 1 .. 256 */
+  int32_t num_seq, num_q_heads, num_kv_heads, head_dim;     /* num_seq <= 2^30, head_dim 1 .. 256 */
   int64_t q_rows, kv_rows;         /* < 2^31 - 1024, and times their heads < 2^29 - 1024 */
   const void *q, *k, *v;
   int64_t q_row_stride, q_head_stride, k_row_stride, k_head_stride, v_row_stride, v_head_stride;

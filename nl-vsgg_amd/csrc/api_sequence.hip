@@ -12,6 +12,7 @@ namespace {
 constexpr int64_t kMaxRows = (int64_t(1) << 31) - 1024, kMaxRowBytes = int64_t(1) << 24, kMaxCacheRowBytes = int64_t(1) << 22;
 constexpr int64_t kMaxHeadRows = (int64_t(1) << 29) - 1024;  // a launch over tiles has 8 threads a head's row at most, and fewer than 2^32 of them
 constexpr int64_t kMaxCapacity = int64_t(1) << 30;            // rows and a chunk of them are counted in 32 bits
+constexpr int32_t kMaxSeq = 1 << 30;                          // the search for a row's sequence adds two numbers of them in 32 bits
 
 bool dtype_ok(int32_t t) { return t == STTRAN_DTYPE_F32 || t == STTRAN_DTYPE_BF16; }
 int elt(int32_t t) { return t == STTRAN_DTYPE_BF16 ? 2 : 4; }
@@ -46,7 +47,7 @@ int code(hipError_t e) { return e == hipSuccess ? STTRAN_OK : STTRAN_ERR_HIP; }
 bool attention_args(const SttranAttention* a, SeqAttnArgs& A, Alignment& al) {
   if (!a || a->struct_size != sizeof(SttranAttention) || !dtype_ok(a->dtype) || !heads_ok(a->num_q_heads, a->num_kv_heads, a->head_dim))
     return false;
-  if (a->num_seq < 0 || a->q_rows < 0 || a->kv_rows < 0 || a->q_rows > kMaxRows || a->kv_rows > kMaxRows) return false;
+  if (a->num_seq < 0 || a->num_seq > kMaxSeq || a->q_rows < 0 || a->kv_rows < 0 || a->q_rows > kMaxRows || a->kv_rows > kMaxRows) return false;
   if (!score_ok(a->scale, a->score_cap)) return false;
   const int es = elt(a->dtype);
   if (!row_stride_ok(a->q_row_stride, es) || !row_stride_ok(a->k_row_stride, es) || !row_stride_ok(a->v_row_stride, es) ||

@@ -193,6 +193,8 @@ def packed_attention(q, k, v, seq_off, key_off=None, *, causal=False, prefix_len
     if seq_off.dim() != 1 or seq_off.shape[0] < 1:
         raise ValueError(f"{name}: seq_off is a vector of sequences + 1 offsets")
     n = seq_off.shape[0]
+    if n - 1 > 1 << 30:
+        raise ValueError(f"{name}: at most 2^30 sequences a call")
     seq_off = _small(name, "seq_off", seq_off, torch.int32, (n,), dev)
     if key_off is None:
         if k.shape[0] != q.shape[0]:

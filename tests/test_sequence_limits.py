@@ -73,3 +73,12 @@ def test_tracers_are_refused():
             torch.jit.trace(flat, tuple(tensors.values()), check_trace=False)
         with pytest.raises(RuntimeError, match="traced"):
             make_fx(flat)(*tensors.values())
+
+
+@pytest.mark.parametrize("n,want", [(1 << 30, 0), ((1 << 30) + 1, 1), (2 ** 31 - 1, 1)])
+def test_attention_counts_its_sequences(native, n, want):
+    """a row's sequence is found by halving: two numbers of sequences, added, stay within 32 bits.  (No rows: nothing is launched)"""
+    lib = native.load()
+    a = native.SttranAttention(struct_size=C.sizeof(native.SttranAttention), dtype=0, num_seq=n, num_q_heads=1, num_kv_heads=1, head_dim=64, seq_off=4096, key_off=4096,
+                               scale=1.0)
+    assert lib.sttran_attention_forward(C.byref(a), None) == want and lib.sttran_attention_backward(C.byref(a), None) == want

@@ -158,3 +158,10 @@ def test_tangents_are_refused_wherever_they_come_in(ops):
         ops.packed_attention(q, k, k, off), ops.attention_step(q, cache, cache, lens), ops.rotary_qk(q, k, pos, freq), ops.dropout_add(q, p=0.5, seed=1)
     with pytest.raises(RuntimeError):
         torch.func.vmap(lambda x: ops.packed_attention(x, k, k, off))(q[None])
+
+
+def test_attention_refuses_more_sequences_than_it_counts(ops):
+    q = _normal(1, 4, 1, 8)
+    off = torch.zeros(1, dtype=torch.int32, device="cuda").expand((1 << 30) + 2)
+    with pytest.raises(ValueError, match="sequences"):
+        ops.packed_attention(q, q, q, off)
