@@ -225,7 +225,7 @@ def attention_step(q, k_cache, v_cache, lengths, *, distance_slope=None, score_c
     q [sequences, query heads, head dim], caches [sequences, capacity, key heads, head dim], `lengths` int32 [sequences]: live rows of
     each cache, the new token's own key (already written) being the last of them; rows behind are not read, length 0 gives zeros,
     a length above the capacity counts as the capacity.  Scores as in packed_attention.  `out`: a contiguous tensor like q to write
-    into.  No gradient."""
+    into (q itself, too).  No gradient."""
     name = "attention_step"
     lib = _checked(name, q, k_cache, v_cache)
     if q.dim() != 3 or k_cache.dim() != 4 or v_cache.dim() != 4 or k_cache.shape[0] != q.shape[0]:
@@ -249,6 +249,9 @@ def attention_step(q, k_cache, v_cache, lengths, *, distance_slope=None, score_c
         _no_tangents(name, out)
         if out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
             raise ValueError(f"{name}: out must be contiguous and like q")
+        if out.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{name} has no gradient: out must not require one")
+        torch.autograd.graph.increment_version(out)        # an earlier call's backward pass that saved it must not use what is written now
     for what, x in (("k_cache", k_cache), ("v_cache", v_cache)):
         if d > 1 and x.stride(3) != 1 or x.shape[1] > 1 and x.stride(1) * x.element_size() > _MAX_CACHE_ROW_BYTES:
             raise ValueError(f"{name}: {what}'s head dim must be contiguous and its rows at most {_MAX_CACHE_ROW_BYTES} bytes apart (a cache is never copied)")

@@ -165,3 +165,25 @@ def test_attention_refuses_more_sequences_than_it_counts(ops):
     off = torch.zeros(1, dtype=torch.int32, device="cuda").expand((1 << 30) + 2)
     with pytest.raises(ValueError, match="sequences"):
         ops.packed_attention(q, q, q, off)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("cap", [100, 3000])
+def test_step_writes_into_a_tensor_as_torch_does(ops, dtype, cap):
+    """q itself; a tensor that autograd saved is marked as written; one that requires a gradient is refused"""
+    q, kc, vc, lens = _normal(1, 2, 4, 64, dtype=DT[dtype]), _normal(2, 2, cap, 2, 64, dtype=DT[dtype]), _normal(3, 2, cap, 2, 64, dtype=DT[dtype]), _i32([cap, 7])
+    want = ops.attention_step(q, kc, vc, lens)
+    same = q.clone()
+    assert ops.attention_step(same, kc, vc, lens, out=same) is same and torch.equal(same, want)
+    x = torch.ones_like(q).requires_grad_()
+    saved = q.clone()
+    y = x * saved
+    ops.attention_step(q, kc, vc, lens, out=saved)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    with pytest.raises(ValueError, match="no gradient"):
+        ops.attention_step(q, kc, vc, lens, out=x)
+    with torch.no_grad():
+        assert torch.equal(ops.attention_step(q, kc, vc, lens, out=x), want)
+    with torch.inference_mode():
+        assert torch.equal(ops.attention_step(q, kc, vc, lens, out=torch.empty_like(q)), want)
