@@ -82,3 +82,19 @@ def test_attention_counts_its_sequences(native, n, want):
     a = native.SttranAttention(struct_size=C.sizeof(native.SttranAttention), dtype=0, num_seq=n, num_q_heads=1, num_kv_heads=1, head_dim=64, seq_off=4096, key_off=4096,
                                scale=1.0)
     assert lib.sttran_attention_forward(C.byref(a), None) == want and lib.sttran_attention_backward(C.byref(a), None) == want
+
+
+def test_one_set_of_compiler_flags():
+    """a change of the flags makes every object anew, and the tools that compile single sources take the flags from the same place"""
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    csrc = os.path.join(root, "nl-vsgg_amd", "csrc")
+    run = lambda *a: subprocess.run(["make", "-C", csrc, "--no-print-directory", *a], capture_output=True, text=True, check=True).stdout  # noqa: E731
+    flags = run("-s", "print-flags").split()
+    assert flags[:4] == ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] and "--offload-arch=gfx950" in flags
+    anew = run("-n", "-W", "Makefile")
+    sources = [f for f in os.listdir(csrc) if f.endswith(".hip")]
+    assert len(sources) > 20 and all(f"-c {f} " in anew for f in sources)
+    for tool in ("kernel_resources.py", "experiments/build_variant.sh", "experiments/build_mc_trace.sh"):
+        text = open(os.path.join(root, "tools", tool)).read()
+        assert "print-flags" in text and "-O3" not in text, tool

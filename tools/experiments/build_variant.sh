@@ -6,7 +6,8 @@ set -euo pipefail
 name=$1; src=$2; shift 2
 cd "$(dirname "$0")/../../nl-vsgg_amd/csrc"
 mkdir -p ab
-/opt/rocm/bin/hipcc "$@" -O3 -std=c++17 -fPIC --offload-arch=gfx950 -Wall -Wno-unused-function -Wno-unused-value -Wno-unused-result -c "$src" -o "ab/${src%.hip}_$name.o"
+flags=$(make -s print-flags)
+/opt/rocm/bin/hipcc "$@" $flags -c "$src" -o "ab/${src%.hip}_$name.o"
 objs=$(ls *.o | grep -v "^${src%.hip}.o$")
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o "ab/libsttran_hip_$name.so" $objs "ab/${src%.hip}_$name.o"
 rm -f "ab/${src%.hip}_$name.o"

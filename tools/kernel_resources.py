@@ -11,9 +11,10 @@ import sys
 
 src = sys.argv[1]
 extra = sys.argv[2:]
-cmd = ["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950", "-Rpass-analysis=kernel-resource-usage",
-       "-c", os.path.basename(src), "-o", "/dev/null"] + extra
-out = subprocess.run(cmd, cwd=os.path.dirname(os.path.abspath(src)), capture_output=True, text=True).stderr
+where = os.path.dirname(os.path.abspath(src))
+flags = subprocess.run(["make", "-s", "print-flags"], cwd=where, capture_output=True, text=True, check=True).stdout.split()
+cmd = ["/opt/rocm/bin/hipcc", *flags, "-Rpass-analysis=kernel-resource-usage", "-c", os.path.basename(src), "-o", "/dev/null"] + extra
+out = subprocess.run(cmd, cwd=where, capture_output=True, text=True).stderr
 rows, cur = [], None
 for line in out.splitlines():
     m = re.search(r"remark:\s+(.*?) \[-Rpass-analysis", line)
