@@ -98,9 +98,18 @@ def _heads(name, q, k, v):
     return hq, hk
 
 
+def _number(name, what, x):
+    """A plain number; of a tensor its value, unless a gradient would get lost with it."""
+    if isinstance(x, torch.Tensor):
+        _no_tangents(name, x)
+        if x.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{name}: {what} is a number, it gets no gradient")
+    return float(x)
+
+
 def _score(name, scale, cap, d):
-    scale = d ** -0.5 if scale is None else float(scale)
-    cap = 0.0 if cap is None else float(cap)
+    scale = d ** -0.5 if scale is None else _number(name, "scale", scale)
+    cap = 0.0 if cap is None else _number(name, "score_cap", cap)
     if not math.isfinite(scale) or not math.isfinite(cap) or cap < 0:
         raise ValueError(f"{name}: scale must be finite and score_cap finite and >= 0 (0: none)")
     if not max(abs(scale), cap, abs(scale) / cap if cap else 0.0) < 1e38 or (cap and cap < 1e-37):
@@ -369,7 +378,7 @@ def rotary_qk(q, k, positions, frequencies, q_weight=None, k_weight=None, *, eps
     if q_weight is not None:
         q_weight = _small(name, "q_weight", q_weight, torch.float32, (d,), dev)
         k_weight = _small(name, "k_weight", k_weight, torch.float32, (d,), dev)
-    eps = float(eps)
+    eps = _number(name, "eps", eps)
     if not (math.isfinite(eps) and eps >= 0):
         raise ValueError(f"{name}: eps is finite and >= 0")
     q, k = _rows(q, limit=False), _rows(k, limit=False)
@@ -421,7 +430,7 @@ def dropout_add(x, residual=None, *, p, rng_state=None, seed=None, offset=0):
     _checked(name, x, *([residual] if residual is not None else []))
     if residual is not None and residual.shape != x.shape:
         raise ValueError(f"{name}: residual {list(residual.shape)} is not x's shape {list(x.shape)}")
-    p = float(p)
+    p = _number(name, "p", p)
     if not 0.0 <= p < 1.0:
         raise ValueError(f"{name}: p is in [0, 1)")
     if (rng_state is None) == (seed is None):

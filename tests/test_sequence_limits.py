@@ -98,3 +98,14 @@ def test_one_set_of_compiler_flags():
     for tool in ("kernel_resources.py", "experiments/build_variant.sh", "experiments/build_mc_trace.sh"):
         text = open(os.path.join(root, "tools", tool)).read()
         assert "print-flags" in text and "-O3" not in text, tool
+
+
+def test_a_number_that_wants_a_gradient_is_refused():
+    from nl_vsgg_amd.lib import sequence_ops as ops
+    x = torch.tensor(0.5, requires_grad=True)
+    for args in ((x, 0.0), (None, x)):
+        with pytest.raises(ValueError, match="no gradient"):
+            ops._score("packed_attention", *args, 64)
+        with torch.no_grad():
+            ops._score("packed_attention", *args, 64)
+    assert ops._score("packed_attention", torch.tensor(0.5), None, 64) == (0.5, 0.0)

@@ -187,3 +187,21 @@ def test_step_writes_into_a_tensor_as_torch_does(ops, dtype, cap):
         assert torch.equal(ops.attention_step(q, kc, vc, lens, out=x), want)
     with torch.inference_mode():
         assert torch.equal(ops.attention_step(q, kc, vc, lens, out=torch.empty_like(q)), want)
+
+
+def test_numbers_that_want_a_gradient_are_refused(ops):
+    """a learned scale, cap, eps or probability would get none, without a word; without a gradient a tensor is its value"""
+    import torch.autograd.forward_ad as fw
+    q, pos, off, lens, cache = _normal(1, 6, 2, 16), torch.arange(6, device="cuda"), _i32([0, 6]), _i32([3] * 6), _normal(2, 6, 5, 2, 16)
+    freq, w = ops.rotary_frequencies(16, device="cuda"), torch.ones(16, device="cuda")
+    calls = (lambda x: ops.packed_attention(q, q, q, off, scale=x), lambda x: ops.packed_attention(q, q, q, off, score_cap=x), lambda x: ops.attention_step(q, cache, cache, lens, scale=x),
+             lambda x: ops.attention_step(q, cache, cache, lens, score_cap=x), lambda x: ops.rotary_qk(q, q, pos, freq, w, w, eps=x)[0], lambda x: ops.dropout_add(q, p=x, seed=3))
+    for call in calls:
+        for x in (torch.tensor(0.5, requires_grad=True), torch.tensor([0.5], device="cuda", requires_grad=True)):
+            with pytest.raises(ValueError, match="no gradient"):
+                call(x)
+            with torch.no_grad():
+                assert torch.equal(call(x), call(0.5))
+        with fw.dual_level(), pytest.raises(ValueError, match="forward-mode"):
+            call(fw.make_dual(torch.tensor(0.5), torch.tensor(1.0)))
+        assert torch.equal(call(torch.tensor(0.5)), call(0.5))
