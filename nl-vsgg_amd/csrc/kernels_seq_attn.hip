@@ -29,6 +29,7 @@ __device__ __forceinline__ void seq_attn_fwd_again(const SeqAttnArgs& A, const S
 #pragma unroll
       for (int u = 0; u < 4; ++u) o[u] = fmaf(o[u], al, p * v.x[u]);
       m = mn;
+      if (!(l == l)) break;                          // a NaN probability: all of the row is NaN, whatever follows
     }
     if (A.splits > 1) {
       const int64_t at = ((int64_t)blockIdx.y * A.hq + head) * A.tq + row;

@@ -88,6 +88,7 @@ __device__ __forceinline__ void seq_attn_dq_again(const SeqAttnArgs& A, const Se
       seq_pair_any(A, sc, s, dp, true, lse, delta, base - key);
 #pragma unroll
       for (int u = 0; u < 4; ++u) o[u] = fmaf(dp, k.x[u], o[u]);
+      if (!(dp == dp)) break;                        // all of the row is NaN, whatever follows
     }
     seq_spread_store<T>(A.dq + ((int64_t)row * A.hq + head) * A.d * C::OS, nullptr, o, A.scale, A.d);
   }
@@ -277,12 +278,13 @@ __device__ __forceinline__ void seq_attn_dkv_again(const SeqAttnArgs& A, uint32_
     const SeqSpread k = seq_spread<T>(A.raw[1].p + kvh * A.raw[1].h + (int64_t)key * A.raw[1].t, A.d);
     const SeqSpread v = seq_spread<T>(A.raw[2].p + kvh * A.raw[2].h + (int64_t)key * A.raw[2].t, A.d);
     float dk[4] = {0.f, 0.f, 0.f, 0.f}, dv[4] = {0.f, 0.f, 0.f, 0.f};
+    bool rest = true;                                // false: all of dk's and dv's row is NaN, whatever follows
 #pragma unroll 1
-    for (int it = i0; it < i1; ++it) {
+    for (int it = i0; it < i1 && rest; ++it) {
       const int head = kvh * grp + it / nt, q0 = qbeg + it % nt * C::BR, q1 = min(q0 + C::BR, qend);
       const SeqScore sc(A, head);
 #pragma unroll 1
-      for (int row = q0; row < q1; ++row) {
+      for (int row = q0; row < q1 && rest; ++row) {
         const int4 r = A.rows[row];
         if (key < r.x || key >= r.y) continue;
         const SeqSpread q = seq_spread<T>(A.raw[0].p + head * A.raw[0].h + (int64_t)row * A.raw[0].t, A.d);
@@ -294,6 +296,7 @@ __device__ __forceinline__ void seq_attn_dkv_again(const SeqAttnArgs& A, uint32_
           dk[u] = fmaf(dp, q.x[u], dk[u]);
           dv[u] = fmaf(s, o.x[u], dv[u]);
         }
+        rest = s == s || dp == dp;
       }
     }
     const int64_t at = ((int64_t)key * A.hk + kvh) * A.d;

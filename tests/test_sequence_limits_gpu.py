@@ -205,3 +205,24 @@ def test_numbers_that_want_a_gradient_are_refused(ops):
         with fw.dual_level(), pytest.raises(ValueError, match="forward-mode"):
             call(fw.make_dual(torch.tensor(0.5), torch.tensor(1.0)))
         assert torch.equal(call(torch.tensor(0.5)), call(0.5))
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("d,n", [(64, 300), (64, 1100), (128, 1100), (242, 60), (242, 1100), (33, 90)])
+@pytest.mark.parametrize("kw", [{}, dict(causal=True, score_cap=4.0)])
+def test_a_sequence_of_nan_beside_another(ops, dtype, d, n, kw):
+    """a diverged sequence: all of its results and gradients are NaN (each row is known after the first key that it sees), the one beside it
+    answers as ever -- tiles that both share are done again pair by pair, sums in another order: 2^-6 of the largest in bfloat16, 1e-5"""
+    q, k, v, do = (_normal(60 + i, 2 * n + 40, 2, d, dtype=DT[dtype]) for i in range(4))
+    off = [0, n, 2 * n + 40]
+    base = _run(ops, q, k, v, do, off, off, **kw)
+    rel = 2.0 ** -6 if dtype == "bf16" else 1e-5
+    for bad in ((q, k, v), (k,)):
+        args = [x.clone() for x in (q, k, v)]
+        for x, y in zip((q, k, v), args):
+            if any(x is z for z in bad):
+                y[:n] = math.nan
+        got = _run(ops, *args, do, off, off, **kw)
+        for g, b in zip(got, base):
+            assert torch.isnan(g[:n]).all()
+            torch.testing.assert_close(g[n:].float(), b[n:].float(), rtol=rel, atol=rel * b.float().abs().max().item())
