@@ -316,6 +316,9 @@ int sttran_roi_align(const float* fmaps, int32_t T, int32_t C, int32_t H, int32_
  *   out = softmax(z) v;  rows that see nothing, or belong to no sequence, become zeros.
  * What a mask hides does not reach a result, infinities and NaN included.  Offsets are device data: they are clamped to the
  * tensors, never checked.
+ * Sums and statistics are fp32.  bfloat16: probabilities enter the second product with 8 bits, and with 16 where the call's
+ * sequences have fewer than 64 rows on average (512 for the gradients' products, any length there above 128 columns), a cap is
+ * above 1024 or rows lie at odd multiples of 2 bytes.
  * For a later backward: lse [num_q_heads, q_rows] fp32 (base-2 log-sums, private), and for bfloat16 out_residual like out (what
  * the rounding of out took away).
  * sttran_attention_backward: dq [q_rows, num_q_heads, head_dim], dk, dv [kv_rows, num_kv_heads, head_dim], contiguous, from dout
@@ -350,7 +353,8 @@ int sttran_attention_backward(const SttranAttention* args, void* stream);
 
 /* One new token a sequence: q [num_seq, num_q_heads, head_dim] over the first lengths[s] rows (clamped to capacity) of the caches
  * k / v [num_seq, capacity, num_kv_heads, head_dim]; the token's place is lengths[s] - 1.  Same z as above; length 0 gives zeros.
- * Rows from lengths[s] on are not read.  num_seq <= 65535, capacity <= 2^30; a row stride is at most 2^22 bytes.  Workspace: sttran_attention_step_workspace_bytes(args). */
+ * Rows from lengths[s] on are not read.  num_seq <= 65535, capacity <= 2^30; a row stride is at most 2^22 bytes.  out may be q.
+ * Workspace: sttran_attention_step_workspace_bytes(args). */
 typedef struct SttranAttentionStep {
   uint32_t struct_size;            /* = sizeof(SttranAttentionStep) */
   int32_t dtype;

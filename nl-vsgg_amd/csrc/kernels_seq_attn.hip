@@ -100,10 +100,12 @@ struct SeqFwdLds {                                       // DS == 1: two tiles o
 // Bound by the matrix pipe where sequences are long -- two products of 2 d operations a visible pair, 4 bytes of LDS read for every 32
 // operations, scores and probabilities never leave the registers -- and by the latency of a workgroup's few blocks where they are short.
 // Measured (a large matrix product reaches 1182 TFLOP/s in bfloat16 and 154 in fp32 on the card):
-//   three sequences of 4000 .. 8000 rows, 8 heads over 2 of 128 columns, causal, bfloat16: 305 us, 870 TFLOP/s; capped, 16 heads over 4: 690
-//   us (the exponential and the reciprocal of each score's tanh), 720;  96 of 37 .. 500 rows, 8 over 2 of 64, distances: 67 us
-//   four of 1800 .. 2240 rows, 8 heads of 242, distances, fp32 on planes: 1240 us (six products for one);  1024 of 5 .. 35, 8 of 242, fp32
-//   instructions: 255 us, 2.5 TB/s
+//   three sequences of 4000 .. 8000 rows, 8 heads over 2 of 128 columns, causal, bfloat16: 305 us, 870 TFLOP/s;
+//   capped, 16 heads over 4: 680 us, 730 TFLOP/s (the exponential and the reciprocal of each score's tanh: vector units busy 0.59 of the
+//   time, where it is 0.40 without a cap; 730 us at the clocks of a profiled run);  a cap above 1024: 663 us where 50 takes 380
+//   96 of 37 .. 500 rows, 8 over 2 of 64, distances: 66 us (vector units 0.46, matrix pipe 0.11)
+//   four of 1800 .. 2240 rows, 8 heads of 242, distances, fp32 on planes: 1150 us (six products for one)
+//   1024 of 5 .. 35, 8 of 242, fp32 instructions: 255 us, 2.5 TB/s
 // 32 own rows a wave: the stationary operand stays in registers, so every value read from LDS serves 32 rows.
 template <class C, int CAP, bool SLOPE, bool TWO>
 __global__ void __launch_bounds__(C::NT) __attribute__((amdgpu_waves_per_eu(2, 2)))
@@ -115,7 +117,8 @@ seq_attn_fwd_kernel(SeqAttnArgs A) {
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int tiles = (A.tq + C::RB - 1) / C::RB;
   const int id = seq_xcd_order(blockIdx.x, gridDim.x);
-  const int head = id / tiles, tile = tiles - 1 - seq_spread_tile(A, id % tiles, tiles, A.hq);      // rows that see most keys first where the order masks
+  // rows that see most keys first where the order masks
+  const int head = id / tiles, tile = tiles - 1 - seq_spread_tile(A, id % tiles, tiles, A.hq);
   const int kvh = head / (A.hq / A.hk), dh = w % C::DS;
   const int row0 = tile * C::RB + 32 * (w / C::DS), row = row0 + (lane & 31);
   const int dbytes = C::row_bytes(A.d);
@@ -439,7 +442,8 @@ int seq_attn_fwd_tile(int bf16, bool planes, int d) {
 // bfloat16 in sequences of fewer than 64 rows on average: probabilities enter the product with 16 bits (TWO; with 8 the result is 1.2 .. 1.4
 // times as far off as its own rounding, with few rows up to 1.48, and dq, dk up to 1.73 through delta).  It costs a third of the products,
 // which such calls hardly wait for (1000 x 32 rows, 8 heads of 64 columns, 43 -> 44 us; 500 x 60, 16 over 4 of 128, 136 -> 145; but three of
-// 4000 .. 8000 rows 305 -> 396).  Rows at odd 2 bytes take 16 bits always.
+// 4000 .. 8000 rows 305 -> 396).  Rows at odd 2 bytes take 16 bits always.  The host knows the average alone: short sequences beside a
+// long one get 8 bits too (ten of 5 .. 50 rows beside one of 8000: 1.1 .. 1.2 times their own rounding, their gradients 1.2 .. 1.5)
 hipError_t launch_seq_attn_fwd(hipStream_t s, int bf16, bool planes, const SeqAttnArgs& A) {
   const bool vec = A.aln >= 4;
   if (planes) return pick_planes(s, A);

@@ -104,7 +104,7 @@ struct SeqDqLds {                                        // as SeqFwdLds, with t
   static constexpr int kRed = 2 * kBufs * C::kTileBytes + (kOver ? 0 : kNeed), kBytes = kRed + C::NW * 8;
 };
 // Three products, bound as the forward pass.  Measured on the same sequences as there: 412 us, 960 TFLOP/s (bfloat16, 128 columns);
-// 77 us (64 columns, short, ds with 16 bits); 1615 us (fp32 on planes, 242 columns).
+// 76 us (64 columns, short, ds with 16 bits: vector units busy 0.46, matrix pipe 0.18); 1520 us (fp32 on planes, 242 columns).
 template <class C, int CAP, bool SLOPE, bool TWO>
 __global__ void __launch_bounds__(C::NT) __attribute__((amdgpu_waves_per_eu(2, 2)))
 seq_attn_dq_kernel(SeqAttnArgs A) {
@@ -314,7 +314,7 @@ template <class C>
 struct SeqDkvLds {                                       // tiles, statistics of the tile's rows, partial and whole score blocks
   // bfloat16 at 128 columns a wave: keys, values and both accumulators are 192 registers of the 256 that two waves a SIMD leave each,
   // too many next to a pair of blocks (spilled, the kernel took 2.4 ms on three sequences of 4000 .. 8000 rows, 8 heads, where it now
-  // takes 0.85): the values' fragments are read from LDS instead
+  // takes 0.7): the values' fragments are read from LDS instead
   static constexpr bool kPark = C::OS == 2 && C::DH == 128;
   static constexpr int kParked = kPark ? C::NF * 1024 : 0;          // bytes a wave
   static constexpr int kBufs = C::DS == 1 ? 2 : 1, kStat = 5 * C::BR * 4;
@@ -324,8 +324,8 @@ struct SeqDkvLds {                                       // tiles, statistics of
 };
 // Four products.  Two accumulators and both stationary operands do not fit the registers, so LDS carries the values' fragments beside the
 // streamed tiles: 40 KB a wave and 32 query rows, 2560 cycles of a CU's LDS for 2048 of its matrix pipes -- the bound.  Measured on the
-// same sequences: 760 us, 700 TFLOP/s, and 41 us to join the shares; 138 us (64 columns, short, 16 bits); 2245 us (fp32 on planes, 242
-// columns).
+// same sequences: 680 us, 780 TFLOP/s, and 40 us to join the shares; 138 us (64 columns, short, 16 bits: one wave a SIMD, which waits for
+// 0.46 of its time); 2120 us (fp32 on planes, 242 columns).
 template <class C, int CAP, bool SLOPE, bool TWO>
 __global__ void __launch_bounds__(C::NT) __attribute__((amdgpu_waves_per_eu(2, 2)))
 seq_attn_dkv_kernel(SeqAttnArgs A) {

@@ -7,8 +7,8 @@
 namespace sttran {
 
 // x [rows][heads][d] -> planes [rows][heads][3][d padded to 8]: 8 columns a thread; blockIdx.y: which tensor.  Reads 4 bytes an element
-// and writes 6, once (four tensors of 8000 rows, 8 heads of 242: 107 us, 6.0 TB/s, some of it out of the caches).  Numbers that the first rounding takes to infinity are cut off instead; infinities and NaN stay in the first
-// plane alone.
+// and writes 6, once (four tensors of 8000 rows, 8 heads of 242: 107 us, 6.0 TB/s, some of it out of the caches).  Numbers that the first
+// rounding takes to infinity are cut off instead; infinities and NaN stay in the first plane alone.
 struct SeqSplitArgs {
   SeqAttnArgs::In in[4];
   char* out[4];

@@ -9,9 +9,9 @@
 // once the contraction index is permuted, so probabilities go from the exponential into the next matrix instruction without
 // leaving their lane; row statistics of an own row live in one lane (plus its partner 32 lanes further).
 // bfloat16: v_mfma_f32_32x32x16_bf16, transposed reads by ds_read_b64_tr_b16; fp32: v_mfma_f32_32x32x2_f32 (exact products), or
-// (PL = 3, sequences of some hundred keys) three bfloat16 planes: x = hi + mid + lo, 8 bits of mantissa each, so the sum is x exactly, and of the nine
-// products of two such numbers the six that are not below 2^-24 of the largest, each exact in the fp32 accumulator.  That is
-// 6 / 16 of the exact instruction's time, and leaves the vector units free meanwhile, which fp32 matrix instructions do not.
+// (PL = 3, sequences of some hundred keys) three bfloat16 planes: x = hi + mid + lo, 8 bits of mantissa each, so the sum is x exactly,
+// and of the nine products of two such numbers the six that are not below 2^-24 of the largest, each exact in the fp32 accumulator.
+// That is 6 / 16 of the exact instruction's time, and leaves the vector units free meanwhile, which fp32 matrix instructions do not.
 // Head dims are padded to DP = 64 / 128 / 256 with zeros.  Where 32 own rows and their accumulators would not fit half of a SIMD's
 // registers (so that two waves share it), a team of DS = 2 or 4 waves shares 32 own rows, each contracting (scores) and accumulating
 // (reductions) its part of d; the partial scores meet in LDS.

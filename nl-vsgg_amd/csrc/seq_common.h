@@ -64,7 +64,8 @@ __device__ __forceinline__ void seq_store16(char* p, seq_u32x4 r, int valid, int
   }
 }
 
-// fp32 <-> the stored type; rounding to bfloat16 is to nearest, ties to even (half a step: 2^-9 of the value's binade)
+// fp32 <-> the stored type; rounding to bfloat16 is to nearest, ties to even (half a step: 2^-8 of the
+// value at most)
 template <class T> struct SeqElt;
 template <> struct SeqElt<float> {
   static constexpr int kPer16 = 4;

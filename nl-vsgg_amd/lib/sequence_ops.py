@@ -11,8 +11,8 @@ float32 or bfloat16 throughout a call (statistics and sums in float32); tensors 
 on the current stream of the tensors' device and may be captured into a graph; nothing is read back.  (As with every torch
 operator: to capture a backward pass, let the results of eager calls on the same leaves go first.)  Bad arguments raise
 ValueError before anything is launched.  Derivatives are reverse-mode and of first order: tensors with a forward-mode tangent are
-refused, and so are calls under a tracer that would record the result's allocation without the kernel.  The last dimension of q / k / v must be contiguous (others are copied), other
-strides are free."""
+refused, and so are calls under a tracer that would record the result's allocation without the kernel.  The last dimension of
+q / k / v must be contiguous (others are copied), other strides are free."""
 from __future__ import annotations
 
 import ctypes as C
@@ -201,7 +201,10 @@ def packed_attention(q, k, v, seq_off, key_off=None, *, causal=False, prefix_len
     Rows that see no key, and rows outside every sequence, come out as zeros (and get zero gradients).  Offsets must ascend within
     the tensors' rows; they live on the device and are not checked (wrong ones give wrong rows, never an access out of bounds).
     Values under a mask do not reach a result, infinities and NaN included (a call that meets them is slow).  Gradients are the
-    same in every run."""
+    same in every run.  In bfloat16, probabilities and their derivatives are rounded to 8 bits on their way into the products
+    where sequences are long, and carry 16 where they are short (below 64 rows in the forward pass, 512 in the backward), by the
+    average over the call: a short sequence answers a little less exactly beside long ones (up to 1.5 times its result's own
+    rounding) than by itself."""
     name = "packed_attention"
     _checked(name, q, k, v)
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
