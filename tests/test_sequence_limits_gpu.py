@@ -86,6 +86,7 @@ def test_attention_gradients_of_the_most_rows(ops, dtype, d, rows):
     """a row for each of more lanes than a launch has threads: queries and gradient broadcast over the rows, the last 50 see 40 keys and
     answer as by themselves (their tiles begin elsewhere: sums in another order, 2^-6 of the largest in bfloat16, 1e-5 in float32)"""
     n, nk, dt = 50, 40, DT[dtype]
+    torch.cuda.empty_cache()
     if torch.cuda.mem_get_info()[0] < 150 << 30:
         pytest.skip("needs 150 GB of device memory")
     q, do, k, v = (_normal(i, m, 1, d, dtype=dt) for i, m in enumerate((1, 1, nk, nk)))
@@ -96,6 +97,8 @@ def test_attention_gradients_of_the_most_rows(ops, dtype, d, rows):
         torch.testing.assert_close(g.float(), w.float(), rtol=rel, atol=rel * w.float().abs().max().item())
     for g in got[:2]:
         assert not g[:rows - n].any()
+    del got, g
+    torch.cuda.empty_cache()                         # tests in processes of their own come behind this one
 
 
 CAPS = [30.0, 1024.0, 1025.0, 1e4, 1e6, 1e9, 1e37]
